@@ -260,6 +260,44 @@ int nmfk_multi_sweep(nmfk_multi *mh, int nk, const int32_t *ks, int nruns, const
                      float *const *H_out, float *const *frob_out, double *const *sse_out, int32_t *const *iters_out,
                      int32_t *const *reason_out);
 
+/* matrix products beside the factorizations ------------------------------------------------------------------- */
+/* Numerics on plain matrices that the reference leaves to other packages: no reference function is replaced here.  They need no context:
+ * every pointer is memory of GPU `device`, the work is put on `stream` (a hipStream_t of that device; NULL = its default stream) and the
+ * call returns without waiting, the thread's current device is left as it was.  The workspace is the caller's: one per call in flight.
+ * No call allocates, copies to the host or keeps anything, so all of them can be captured into a hipGraph. */
+enum { NMFK_F32 = 0, NMFK_BF16 = 1, NMFK_F16 = 2 };  /* types of the matrices that are not in 8 bits */
+
+/* X (rows x cols) in 8-bit floating point, e4m3, with a scale for each block: 128 consecutive entries of a row (tiles = 0) or a 128 x 128
+ * tile (tiles = 1), the last ones shorter.  scale = max(max |x| / 448, 2^-126) over the block's finite entries in fp32; value = x / scale,
+ * rounded to fp32, then to e4m3, both to nearest with ties to even; NaN where x is not finite.
+ *  X          entry (i, j) at X[i * row_stride + j * col_stride]; one of the strides is 1
+ *  values     rows x ldv bytes, entry (i, j) at values[i * ldv + j]; ldv a multiple of 16 that holds whole blocks, which are filled with zeros
+ *  scales     scale of (row i, block b) at scales[b * lds + i], lds >= rows; tiles: of tile (t, b) at scales[b * lds + t]
+ *  tvalues, tscales   the same of the transpose (cols x rows, blocks along ITS rows), from the same pass over X; both NULL = not wanted */
+int nmfk_quantize(int device, void *stream, int dtype, const void *X, int64_t rows, int64_t cols, int64_t row_stride,
+                  int64_t col_stride, int tiles, uint8_t *values, int64_t ldv, float *scales, int64_t lds, uint8_t *tvalues,
+                  int64_t ldtv, float *tscales, int64_t ldts);
+
+/* Y = A * B' (m x n, entry (i, j) at Y[i * ldy + j]) of two matrices in 8 bits, A m x k and B n x k, as nmfk_quantize lays them out:
+ * Y[i, j] = sum over blocks b of sA[i, b] * sB[j, b] * sum of the block's a[i, t] * b[j, t], summed in fp32, rounded once to `dtype`.
+ * k = 0 gives zeros.  The result does not depend on the run (no atomics).  nmfk_product_workspace: bytes of `work` for these sizes. */
+int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int64_t *bytes);
+int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, const uint8_t *A, int64_t lda, const float *sA,
+                 int64_t ldsa, int a_tiles, const uint8_t *B, int64_t ldb, const float *sB, int64_t ldsb, int b_tiles, int dtype,
+                 void *Y, int64_t ldy, void *work, int64_t work_bytes);
+
+/* The orthogonal factor of each of `batch` matrices G (rows x cols) by Newton-Schulz products: X = G / |G|_F, then for every step, with
+ * its three coefficients (a, b, c), X <- a X + (b S + c S S) X where S = X X' (rows <= cols; otherwise of the transpose).  Singular values
+ * go towards one (which ones and how close is the coefficients' doing), singular vectors stay.  Accuracy of fp32 or better inside.
+ * A matrix of zeros gives zeros; one with an entry that is not finite gives NaN everywhere.
+ *  G, O       entry (i, j) of matrix r at G[r * g_batch + i * g_row + j * g_col]; O likewise, not overlapping G
+ *  coefficients   3 * steps doubles on the HOST (1 to 32 steps), read before the call returns; refused when they let a singular value grow beyond 64
+ * The shorter side is at most 32768. */
+int nmfk_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int64_t *bytes);
+int nmfk_orthogonalize(int device, void *stream, int dtype, int64_t batch, int64_t rows, int64_t cols, const void *G,
+                       int64_t g_batch, int64_t g_row, int64_t g_col, void *O, int64_t o_batch, int64_t o_row, int64_t o_col,
+                       int steps, const double *coefficients, void *work, int64_t work_bytes);
+
 /* measurement ----------------------------------------------------------------------------------------------- */
 /* HIP-event timing of the MU kernels on the streams they are launched on (bench.py's roofline leg).
  * After a sweep with profiling enabled: names[i] / total_ms[i] / launches[i] / flops[i] for i < *count:

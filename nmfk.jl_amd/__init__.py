@@ -10,6 +10,8 @@ from ._lib import (COMPUTE_F32, COMPUTE_F64, STOP_CONSISTENCY, STOP_MAXITER, STO
 from .execute import ExecuteOptions, execute, execute_run, getk, input_checks, run_seed, signalorder
 from . import parallel
 from .cluster import robustkmeans, sortclustering
+from .products import Quantized, orthogonalize, product, product_grads, quantize, rangebasis
 
 __all__ = ["ExecuteOptions", "robustkmeans", "sortclustering", "execute", "execute_run", "getk", "signalorder", "input_checks", "run_seed", "Context", "Comm", "Multi", "NMFkError",
-           "build", "lib", "device_count", "default_params", "parallel"]
+           "build", "lib", "device_count", "default_params", "parallel",
+           "Quantized", "quantize", "product", "product_grads", "orthogonalize", "rangebasis"]

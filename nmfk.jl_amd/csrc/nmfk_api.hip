@@ -168,7 +168,7 @@ Tuning read_tuning() {
 
 }  // namespace
 
-NMFK_EXPORT int nmfk_version(void) { return 210; }
+NMFK_EXPORT int nmfk_version(void) { return 220; }
 
 NMFK_EXPORT const char *nmfk_last_error(void) { return nmfk_error_slot().c_str(); }
 

@@ -1,0 +1,628 @@
+// The orthogonal factor of a matrix by Newton-Schulz products:  X = G / |G|_F, then for every step with coefficients (a, b, c)
+//
+//   S = X X',   X <- a X + (b S + c S S) X        (s = the shorter side, l = the longer one; X stands as s x l)
+//
+// which drives every singular value of X towards one and leaves its singular vectors.  Small singular values grow by a in each step, so
+// does a rounding error made early: everything is carried to 32-bit accuracy or better.
+//
+//   s <= 64: the polynomials of all steps are polynomials of the first S.  One pass over G makes S in 64 bits, one workgroup per matrix
+//     iterates on s x s matrices in LDS in 64 bits (S <- P S P, Q <- Q P), a second pass applies Q.  Two reads and a write of G.
+//   s > 64: products on the 16-bit matrix pipes.  An entry x is kept as two fp16 numbers, hi + lo (22 significant bits), scaled by a power of
+//     two that the growth bound of the step allows; a product is hi hi + hi lo + lo hi, summed in 32 bits (what is dropped is 2^-22 of it).
+#include "nmfk_matrix.h"
+
+using namespace nmfk_mat;
+
+namespace {
+
+constexpr int SMALL = 64;
+
+struct Strided {
+  char *p;
+  int64_t batch, row, col;  // strides in entries: row along s, col along l
+};
+
+template <typename T>
+__device__ __forceinline__ float read_at(const Strided &g, int64_t b, int64_t i, int64_t j) {
+  return to_f32(((const T *)g.p)[b * g.batch + i * g.row + j * g.col]);
+}
+template <typename T>
+__device__ __forceinline__ void write_at(const Strided &g, int64_t b, int64_t i, int64_t j, float x) {
+  ((T *)g.p)[b * g.batch + i * g.row + j * g.col] = from_f32<T>(x);
+}
+
+// ---- s <= 64 ---------------------------------------------------------------------------------------------------------------------
+
+struct SmallArgs {
+  Strided g, o;
+  double *part;  // [batch][chunks][s][s]
+  float *q;      // [batch][s][s]
+  int64_t b0;
+  int s, chunks, steps;
+  int64_t l, chunk;  // entries of l per workgroup
+  const double *coef;
+};
+
+struct Coefs {
+  double v[3 * 32];
+};
+
+// partial S over a chunk of l: 64 columns of X at a time in LDS, a pair (i, j) a thread
+template <typename T>
+__global__ __launch_bounds__(256) void small_gram_kernel(SmallArgs a) {
+  __shared__ float x[64][SMALL + 1];
+  const int64_t b = a.b0 + blockIdx.y;
+  const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
+  const int s = a.s, t = threadIdx.x;
+  double acc[SMALL * SMALL / 256];
+#pragma unroll
+  for (int k = 0; k < SMALL * SMALL / 256; ++k) acc[k] = 0;
+  for (int64_t base = l0; base < l1; base += 64) {
+    const int w = (int)min((int64_t)64, l1 - base);
+    for (int e = t; e < 64 * s; e += 256) {  // along whichever side is contiguous
+      const int i = a.g.row == 1 ? e % s : e / 64, j = a.g.row == 1 ? e / s : e % 64;
+      x[j][i] = j < w ? read_at<T>(a.g, b, i, base + j) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < SMALL * SMALL / 256; ++k) {
+      const int e = t + k * 256;
+      if (e < s * s) {
+        const int i = e / s, j = e % s;
+        double v = acc[k];
+        for (int c = 0; c < 64; ++c) v = fma((double)x[c][i], (double)x[c][j], v);
+        acc[k] = v;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < SMALL * SMALL / 256; ++k) {
+    const int e = t + k * 256;
+    if (e < s * s) a.part[((int64_t)blockIdx.y * a.chunks + blockIdx.x) * s * s + e] = acc[k];
+  }
+}
+
+__device__ __forceinline__ double dot_row(const double *x, const double *y, int s, int i, int j) {
+  double v = 0;
+  for (int k = 0; k < s; ++k) v = fma(x[i * s + k], y[k * s + j], v);
+  return v;
+}
+
+// the iteration on s x s matrices: one workgroup per matrix
+__global__ __launch_bounds__(256) void small_iterate_kernel(SmallArgs a, Coefs cf) {
+  extern __shared__ double mats[];
+  const int s = a.s, n = s * s, t = threadIdx.x;
+  double *S = mats, *P = S + n, *Q = P + n, *U = Q + n;
+  const double *part = a.part + (int64_t)blockIdx.x * a.chunks * n;
+  for (int e = t; e < n; e += 256) {
+    double v = 0;
+    for (int c = 0; c < a.chunks; ++c) v += part[(int64_t)c * n + e];
+    S[e] = v;
+    Q[e] = (e / s == e % s) ? 1.0 : 0.0;
+  }
+  __syncthreads();
+  double norm2 = 0;
+  for (int i = 0; i < s; ++i) norm2 += S[i * s + i];
+  __syncthreads();
+  const bool finite = norm2 <= 1.7e308;
+  const double scale = !finite ? __longlong_as_double(0x7ff8000000000000ll) : norm2 > 0 ? 1.0 / norm2 : 0.0;
+  for (int e = t; e < n; e += 256) S[e] *= scale;
+  __syncthreads();
+  for (int k = 0; k < a.steps; ++k) {
+    const double ca = cf.v[3 * k], cb = cf.v[3 * k + 1], cc = cf.v[3 * k + 2];
+    for (int e = t; e < n; e += 256) P[e] = cb * S[e] + cc * dot_row(S, S, s, e / s, e % s) + ((e / s == e % s) ? ca : 0.0);
+    __syncthreads();
+    for (int e = t; e < n; e += 256) U[e] = dot_row(Q, P, s, e / s, e % s);
+    __syncthreads();
+    double *sw = Q;
+    Q = U;
+    U = sw;
+    if (k + 1 < a.steps) {
+      for (int e = t; e < n; e += 256) U[e] = dot_row(S, P, s, e / s, e % s);
+      __syncthreads();
+      for (int e = t; e < n; e += 256) S[e] = dot_row(U, P, s, e / s, e % s);
+      __syncthreads();
+    }
+  }
+  const double inv = !finite ? __longlong_as_double(0x7ff8000000000000ll) : norm2 > 0 ? 1.0 / sqrt(norm2) : 0.0;
+  for (int e = t; e < n; e += 256) a.q[(int64_t)blockIdx.x * n + e] = (float)(Q[e] * inv);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a) {
+  __shared__ float x[64][SMALL + 1], q[SMALL * SMALL], y[64][SMALL + 1];
+  const int64_t b = a.b0 + blockIdx.y;
+  const int s = a.s, t = threadIdx.x;
+  for (int e = t; e < s * s; e += 256) q[e] = a.q[(int64_t)blockIdx.y * s * s + e];
+  const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
+  for (int64_t base = l0; base < l1; base += 64) {
+    const int w = (int)min((int64_t)64, l1 - base);
+    for (int e = t; e < 64 * s; e += 256) {
+      const int i = a.g.row == 1 ? e % s : e / 64, j = a.g.row == 1 ? e / s : e % 64;
+      x[j][i] = j < w ? read_at<T>(a.g, b, i, base + j) : 0.f;
+    }
+    __syncthreads();
+    for (int e = t; e < 64 * s; e += 256) {
+      const int j = e & 63, i = e >> 6;
+      float v = 0.f;
+      for (int k = 0; k < s; ++k) v = fmaf(q[i * s + k], x[j][k], v);
+      y[j][i] = v;
+    }
+    __syncthreads();
+    for (int e = t; e < 64 * s; e += 256) {
+      const int i = a.o.row == 1 ? e % s : e / 64, j = a.o.row == 1 ? e / s : e % 64;
+      if (j < w) write_at<T>(a.o, b, i, base + j, y[j][i]);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- s > 64 ----------------------------------------------------------------------------------------------------------------------
+//
+// A split matrix: rows of 128-byte blocks, a block = the hi parts of 32 consecutive entries, then their lo parts; zeros behind the last entry.
+
+struct Split {
+  char *p;
+  int64_t batch, ld;  // bytes
+};
+
+__device__ __forceinline__ void split4(f32x4 v, f16x4 &hi, f16x4 &lo) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    hi[r] = (_Float16)v[r];
+    lo[r] = (_Float16)(v[r] - (float)hi[r]);
+  }
+}
+// entries col .. col + 3 of a row (col a multiple of 4)
+__device__ __forceinline__ void put4(char *row, int col, f32x4 v) {
+  f16x4 hi, lo;
+  split4(v, hi, lo);
+  char *q = row + (col >> 5) * 128 + (col & 31) * 2;
+  *(f16x4 *)q = hi;
+  *(f16x4 *)(q + 64) = lo;
+}
+__device__ __forceinline__ void put1(char *row, int col, float v) {
+  const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
+  char *q = row + (col >> 5) * 128 + (col & 31) * 2;
+  *(_Float16 *)q = hi;
+  *(_Float16 *)(q + 64) = lo;
+}
+__device__ __forceinline__ f32x4 get4(const char *row, int col) {
+  const char *q = row + (col >> 5) * 128 + (col & 31) * 2;
+  const f16x4 hi = *(const f16x4 *)q, lo = *(const f16x4 *)(q + 64);
+  f32x4 v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = (float)hi[r] + (float)lo[r];
+  return v;
+}
+
+constexpr int NORM_PARTS = 64;
+
+// |G|^2 in 64 bits, NORM_PARTS partial sums per matrix
+template <typename T>
+__global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s, int64_t l, double *part) {
+  const int64_t b = b0 + blockIdx.y;
+  const bool flip = g.row == 1;
+  const int64_t outer = flip ? l : s, inner = flip ? s : l;
+  const int64_t so = flip ? g.col : g.row, si = flip ? g.row : g.col;
+  const T *p = (const T *)g.p + b * g.batch;
+  double v = 0;
+  const int64_t total = outer * inner, per = (total + NORM_PARTS - 1) / NORM_PARTS;
+  const int64_t e0 = blockIdx.x * per, e1 = min(total, e0 + per);
+  for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
+    const int64_t o = e / inner;
+    const double x = to_f32(p[o * so + (e - o * inner) * si]);
+    v = fma(x, x, v);
+  }
+  __shared__ double sum[4];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * NORM_PARTS + blockIdx.x] = ((sum[0] + sum[1]) + sum[2]) + sum[3];
+}
+
+// X = G * (1 / |G|) * 2^e, split, as s x l and as l x s.  A 64 x 64 tile per workgroup, turned in LDS.
+template <typename T>
+__global__ __launch_bounds__(256) void split_kernel(Strided g, int64_t b0, int s, int64_t l, const double *part, double pow2, Split x, Split xt) {
+  __shared__ float tile[64][65];
+  const int t = threadIdx.x;
+  const int64_t b = b0 + blockIdx.z;
+  double norm2 = 0;
+  for (int k = 0; k < NORM_PARTS; ++k) norm2 += part[(int64_t)blockIdx.z * NORM_PARTS + k];
+  const double scale = !(norm2 <= 1.7e308) ? __longlong_as_double(0x7ff8000000000000ll) : norm2 > 0 ? pow2 / sqrt(norm2) : 0.0;
+  const int64_t j0 = (int64_t)blockIdx.x * 64;
+  const int i0 = blockIdx.y * 64;
+  const int64_t lp = (l + 31) & ~(int64_t)31;
+  const int sp = (s + 31) & ~31;
+#pragma unroll 4
+  for (int k = 0; k < 16; ++k) {
+    const int e = t + k * 256, u = e >> 6, v = e & 63;
+    const int i = g.row == 1 ? v : u, j = g.row == 1 ? u : v;
+    tile[i][j] = i0 + i < s && j0 + j < l ? (float)(scale * (double)read_at<T>(g, b, i0 + i, j0 + j)) : 0.f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int e = t + k * 256, u = e >> 4, v = (e & 15) * 4;
+    if (i0 + u < s && j0 + v < lp)
+      put4(x.p + blockIdx.z * x.batch + (i0 + u) * x.ld, (int)(j0 + v), (f32x4){tile[u][v], tile[u][v + 1], tile[u][v + 2], tile[u][v + 3]});
+    if (j0 + u < l && i0 + v < sp)
+      put4(xt.p + blockIdx.z * xt.batch + (j0 + u) * xt.ld, i0 + v, (f32x4){tile[v][u], tile[v + 1][u], tile[v + 2][u], tile[v + 3][u]});
+  }
+}
+
+enum { GRAM = 0, GRAM_PART = 1, POLY = 2, APPLY = 3, LAST = 4 };
+
+struct GemmArgs {
+  Split p, q;    // C[i, j] = sum_k P[i, k] Q[j, k]
+  int m, n, kb;  // kb: blocks of 32
+  float add, mul;  // result = add * D + mul * C
+  Split d;         // POLY: S, APPLY / LAST: X   (entry [i, j])
+  Split out, out_t;  // [i, j] and [j, i]
+  float *part;     // GRAM_PART: [batch][splits][m][m]
+  int kb_split, splits, tiles_n;
+  Strided o;  // LAST
+  int64_t b0;
+  int vec;
+};
+
+// 128 x 128 outputs a workgroup, 64 x 64 a wave; two buffers of 128-byte rows in LDS.  The results of GRAM and POLY are symmetric: only the
+// tiles on and below the diagonal are computed, each is written to both places.
+template <int MODE, typename T>
+__global__ __launch_bounds__(256) void gemm_kernel(GemmArgs a) {
+  constexpr int STAGE = 256 * 128;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+  int ti, tj;
+  constexpr bool SYM = MODE == GRAM || MODE == GRAM_PART || MODE == POLY;
+  if (SYM) {
+    const int id = blockIdx.x;
+    ti = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);
+    while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
+    while (ti * (ti + 1) / 2 > id) --ti;
+    tj = id - ti * (ti + 1) / 2;
+  } else {
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    ti = id / a.tiles_n;
+    tj = id - ti * a.tiles_n;
+  }
+  const int i0 = ti * 128, j0 = tj * 128;
+  const int64_t b = blockIdx.z;
+  const int kb0 = MODE == GRAM_PART ? blockIdx.y * a.kb_split : 0, kb1 = MODE == GRAM_PART ? min(a.kb, kb0 + a.kb_split) : a.kb;
+  const int lr = lane >> 3, lc = ((lane & 7) ^ lr) << 4;
+  const char *src[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int row = (k * 4 + w) * 8;
+    src[k] = row < 128 ? a.p.p + b * a.p.batch + (int64_t)min(i0 + row + lr, a.m - 1) * a.p.ld + lc
+                       : a.q.p + b * a.q.batch + (int64_t)min(j0 + row - 128 + lr, a.n - 1) * a.q.ld + lc;
+  }
+  auto stage = [&](int kb, int buf) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) stage8(src[k] + (int64_t)kb * 128, lds + buf * STAGE + (k * 4 + w) * 1024);
+  };
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (kb0 < kb1) {
+    stage(kb0, 0);
+    staged();
+  }
+  __syncthreads();
+  const int fr = lane & 15, fg = lane >> 4, wi = (w >> 1) * 64, wj = (w & 1) * 64;
+  for (int kb = kb0, buf = 0; kb < kb1; ++kb, buf ^= 1) {
+    if (kb + 1 < kb1) stage(kb + 1, buf ^ 1);
+    const char *lp = lds + buf * STAGE, *lq = lp + 128 * 128;
+    f16x8 qh[4], ql[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      qh[j] = __builtin_bit_cast(f16x8, lds_chunk(lq, wj + j * 16 + fr, fg));
+      ql[j] = __builtin_bit_cast(f16x8, lds_chunk(lq, wj + j * 16 + fr, fg + 4));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f16x8 ph = __builtin_bit_cast(f16x8, lds_chunk(lp, wi + i * 16 + fr, fg));
+      const f16x8 pl = __builtin_bit_cast(f16x8, lds_chunk(lp, wi + i * 16 + fr, fg + 4));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph, acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph, acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl, acc[i][j], 0, 0, 0);
+    }
+    staged();
+    __syncthreads();
+  }
+  const int mp = (a.m + 31) & ~31, np = (a.n + 31) & ~31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = i0 + wi + i * 16 + fr;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = j0 + wj + j * 16 + fg * 4;
+      f32x4 v = acc[i][j];
+      if (MODE == GRAM_PART) {
+        if (m < a.m) {
+          float *q = a.part + ((b * a.splits + blockIdx.y) * a.m + m) * a.m + n;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < a.n) q[r] = v[r];
+        }
+        continue;
+      }
+      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+      if (MODE != GRAM && m < a.m && n < np) d = get4(a.d.p + b * a.d.batch + (int64_t)m * a.d.ld, n);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = m < a.m && n + r < a.n ? fmaf(a.mul, v[r], a.add * d[r]) : 0.f;
+      if (MODE == LAST) {
+        if (m >= a.m || n >= a.n) continue;
+        T *q = (T *)a.o.p + (a.b0 + b) * a.o.batch + m * a.o.row + (int64_t)n * a.o.col;
+        if (a.vec && n + 4 <= a.n) {
+          vec4<T> u;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) u.v[r] = from_f32<T>(v[r]);
+          *(vec4<T> *)q = u;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < a.n) q[r * a.o.col] = from_f32<T>(v[r]);
+        }
+        continue;
+      }
+      if (m < a.m && n < np) put4(a.out.p + b * a.out.batch + (int64_t)m * a.out.ld, n, v);
+      if (SYM && ti == tj) continue;
+      if (m < mp) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < a.n) put1(a.out_t.p + b * a.out_t.batch + (int64_t)(n + r) * a.out_t.ld, m, v[r]);
+      }
+    }
+  }
+}
+
+// sums the partial S of GRAM_PART in the order of the splits
+__global__ __launch_bounds__(256) void gram_join_kernel(GemmArgs a) {
+  const int mp = (a.m + 31) & ~31;
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t b = blockIdx.z;
+  if (e >= (int64_t)a.m * mp) return;
+  const int m = (int)(e / mp), n = (int)(e % mp);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int c = n + r;
+    if (c >= a.m) continue;
+    const bool lower = (m >> 7) >= (c >> 7);
+    const float *q = a.part + b * a.splits * (int64_t)a.m * a.m + (lower ? (int64_t)m * a.m + c : (int64_t)c * a.m + m);
+    float x = 0.f;
+    for (int k = 0; k < a.splits; ++k) x += q[(int64_t)k * a.m * a.m];
+    v[r] = x * a.mul;
+  }
+  put4(a.out.p + b * a.out.batch + (int64_t)m * a.out.ld, n, v);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+
+struct Layout {
+  int64_t s, l, batch;
+  int64_t chunks, chunk;                       // small
+  int64_t x, xt[2], sm, bm, norm, part, q;     // byte offsets
+  int64_t ldx, ldt, splits, kb_split;
+  int64_t bytes;
+};
+
+Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
+  Layout y = {};
+  y.s = std::min(rows, cols);
+  y.l = std::max(rows, cols);
+  y.batch = batch;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += nmfk_round_up(bytes, 256);
+    return o;
+  };
+  if (y.s <= SMALL) {
+    y.chunks = std::max<int64_t>(1, std::min<int64_t>(nmfk_div_up(y.l, 64), nmfk_div_up(1024, batch)));
+    y.chunk = nmfk_round_up(nmfk_div_up(y.l, y.chunks), 64);
+    y.chunks = nmfk_div_up(y.l, y.chunk);
+    y.part = take(batch * y.chunks * y.s * y.s * 8);
+    y.q = take(batch * y.s * y.s * 4);
+  } else {
+    y.ldx = nmfk_round_up(y.l, 32) * 4;
+    y.ldt = nmfk_round_up(y.s, 32) * 4;
+    y.x = take(batch * y.s * y.ldx);
+    y.xt[0] = take(batch * y.l * y.ldt);
+    y.xt[1] = take(batch * y.l * y.ldt);
+    y.sm = take(batch * y.s * y.ldt);
+    y.bm = take(batch * y.s * y.ldt);
+    y.norm = take(batch * NORM_PARTS * 8);
+    const int64_t tm = nmfk_div_up(y.s, 128), tiles = tm * (tm + 1) / 2 * batch, kb = nmfk_div_up(y.l, 32);
+    y.splits = tiles >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / tiles, kb / 8));
+    y.kb_split = nmfk_div_up(kb, y.splits);
+    y.splits = nmfk_div_up(kb, y.kb_split);
+    if (y.splits > 1) y.part = take(batch * y.splits * y.s * y.s * 4);
+  }
+  y.bytes = at;
+  return y;
+}
+
+// the largest |t (a + b t^2 + c t^4)| (odd) or |b t^2 + c t^4| (even) for 0 <= t <= u
+double peak(double a, double b, double c, double u, bool odd) {
+  auto f = [&](double t) { return fabs(odd ? t * (a + t * t * (b + c * t * t)) : t * t * (b + c * t * t)); };
+  double best = f(u);
+  if (odd) {
+    const double disc = 9 * b * b - 20 * a * c;
+    if (c != 0 && disc >= 0)
+      for (int sgn = -1; sgn <= 1; sgn += 2) {
+        const double x = (-3 * b + sgn * sqrt(disc)) / (10 * c);
+        if (x > 0 && x < u * u) best = std::max(best, f(sqrt(x)));
+      }
+    else if (c == 0 && b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < u * u)
+      best = std::max(best, f(sqrt(-a / (3 * b))));
+  } else if (c != 0) {
+    const double x = -b / (2 * c);
+    if (x > 0 && x < u * u) best = std::max(best, f(sqrt(x)));
+  }
+  return best;
+}
+
+// the power of two that brings `bound` to at most 2^15: an entry is never larger than the norm, and 65504 stays out of reach
+int exponent(double bound) {
+  int e;
+  (void)frexp(bound, &e);  // bound < 2^e
+  return std::min(15 - e, 100);
+}
+
+template <typename T>
+int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, const double *coef, char *work, hipStream_t st) {
+  Coefs cf = {};
+  for (int k = 0; k < 3 * steps; ++k) cf.v[k] = coef[k];
+  static std::atomic<uint64_t> done{0};
+  nmfk_allow_dynamic_lds((const void *)small_iterate_kernel, done, 4 * SMALL * SMALL * 8);
+  for (int64_t b0 = 0; b0 < y.batch; b0 += 32768) {
+    const unsigned nb = (unsigned)std::min<int64_t>(32768, y.batch - b0);
+    SmallArgs a = {};
+    a.g = g;
+    a.o = o;
+    a.part = (double *)(work + y.part) + b0 * y.chunks * y.s * y.s;
+    a.q = (float *)(work + y.q) + b0 * y.s * y.s;
+    a.b0 = b0;
+    a.s = (int)y.s;
+    a.chunks = (int)y.chunks;
+    a.steps = steps;
+    a.l = y.l;
+    a.chunk = y.chunk;
+    small_gram_kernel<T><<<dim3((unsigned)y.chunks, nb), 256, 0, st>>>(a);
+    small_iterate_kernel<<<dim3(nb), 256, 4 * y.s * y.s * 8, st>>>(a, cf);
+    small_apply_kernel<T><<<dim3((unsigned)y.chunks, nb), 256, 0, st>>>(a);
+  }
+  return nmfk_launched("nmfk_orthogonalize");
+}
+
+template <int MODE, typename T>
+void gemm(const GemmArgs &a, dim3 grid, hipStream_t st) {
+  constexpr int BYTES = 2 * 256 * 128;
+  static std::atomic<uint64_t> done{0};
+  nmfk_allow_dynamic_lds((const void *)gemm_kernel<MODE, T>, done, BYTES);
+  gemm_kernel<MODE, T><<<grid, 256, BYTES, st>>>(a);
+}
+
+template <typename T>
+int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, const double *coef, char *work, hipStream_t st) {
+  const int s = (int)y.s, l = (int)y.l;
+  const unsigned tm = (unsigned)nmfk_div_up(s, 128), tl = (unsigned)nmfk_div_up(l, 128), sym = tm * (tm + 1) / 2;
+  const int64_t bx = y.s * y.ldx, bt = y.l * y.ldt, bs = y.s * y.ldt;
+  for (int64_t b0 = 0; b0 < y.batch; b0 += 32768) {
+    const unsigned nb = (unsigned)std::min<int64_t>(32768, y.batch - b0);
+    Split X = {work + y.x + b0 * bx, bx, y.ldx}, XT = {work + y.xt[0] + b0 * bt, bt, y.ldt}, NT = {work + y.xt[1] + b0 * bt, bt, y.ldt};
+    Split S = {work + y.sm + b0 * bs, bs, y.ldt}, B = {work + y.bm + b0 * bs, bs, y.ldt};
+    double *norm = (double *)(work + y.norm) + b0 * NORM_PARTS;
+    double u = 1.0;
+    int ex = exponent(1.01 * u);
+    norm_kernel<T><<<dim3(NORM_PARTS, nb), 256, 0, st>>>(g, b0, s, l, norm);
+    split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, ldexp(1.0, ex), X, XT);
+    for (int k = 0; k < steps; ++k) {
+      const double ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
+      const int es = exponent(1.02 * u * u), eb = exponent(1.02 * std::max(peak(ca, cb, cc, u, false), 1e-3));
+      GemmArgs a = {};
+      a.p = a.q = X;
+      a.m = a.n = s;
+      a.kb = (int)nmfk_div_up(l, 32);
+      a.mul = (float)ldexp(1.0, es - 2 * ex);
+      a.out = a.out_t = S;
+      a.tiles_n = (int)tm;
+      a.splits = (int)y.splits;
+      a.kb_split = (int)y.kb_split;
+      if (y.splits > 1) {
+        a.part = (float *)(work + y.part) + b0 * y.splits * y.s * y.s;
+        gemm<GRAM_PART, T>(a, dim3(sym, (unsigned)y.splits, nb), st);
+        gram_join_kernel<<<dim3((unsigned)nmfk_div_up((int64_t)s * (y.ldt / 4), 1024), 1, nb), 256, 0, st>>>(a);
+      } else {
+        gemm<GRAM, T>(a, dim3(sym, 1, nb), st);
+      }
+      a.p = a.q = a.d = S;
+      a.kb = (int)nmfk_div_up(s, 32);
+      a.add = (float)(cb * ldexp(1.0, eb - es));
+      a.mul = (float)(cc * ldexp(1.0, eb - 2 * es));
+      a.out = a.out_t = B;
+      gemm<POLY, T>(a, dim3(sym, 1, nb), st);
+      u = std::max(peak(ca, cb, cc, u, true), 1e-3);
+      const bool last = k + 1 == steps;
+      const int nx = last ? 0 : exponent(1.02 * u);
+      a.p = B;
+      a.q = XT;
+      a.d = X;
+      a.n = l;
+      a.tiles_n = (int)tl;
+      a.add = (float)(ca * ldexp(1.0, nx - ex));
+      a.mul = (float)ldexp(1.0, nx - eb - ex);
+      a.out = X;  // the entry [i, j] of X is read by the lane that overwrites it, and by no other
+      a.out_t = NT;
+      if (last) {
+        a.o = o;
+        a.b0 = b0;
+        a.vec = o.col == 1 && o.row % 4 == 0 && o.batch % 4 == 0 && (uintptr_t)o.p % (4 * sizeof(T)) == 0;
+        gemm<LAST, T>(a, dim3(tm * tl, 1, nb), st);
+      } else {
+        gemm<APPLY, T>(a, dim3(tm * tl, 1, nb), st);
+      }
+      std::swap(XT, NT);
+      ex = nx;
+    }
+  }
+  return nmfk_launched("nmfk_orthogonalize");
+}
+
+int ortho_sizes(int64_t batch, int64_t rows, int64_t cols, const char *who) {
+  if (batch < 0 || rows < 0 || cols < 0) return fail(NMFK_ERR_BAD_ARG, std::string(who) + ": negative size");
+  if (batch > ((int64_t)1 << 22) || std::max(rows, cols) > ((int64_t)1 << 22)) return fail(NMFK_ERR_UNSUPPORTED, std::string(who) + ": a size above 2^22");
+  if (std::min(rows, cols) > 32768) return fail(NMFK_ERR_UNSUPPORTED, std::string(who) + ": both sides above 32768");
+  return NMFK_OK;
+}
+
+}  // namespace
+
+NMFK_EXPORT int nmfk_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int64_t *bytes) {
+  if (!bytes) return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize_workspace: null pointer");
+  if (int rc = ortho_sizes(batch, rows, cols, "nmfk_orthogonalize_workspace")) return rc;
+  *bytes = batch && rows && cols ? ortho_layout(batch, rows, cols).bytes : 0;
+  return NMFK_OK;
+}
+
+NMFK_EXPORT int nmfk_orthogonalize(int device, void *stream, int dtype, int64_t batch, int64_t rows, int64_t cols, const void *G,
+                                   int64_t g_batch, int64_t g_row, int64_t g_col, void *O, int64_t o_batch, int64_t o_row, int64_t o_col,
+                                   int steps, const double *coefficients, void *work, int64_t work_bytes) {
+  if (int rc = ortho_sizes(batch, rows, cols, "nmfk_orthogonalize")) return rc;
+  if (dtype < NMFK_F32 || dtype > NMFK_F16) return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize: dtype must be NMFK_F32, NMFK_BF16 or NMFK_F16");
+  if (steps < 1 || steps > 32) return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize: 1 to 32 steps");
+  if (!coefficients) return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize: null pointer");
+  double u = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    const double *c = coefficients + 3 * k;
+    if (!(fabs(c[0]) <= 1e3 && fabs(c[1]) <= 1e3 && fabs(c[2]) <= 1e3)) return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize: a coefficient is not finite or above 1000");
+    u = peak(c[0], c[1], c[2], u, true);
+    if (u > 64.0) return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize: these coefficients let a singular value grow beyond 64");
+  }
+  if (batch == 0 || rows == 0 || cols == 0) return NMFK_OK;
+  if (!G || !O) return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize: null pointer");
+  const Layout y = ortho_layout(batch, rows, cols);
+  if (!work || work_bytes < y.bytes || (uintptr_t)work % 256)
+    return fail(NMFK_ERR_BAD_ARG, "nmfk_orthogonalize: the workspace is too small or not 256-byte aligned (nmfk_orthogonalize_workspace)");
+  NmfkDeviceGuard guard(device);
+  if (guard.status) return guard.status;
+  const bool flip = rows > cols;
+  const Strided g = {(char *)G, g_batch, flip ? g_col : g_row, flip ? g_row : g_col};
+  const Strided o = {(char *)O, o_batch, flip ? o_col : o_row, flip ? o_row : o_col};
+  hipStream_t st = (hipStream_t)stream;
+  const bool small = y.s <= SMALL;
+#define NMFK_ORTHO(T) (small ? ortho_small<T>(y, g, o, steps, coefficients, (char *)work, st) : ortho_large<T>(y, g, o, steps, coefficients, (char *)work, st))
+  if (dtype == NMFK_F32) return NMFK_ORTHO(float);
+  if (dtype == NMFK_BF16) return NMFK_ORTHO(bf16);
+  return NMFK_ORTHO(_Float16);
+#undef NMFK_ORTHO
+}

@@ -1,0 +1,219 @@
+// Matrices in 8-bit floating point (e4m3) with a scale for each block of 128 entries of a row, or for each 128 x 128 tile.
+//
+//   scale = max(max |x| / 448, 2^-126)   over the finite entries of the block, in 32 bits
+//   value = e4m3(x / scale)              the quotient rounded to 32 bits, then to e4m3, ties to even; NaN where x is not finite
+//
+// What bounds it: memory.  An fp32 matrix in both orientations is 4 bytes read and 2 written for each entry, so the entries are read ONCE:
+// a workgroup holds a 128 x 128 tile in registers, has the maxima of its rows, of its columns and of the whole, and writes the tile and
+// its transpose (the latter turned in LDS, so that whole 128-byte lines leave).
+#include "nmfk_matrix.h"
+
+using namespace nmfk_mat;
+
+namespace {
+
+struct QuantArgs {
+  const void *x;  // entry (r, c) at x[r * ld + c]
+  int64_t rows, cols, ld;
+  uint8_t *v;  // [rows][ldv], or null
+  int64_t ldv;
+  float *s;  // [blocks of a row][sld]: sld >= rows (blocks of rows) or blocks of rows (tiles)
+  int64_t sld;
+  uint8_t *tv;  // the transpose: [cols][ldtv], or null
+  int64_t ldtv;
+  float *ts;
+  int64_t tsld;
+  int vec;  // four entries may be loaded at once
+};
+
+__device__ __forceinline__ float block_scale(float top) { return fmaxf(top / 448.0f, 1.17549435e-38f); }
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;
+}
+__device__ __forceinline__ float quotient(float x, float s) {
+  return fabsf(x) <= 3.402823466e38f ? x / s : __uint_as_float(0x7fc00000u);
+}
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+template <typename T>
+__device__ __forceinline__ void load4(const QuantArgs &a, int64_t r, int64_t c, float out[4]) {
+  const T *p = (const T *)a.x + r * a.ld + c;
+  if (r < a.rows && c + 4 <= a.cols && a.vec) {
+    const vec4<T> q = *(const vec4<T> *)p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = to_f32(q.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = r < a.rows && c + j < a.cols ? to_f32(p[j]) : 0.f;
+  }
+}
+
+// blocks of rows, one orientation: a half wave per block, four entries a lane
+template <typename T>
+__global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a, int64_t blocks, int64_t per_row) {
+  const int64_t b = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (b >= blocks) return;
+  const int64_t r = b / per_row, kb = b - r * per_row;
+  const int64_t c = kb * 128 + (threadIdx.x & 31) * 4;
+  float x[4];
+  load4<T>(a, r, c, x);
+  float top = fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float s = block_scale(top);
+  *(uint32_t *)(a.v + r * a.ldv + c) = pack4(quotient(x[0], s), quotient(x[1], s), quotient(x[2], s), quotient(x[3], s));
+  if ((threadIdx.x & 31) == 0) a.s[kb * a.sld + r] = s;
+}
+
+// A 128 x 128 tile per workgroup of 256: lane group g = thread / 32 owns the rows 16 g .. 16 g + 15, thread % 32 four columns.
+template <typename T, bool TILES>
+__global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
+  __shared__ __attribute__((aligned(16))) char turn[128 * 128];
+  __shared__ float ctop[8][128];
+  const int t = threadIdx.x, g = t >> 5, cg = t & 31;
+  const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
+  float x[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) load4<T>(a, r0 + g * 16 + i, c0 + cg * 4, x[i]);
+  float cmax[4] = {0.f, 0.f, 0.f, 0.f};
+  float rmax[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = finite_abs(x[i][j]);
+      m = fmaxf(m, f);
+      cmax[j] = fmaxf(cmax[j], f);
+    }
+    rmax[i] = m;
+  }
+  float tile_s = 1.f;
+  if (TILES || a.tv) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ctop[g][cg * 4 + j] = cmax[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 8; ++h) cmax[j] = fmaxf(cmax[j], ctop[h][cg * 4 + j]);
+  }
+  if (TILES) {
+    float m = fmaxf(fmaxf(cmax[0], cmax[1]), fmaxf(cmax[2], cmax[3]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    tile_s = block_scale(m);
+    if (t == 0) {
+      if (a.v) a.s[(int64_t)blockIdx.x * a.sld + blockIdx.y] = tile_s;
+      if (a.tv) a.ts[(int64_t)blockIdx.y * a.tsld + blockIdx.x] = tile_s;
+    }
+  }
+  uint32_t q[16];  // TILES: the values serve both orientations
+  if (a.v || TILES) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = tile_s;
+      if (!TILES) {
+        float m = rmax[i];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        s = block_scale(m);
+      }
+      q[i] = pack4(quotient(x[i][0], s), quotient(x[i][1], s), quotient(x[i][2], s), quotient(x[i][3], s));
+      const int64_t r = r0 + g * 16 + i;
+      if (a.v && r < a.rows) {
+        *(uint32_t *)(a.v + r * a.ldv + c0 + cg * 4) = q[i];
+        if (!TILES && cg == 0) a.s[(int64_t)blockIdx.x * a.sld + r] = s;
+      }
+    }
+  }
+  if (!a.tv) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = cg * 4 + j;
+    i32x4 w;
+    if (TILES) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t o = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o |= ((q[k * 4 + i] >> (8 * j)) & 255u) << (8 * i);
+        w[k] = (int)o;
+      }
+    } else {
+      const float s = block_scale(cmax[j]);
+      if (g == 0 && c0 + c < a.cols) a.ts[(int64_t)blockIdx.y * a.tsld + c0 + c] = s;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = (int)pack4(quotient(x[k * 4][j], s), quotient(x[k * 4 + 1][j], s), quotient(x[k * 4 + 2][j], s), quotient(x[k * 4 + 3][j], s));
+    }
+    *(i32x4 *)(turn + c * 128 + ((g ^ (cg & 7)) << 4)) = w;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = i * 32 + (t >> 3), slot = t & 7;
+    if (c0 + c < a.cols)
+      *(i32x4 *)(a.tv + (c0 + c) * a.ldtv + r0 + slot * 16) = *(const i32x4 *)(turn + c * 128 + ((slot ^ ((c >> 2) & 7)) << 4));
+  }
+}
+
+template <typename T>
+void quant_launch(const QuantArgs &a, bool tiles, hipStream_t st) {
+  const int64_t kb = nmfk_div_up(a.cols, 128), rb = nmfk_div_up(a.rows, 128);
+  if (!tiles && !a.tv) {
+    const int64_t blocks = a.rows * kb;
+    quant_rows_kernel<T><<<dim3((unsigned)nmfk_div_up(blocks, 8)), 256, 0, st>>>(a, blocks, kb);
+  } else if (tiles) {
+    quant_tile_kernel<T, true><<<dim3((unsigned)kb, (unsigned)rb), 256, 0, st>>>(a);
+  } else {
+    quant_tile_kernel<T, false><<<dim3((unsigned)kb, (unsigned)rb), 256, 0, st>>>(a);
+  }
+}
+
+bool aligned16(const void *p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 15) == 0; }
+
+}  // namespace
+
+NMFK_EXPORT int nmfk_quantize(int device, void *stream, int dtype, const void *X, int64_t rows, int64_t cols, int64_t row_stride,
+                              int64_t col_stride, int tiles, uint8_t *values, int64_t ldv, float *scales, int64_t lds, uint8_t *tvalues,
+                              int64_t ldtv, float *tscales, int64_t ldts) {
+  if (rows < 0 || cols < 0) return fail(NMFK_ERR_BAD_ARG, "nmfk_quantize: negative size");
+  if (dtype < NMFK_F32 || dtype > NMFK_F16) return fail(NMFK_ERR_BAD_ARG, "nmfk_quantize: dtype must be NMFK_F32, NMFK_BF16 or NMFK_F16");
+  if (rows > ((int64_t)1 << 22) || cols > ((int64_t)1 << 22)) return fail(NMFK_ERR_UNSUPPORTED, "nmfk_quantize: more than 2^22 rows or columns");
+  if (rows == 0 || cols == 0) return NMFK_OK;
+  const int64_t kb = nmfk_div_up(cols, 128), rb = nmfk_div_up(rows, 128);
+  if (!X || !values || !scales || (tvalues != nullptr) != (tscales != nullptr))
+    return fail(NMFK_ERR_BAD_ARG, "nmfk_quantize: X, values and scales are needed, tvalues and tscales both or neither");
+  if (!(col_stride == 1 && (row_stride >= cols || rows == 1)) && !(row_stride == 1 && (col_stride >= rows || cols == 1)))
+    return fail(NMFK_ERR_BAD_ARG, "nmfk_quantize: the entries of a row or those of a column must be contiguous");
+  if (!aligned16(values, ldv) || ldv < kb * 128 || lds < (tiles ? rb : rows))
+    return fail(NMFK_ERR_BAD_ARG, "nmfk_quantize: values must be 16-byte aligned with ldv a multiple of 16 that holds whole blocks of 128; lds is too small");
+  if (tvalues && (!aligned16(tvalues, ldtv) || ldtv < rb * 128 || ldts < (tiles ? kb : cols)))
+    return fail(NMFK_ERR_BAD_ARG, "nmfk_quantize: tvalues must be 16-byte aligned with ldtv a multiple of 16 that holds whole blocks of 128; ldts is too small");
+  NmfkDeviceGuard guard(device);
+  if (guard.status) return guard.status;
+  // the kernels walk the matrix as it stands in memory: if its columns are contiguous they see the transpose, and the outputs change places
+  QuantArgs a;
+  const bool as_is = col_stride == 1 && (row_stride >= cols || rows == 1);
+  a.x = X;
+  if (as_is)
+    a = {X, rows, cols, rows == 1 ? cols : row_stride, values, ldv, scales, lds, tvalues, ldtv, tscales, ldts, 0};
+  else
+    a = {X, cols, rows, cols == 1 ? rows : col_stride, tvalues, ldtv, tscales, ldts, values, ldv, scales, lds, 0};
+  const int64_t size = nmfk_type_size(dtype);
+  a.vec = ((uintptr_t)X % (4 * size)) == 0 && (a.ld % 4) == 0;
+  if (nmfk_div_up(a.rows, 128) > 65535) return fail(NMFK_ERR_UNSUPPORTED, "nmfk_quantize: too many rows");
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == NMFK_F32)
+    quant_launch<float>(a, tiles != 0, st);
+  else if (dtype == NMFK_BF16)
+    quant_launch<bf16>(a, tiles != 0, st);
+  else
+    quant_launch<_Float16>(a, tiles != 0, st);
+  return nmfk_launched("nmfk_quantize");
+}

@@ -1,0 +1,253 @@
+"""Matrix products beside the factorizations: matrices in 8-bit floating point with a scale for each block of 128 (`quantize`, `product`,
+`product_grads`), the orthogonal factor of a matrix by Newton-Schulz products (`orthogonalize`), and what the two are for next to a sweep:
+`rangebasis`, an orthonormal basis of the leading directions of a large X.  The reference leaves such numerics to other packages.
+
+The operators take and return torch tensors on the GPU; they run on torch's current stream of the tensors' device, do not wait, and can be
+captured into a graph.  `rangebasis` takes a numpy array like `execute` does, or a tensor."""
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from ._lib import ERR_BAD_ARG, NMFkError, _check
+
+# (a, b, c) of X <- a X + (b S + c S S) X: steep at zero (a singular value grows 3.4445-fold a step), every singular value from about 0.003
+# to 1 is between 0.68 and 1.13 after five steps
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+# three more of the steps that converge (error^3 in each) make the columns orthonormal to 32 bits
+CONVERGING = (1.875, -1.25, 0.375)
+
+_TYPES = None
+
+
+def _torch():
+    global _TYPES
+    import torch
+
+    if _TYPES is None:
+        _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    return torch
+
+
+def _bad(msg):
+    return NMFkError(ERR_BAD_ARG, msg)
+
+
+def _tensor(x, name, ndim=2):
+    torch = _torch()
+    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+        raise _bad(f"{name} must be a torch tensor on the GPU")
+    if x.dtype not in _TYPES:
+        raise _bad(f"{name} must be float32, bfloat16 or float16, not {x.dtype}")
+    if x.dim() < ndim or (ndim == 2 and x.dim() != 2):
+        raise _bad(f"{name} must be a matrix")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise _bad(f"{name} requires a gradient, which this operator does not record: pass {name}.detach()")
+    return x
+
+
+def _stream(device):
+    return _torch().cuda.current_stream(device).cuda_stream
+
+
+class Quantized:
+    """A matrix in 8-bit floating point (e4m3) with a scale for each block of 128 entries of a row, or for each 128 x 128 tile.
+
+    values   float8_e4m3fn (rows, cols)
+    scales   float32 (rows, ceil(cols / 128)), tiles: (ceil(rows / 128), ceil(cols / 128))
+    The matrix is values * scales.  Quantized(values, scales, tiles) takes a matrix quantized elsewhere and lays it out once."""
+
+    __slots__ = ("shape", "tiles", "_v", "_s", "__weakref__")
+
+    def __init__(self, values, scales, tiles=False):
+        torch = _torch()
+        if not (isinstance(values, torch.Tensor) and isinstance(scales, torch.Tensor)) or values.device.type != "cuda" or scales.device != values.device:
+            raise _bad("values and scales must be torch tensors on one GPU")
+        if values.dtype not in (torch.float8_e4m3fn, torch.uint8) or values.dim() != 2 or scales.dtype != torch.float32:
+            raise _bad("values must be a float8_e4m3fn matrix and scales float32")
+        r, c = values.shape
+        kb = -(-c // 128)
+        if tuple(scales.shape) != ((-(-r // 128) if tiles else r), kb):
+            raise _bad(f"{'tiles' if tiles else 'rows'} of a {r} x {c} matrix have {(-(-r // 128) if tiles else r)} x {kb} scales, not {tuple(scales.shape)}")
+        self._make(r, c, bool(tiles), values.device)
+        self._v[:, :c].copy_(values.view(torch.uint8))
+        if c < self._v.shape[1]:
+            self._v[:, c:].zero_()
+        self._s.copy_(scales.t())
+
+    def _make(self, r, c, tiles, device):
+        torch = _torch()
+        kb = -(-c // 128)
+        self.shape, self.tiles = (r, c), tiles
+        self._v = torch.empty((r, kb * 128), dtype=torch.uint8, device=device)
+        self._s = torch.empty((kb, -(-r // 128) if tiles else r), dtype=torch.float32, device=device)
+        return self
+
+    @property
+    def values(self):
+        return self._v.view(_torch().float8_e4m3fn)[:, : self.shape[1]]
+
+    @property
+    def scales(self):
+        return self._s.t()
+
+    @property
+    def device(self):
+        return self._v.device
+
+    def dequantize(self, dtype=None):
+        """the matrix that values and scales stand for (float32 unless told otherwise)"""
+        torch = _torch()
+        s = self._s.t().repeat_interleave(128, 1)[:, : self.shape[1]]
+        if self.tiles:
+            s = s.repeat_interleave(128, 0)[: self.shape[0]]
+        return (self.values.float() * s).to(dtype or torch.float32)
+
+
+def quantize(X, tiles=False, both=False):
+    """X (a matrix of float32, bfloat16 or float16) in 8 bits with a scale for each block of 128 entries of a row, or (tiles) for each
+    128 x 128 tile.  scale = max(max |x| / 448, 2^-126) over the block's finite entries, value = x / scale rounded to e4m3, ties to even; an
+    entry that is not finite becomes NaN and leaves its block alone.
+    both=True: a pair, X and its transpose (blocks along ITS rows), from one pass over X."""
+    _tensor(X, "X")
+    r, c = X.shape
+    sr, sc = X.stride()
+    if not (sc == 1 and (sr >= c or r == 1)) and not (sr == 1 and (sc >= r or c == 1)):
+        X = X.contiguous()
+        sr, sc = X.stride()
+    q = Quantized.__new__(Quantized)._make(r, c, bool(tiles), X.device)
+    t = Quantized.__new__(Quantized)._make(c, r, bool(tiles), X.device) if both else None
+    _check(_lib.lib().nmfk_quantize(X.device.index, _stream(X.device), _TYPES[X.dtype], X.data_ptr(), r, c, sr, sc, int(q.tiles),
+                                    q._v.data_ptr(), q._v.shape[1], q._s.data_ptr(), q._s.shape[1],
+                                    t._v.data_ptr() if both else None, t._v.shape[1] if both else 0,
+                                    t._s.data_ptr() if both else None, t._s.shape[1] if both else 0))
+    return (q, t) if both else q
+
+
+def _quantized(x, name):
+    if not isinstance(x, Quantized):
+        raise _bad(f"{name} must be a Quantized matrix (quantize)")
+    return x
+
+
+def product(A, B, dtype=None, out=None):
+    """A * B' of two Quantized matrices (m x k and n x k), summed in 32 bits and rounded once to dtype (float32, bfloat16 or float16).
+    out: the m x n tensor to write, rows contiguous."""
+    torch = _torch()
+    _quantized(A, "A")
+    _quantized(B, "B")
+    if A.shape[1] != B.shape[1] or A.device != B.device:
+        raise _bad(f"A * B' needs rows of one length on one GPU, not {A.shape} on {A.device} and {B.shape} on {B.device}")
+    (m, k), n, dev = A.shape, B.shape[0], A.device
+    if out is None:
+        dtype = dtype or torch.float32
+        if dtype not in _TYPES:
+            raise _bad(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+    else:
+        _tensor(out, "out")
+        if tuple(out.shape) != (m, n) or out.device != dev or (dtype is not None and out.dtype != dtype) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+            raise _bad(f"out must be {m} x {n} on {dev} with contiguous rows")
+    L = _lib.lib()
+    nb = C.c_int64()
+    _check(L.nmfk_product_workspace(m, n, k, C.byref(nb)))
+    work = torch.empty(nb.value, dtype=torch.uint8, device=dev) if nb.value else None
+    _check(L.nmfk_product(dev.index, _stream(dev), m, n, k, A._v.data_ptr(), A._v.shape[1], A._s.data_ptr(), A._s.shape[1], int(A.tiles),
+                          B._v.data_ptr(), B._v.shape[1], B._s.data_ptr(), B._s.shape[1], int(B.tiles), _TYPES[out.dtype],
+                          out.data_ptr(), out.stride(0) if m > 1 else n, work.data_ptr() if work is not None else None, nb.value))
+    return out
+
+
+def product_grads(dY, At, Bt, dtype=None):
+    """The backward pass of Y = product(A, B): (dA, dB) = (dY * B, dY' * A), both products in 8 bits.  dY and its transpose are quantized by
+    rows; At and Bt are the Quantized transposes of A and of B (quantize(..., both=True) leaves them beside the forward's).  The gradients are
+    those with respect to the matrices that the 8 bits stand for."""
+    _tensor(dY, "dY")
+    _quantized(At, "At")
+    _quantized(Bt, "Bt")
+    m, n = dY.shape
+    if At.shape[1] != m or Bt.shape[1] != n or At.shape[0] != Bt.shape[0] or At.device != dY.device or Bt.device != dY.device:
+        raise _bad(f"dY {m} x {n} needs At k x {m} and Bt k x {n} on its GPU, not {At.shape} on {At.device} and {Bt.shape} on {Bt.device}")
+    dtype = dtype or dY.dtype
+    q, t = quantize(dY, both=True)
+    return product(q, Bt, dtype), product(t, At, dtype)
+
+
+def orthogonalize(G, steps=5, coefficients=None, out=None):
+    """The orthogonal factor of G (..., rows, cols), or of each matrix of a stack, by Newton-Schulz products: X = G / |G|_F, then `steps`
+    times X <- a X + (b S + c S S) X, S = X X' (of the transpose where rows > cols).  coefficients: (a, b, c), or one such triple per step.
+    The default five steps bring every singular value from about 0.003 |G|_F upwards to between 0.68 and 1.13, which is what an update wants;
+    for orthonormal rows or columns add steps with (1.875, -1.25, 0.375).  Sums in 32 bits or more, one rounding to G's type.
+    Zeros give zeros, an entry that is not finite gives NaN in its matrix."""
+    torch = _torch()
+    _tensor(G, "G", ndim=0)
+    if G.dim() < 2:
+        raise _bad("G must be a matrix or a stack of matrices")
+    steps = int(steps)
+    if steps < 1 or steps > 32:
+        raise _bad("1 to 32 steps")
+    cf = np.asarray(COEFFICIENTS if coefficients is None else coefficients, dtype=np.float64)
+    if cf.shape == (3,):
+        cf = np.broadcast_to(cf, (steps, 3))
+    if cf.shape != (steps, 3):
+        raise _bad(f"coefficients must be (a, b, c) or {steps} such triples")
+    cf = np.ascontiguousarray(cf)
+    if out is None:
+        out = torch.empty_like(G)
+    else:
+        _tensor(out, "out", ndim=0)
+        if out.shape != G.shape or out.dtype != G.dtype or out.device != G.device:
+            raise _bad("out must have G's shape, type and GPU")
+    g = G if G.dim() == 3 else G.unsqueeze(0) if G.dim() == 2 else G.reshape(-1, *G.shape[-2:])
+    o = out if out.dim() == 3 else out.unsqueeze(0) if out.dim() == 2 else out.view(-1, *out.shape[-2:])
+    b, r, c = g.shape
+    L = _lib.lib()
+    nb = C.c_int64()
+    _check(L.nmfk_orthogonalize_workspace(b, r, c, C.byref(nb)))
+    work = torch.empty(nb.value, dtype=torch.uint8, device=G.device) if nb.value else None
+    _check(L.nmfk_orthogonalize(G.device.index, _stream(G.device), _TYPES[G.dtype], b, r, c, g.data_ptr(), *g.stride(), o.data_ptr(), *o.stride(),
+                                steps, cf.ctypes.data, work.data_ptr() if work is not None else None, nb.value))
+    return out
+
+
+def rangebasis(X, k, oversample=8, iterations=2, seed=0, device=None):
+    """An orthonormal basis of the k leading directions of X (n x m), by subspace iteration on X in 8 bits: products with X and X', each
+    orthogonalized.  Returns (Q, B, sigma): Q (n x k), B = Q' X (k x m, so X is near Q B), and sigma, the k leading singular values of X as the
+    basis sees them.  Next to a sweep: sigma says where the candidate ranks end, Q and B are X compressed.  X is read once in 32 bits and kept in
+    8, so sigma carries 8-bit noise: of about 3 % of |X| / sqrt(max(n, m)), below which nothing is resolved.
+    X: a numpy array (results are numpy arrays) or a torch tensor on the GPU (results are tensors).  NaN (missing data) is refused."""
+    torch = _torch()
+    host = not isinstance(X, torch.Tensor)
+    if host:
+        X = np.asarray(X)
+        if X.ndim != 2:
+            raise _bad("NMFk analysis can be executed for matrices!")
+        if _lib.device_count() == 0:
+            raise NMFkError(_lib.ERR_NO_DEVICE, "no usable gfx950 device: the library has no CPU fallback")
+        X = torch.from_numpy(np.ascontiguousarray(X, dtype=np.float32)).to(torch.device("cuda", int(device or 0)))
+    _tensor(X, "X")
+    n, m = X.shape
+    k = int(k)
+    if not 1 <= k <= min(n, m):
+        raise _bad(f"k must be between 1 and {min(n, m)}")
+    if not bool(torch.isfinite(X).all()):
+        raise _bad("X must be finite (no missing data)")
+    r = min(k + max(0, int(oversample)), n, m)
+    X8, Xt8 = quantize(X, tiles=True, both=True)
+    g = torch.Generator(device=X.device)
+    g.manual_seed(int(seed))
+    steps = [COEFFICIENTS] * 10 + [CONVERGING] * 4
+
+    def basis(y):
+        return orthogonalize(y, len(steps), steps)
+
+    Q = basis(product(X8, quantize(torch.randn(r, m, generator=g, device=X.device))))
+    for _ in range(int(iterations)):
+        Z = basis(product(Xt8, quantize(Q.t())))
+        Q = basis(product(X8, quantize(Z.t())))
+    B = Q.t() @ X.float()
+    U, sigma, V = torch.linalg.svd(B.double(), full_matrices=False)  # r x m, r small
+    Q = (Q.double() @ U[:, :k]).float()
+    B = (sigma[:k, None] * V[:k]).float()
+    sigma = sigma[:k].float()
+    return tuple(x.cpu().numpy() for x in (Q, B, sigma)) if host else (Q, B, sigma)

@@ -1,0 +1,500 @@
+"""The matrix operators on the GPU against plain implementations in 64 bits.
+
+Tolerances.  u = 2^-24 is half a step of fp32, h(t) half a step of the output's type.
+  quantize: equal.
+  product in fp32: entry (i, j) sums 128 kb terms; the additions inside a block round or truncate (2 u each, 128 of them), the scale is a rounded
+    product (u) and the blocks are added with one rounding each: |error| <= (2 * 128 + kb + 3) u * sum |terms|, a split sum adds the
+    number of splits (<= kb); then one rounding to the type.
+  product in 16 bits: the 8-bit matrix instruction aligns 16 products at a time to the largest of them and cuts off what is more than 13 bits below
+    that (a product 2^14 times smaller than another of its 16 vanishes, one 2^13 times smaller does not): at most 2^-13 of the largest for each, so
+    16 * 2^-13 max|term| <= 2^-9 sum |terms| more.  The cut-off parts have the terms' signs, so over a whole matrix they add up
+    like the terms do and the norm of the error stays below 2^-13 of the norm of the terms' sums (besides the one rounding).
+  orthogonalize, shorter side s <= 64: the s x s factor is made in 64 bits and rounded to fp32 (u), applied in fp32 (s + 1 roundings):
+    |error| <= (s + 3) u * (|Q| |G|)[i, j], Q = the factor with O = Q G.
+  orthogonalize, s > 64: "accuracy of fp32": at most four times the error of the same steps in plain fp32, and at least 2^-22 of the largest entry,
+    which is the split of an entry into two fp16 numbers."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+F8 = torch.float8_e4m3fn
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+CF = (3.4445, -4.7750, 2.0315)
+
+
+@pytest.fixture(scope="module")
+def P():
+    import nmfk_jl_amd
+
+    return nmfk_jl_amd
+
+
+def randn(seed, *shape, t=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g) * torch.exp(torch.randn(*shape[:-1], 1, generator=g))
+    return x.to(t).cuda()
+
+
+# ---- quantize ---------------------------------------------------------------------------------------------------------------
+
+def ref_quantize(x, tiles):
+    """values (uint8 bits of e4m3) and scales on the CPU, block by block"""
+    x = x.detach().cpu().float().numpy()
+    r, c = x.shape
+    br = 128 if tiles else 1
+    v = torch.zeros(r, c, dtype=torch.uint8)
+    s = np.zeros((-(-r // br), -(-c // 128)), np.float32)
+    for b in range(s.shape[1]):
+        for a in range(s.shape[0]):
+            blk = x[a * br:(a + 1) * br, b * 128:(b + 1) * 128]
+            fin = np.abs(blk[np.isfinite(blk)])
+            top = np.float32(fin.max()) if fin.size else np.float32(0)
+            s[a, b] = max(np.float32(top / np.float32(448)), np.float32(2.0 ** -126))
+            with np.errstate(invalid="ignore"):
+                q = np.where(np.isfinite(blk), blk / s[a, b], np.nan).astype(np.float32)
+            v[a * br:(a + 1) * br, b * 128:(b + 1) * 128] = torch.from_numpy(q).to(F8).view(torch.uint8)
+    return v, torch.from_numpy(s)
+
+
+def check_quantized(q, x, tiles):
+    v, s = ref_quantize(x, tiles)
+    assert torch.equal(q.scales.cpu(), s)
+    got, want = q.values.view(torch.uint8).cpu(), v
+    nan = (want & 0x7F) == 0x7F  # a NaN of either sign
+    assert torch.equal((got & 0x7F) == 0x7F, nan)
+    assert torch.equal(torch.where(nan, 0, got), torch.where(nan, 0, want))
+    assert int(q._v[:, q.shape[1]:].sum()) == 0  # whole blocks of 128, filled with zeros
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("r,c", [(1, 1), (1, 129), (3, 127), (128, 128), (129, 260), (70, 1000), (1000, 4), (257, 515)])
+def test_quantize(P, t, tiles, both, r, c):
+    x = randn(r * 1000 + c, r, c, t=TYPES[t])
+    q = P.quantize(x, tiles=tiles, both=both)
+    if both:
+        check_quantized(q[0], x, tiles)
+        check_quantized(q[1], x.t(), tiles)
+    else:
+        check_quantized(q, x, tiles)
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_quantize_strides(P, tiles):
+    x = randn(5, 300, 400)
+    for v in (x.t(), x[3:, 5:390], x[:, 1:].t(), x[::2], x[::2].t(), x[:, ::3], x[7:8, 2:], x[:, 9:10], x[0:1].expand(5, 400)):
+        q, w = P.quantize(v, tiles=tiles, both=True)
+        check_quantized(q, v, tiles)
+        check_quantized(w, v.t(), tiles)
+        check_quantized(P.quantize(v, tiles=tiles), v, tiles)
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_quantize_special_values(P, tiles):
+    x = randn(6, 200, 300)
+    x[3] = 0
+    x[4, :128] = 1e-45  # the smallest subnormal: the scale is held at 2^-126
+    x[5, 7] = float("nan")
+    x[6, 130:140] = float("inf")
+    x[7, 0] = -float("inf")
+    x[8] = float("nan")
+    x[9, 5] = 3.4e38
+    x[10] *= 2.0 ** -120
+    x[11, 0], x[11, 1:128] = 448.0, torch.linspace(-448, 448, 127).cuda()  # scale 1: values on and between e4m3's steps
+    q, w = P.quantize(x, tiles=tiles, both=True)
+    check_quantized(q, x, tiles)
+    check_quantized(w, x.t(), tiles)
+
+
+def test_quantize_ties_go_to_even(P):
+    steps = torch.arange(0, 127, dtype=torch.uint8).view(F8).float()  # every finite non-negative value of e4m3
+    mid = (steps[1:] + steps[:-1]) / 2
+    x = torch.zeros(3, 256)
+    x[0, :127], x[1, :126], x[2, :126] = steps, mid, -mid
+    x[:, 127] = 448.0
+    check_quantized(P.quantize(x.cuda()), x, False)
+
+
+def test_quantize_empty(P):
+    for r, c in ((0, 5), (5, 0), (0, 0)):
+        q, t = P.quantize(torch.empty(r, c, device="cuda"), both=True)
+        assert q.shape == (r, c) and t.shape == (c, r)
+
+
+# ---- product ----------------------------------------------------------------------------------------------------------------
+
+def values64(q):
+    s = q.scales.double()
+    if q.tiles:
+        s = s.repeat_interleave(128, 0)[: q.shape[0]]
+    return q.values.float().double() * s.repeat_interleave(128, 1)[:, : q.shape[1]]
+
+
+def check_product(y, a, b, t):
+    """a, b: the matrices in 64 bits"""
+    kb = -(-a.shape[1] // 128)
+    want, mag = a @ b.t(), a.abs() @ b.abs().t()
+    tol = ((256 + 2 * kb + 3) * 2.0 ** -24 + (2.0 ** -9 if t != torch.float32 else 0)) * mag
+    if t != torch.float32:
+        assert float((y.double() - want).norm()) <= (2.0 ** -13 + HALF[t]) * float(want.norm()) + TINY[t] * want.numel() ** 0.5
+    tol = tol + (want.abs() + tol) * HALF[t] + TINY[t]
+    assert y.dtype == t and y.shape == want.shape
+    err = (y.double() - want).abs()
+    assert bool((err <= tol).all()), f"largest error / tolerance {float((err / tol).max())}"
+
+
+SHAPES = [(1, 1, 1), (1, 64, 128), (16, 16, 129), (17, 130, 500), (1, 4096, 1024), (5, 1000, 2048), (128, 128, 128), (129, 65, 4000), (300, 64, 777), (64, 300, 777),
+          (33, 31, 20000), (257, 511, 640), (1025, 700, 256), (2048, 1, 512), (7, 3, 70000)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("ta,tb", [(False, True), (False, False), (True, True), (True, False)])
+def test_product(P, m, n, k, ta, tb):
+    a, b = P.quantize(randn(m + k, m, k), tiles=ta), P.quantize(randn(n * 3 + k, n, k), tiles=tb)
+    for t in TYPES.values():
+        y = P.product(a, b, dtype=t)
+        check_product(y, values64(a), values64(b), t)
+        assert torch.equal(y, P.product(a, b, dtype=t))  # the same bits again
+
+
+@pytest.mark.parametrize("m,n,k", [(1024, 2048, 1024), (2000, 1500, 1100), (4096, 4096, 256), (40000, 64, 512), (700, 48, 30000)])
+def test_product_larger(P, m, n, k):
+    a, b = P.quantize(randn(1, m, k)), P.quantize(randn(2, n, k), tiles=True)
+    check_product(P.product(a, b, dtype=torch.bfloat16), values64(a), values64(b), torch.bfloat16)
+    check_product(P.product(a, b), values64(a), values64(b), torch.float32)
+
+
+def test_product_out_rows_beside_it_stay(P):
+    a, b = P.quantize(randn(1, 50, 300)), P.quantize(randn(2, 37, 300))
+    big = torch.full((60, 80), 7.0, device="cuda")
+    y = P.product(a, b, out=big[5:55, 3:40])
+    assert y.data_ptr() == big[5:55, 3:40].data_ptr()
+    check_product(y, values64(a), values64(b), torch.float32)
+    big[5:55, 3:40] = 7.0
+    assert bool((big == 7.0).all())
+    for bad in (big[:50, :38], big[:50, :74:2], big[:50, :37].half(), big.t()[:50, :37], torch.empty(50, 37)):
+        with pytest.raises(P.NMFkError):
+            P.product(a, b, dtype=torch.float32, out=bad)
+
+
+def test_product_special(P):
+    x = randn(3, 40, 300)
+    x[3, 200] = float("nan")
+    x[5, 1] = float("inf")
+    x[7] = 0
+    y = P.product(P.quantize(x), P.quantize(randn(4, 30, 300)))
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[[3, 5]] = True
+    assert bool(torch.isnan(y[bad]).all()) and bool(torch.isfinite(y[~bad]).all()) and bool((y[7] == 0).all())
+    e = P.product(P.quantize(torch.empty(4, 0, device="cuda")), P.quantize(torch.empty(6, 0, device="cuda")))
+    assert e.shape == (4, 6) and bool((e == 0).all())
+    assert P.product(P.quantize(torch.empty(0, 9, device="cuda")), P.quantize(randn(1, 6, 9))).shape == (0, 6)
+    with pytest.raises(P.NMFkError):
+        P.product(P.quantize(randn(1, 4, 5)), P.quantize(randn(1, 4, 6)))
+    with pytest.raises(P.NMFkError):
+        P.product(P.quantize(randn(1, 4, 5)), P.quantize(randn(1, 4, 5)), dtype=torch.float64)
+
+
+def test_product_offsets_beyond_32_bits(P):
+    """operands of more than 2^31 bytes and an output of more than 2^31 entries: the far corners are checked"""
+    m, n, k = 70000, 40, 32768  # A: 2.3 GB
+    a = P.quantize(torch.rand(m, k, device="cuda") - 0.5)
+    b = P.quantize(randn(2, n, k))
+    y = P.product(a, b)
+    for rows in (slice(0, 50), slice(m - 300, m)):
+        part = P.Quantized(a.values[rows], a.scales[rows])
+        check_product(y[rows], values64(part), values64(b), torch.float32)
+    del a, b, y
+    a, b = P.quantize(randn(3, 50000, 128)), P.quantize(randn(4, 50000, 128))
+    y = P.product(a, b, dtype=torch.bfloat16)
+    for rows in (slice(0, 10), slice(49990, 50000)):
+        part = P.Quantized(a.values[rows], a.scales[rows])
+        check_product(y[rows], values64(part), values64(b), torch.bfloat16)
+
+
+def test_quantized_from_parts(P):
+    x = randn(9, 200, 333)
+    for tiles in (False, True):
+        q = P.quantize(x, tiles=tiles)
+        p = P.Quantized(q.values.contiguous(), q.scales.contiguous(), tiles=tiles)
+        assert torch.equal(p._v, q._v) and torch.equal(p._s, q._s)
+        assert torch.allclose(q.dequantize(), x, rtol=2.0 ** -4, atol=float(x.abs().max()) * 2.0 ** -9)
+    with pytest.raises(P.NMFkError):
+        P.Quantized(q.values, q.scales, tiles=False)
+    with pytest.raises(P.NMFkError):
+        P.Quantized(q.values.float(), q.scales, tiles=True)
+
+
+# ---- gradients --------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (16, 200, 130), (300, 129, 257), (777, 513, 1111)])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_product_grads(P, m, n, k, t):
+    a, b = randn(1, m, k), randn(2, n, k)
+    dy = randn(3, m, n, t=TYPES[t])
+    (a8, at), (b8, bt) = P.quantize(a, both=True), P.quantize(b, tiles=True, both=True)
+    da, db = P.product_grads(dy, at, bt)
+    q, w = P.quantize(dy), P.quantize(dy.t())
+    check_product(da, values64(q), values64(bt), TYPES[t])
+    check_product(db, values64(w), values64(at), TYPES[t])
+
+
+def test_product_grads_against_differences(P):
+    """The loss sum(dY * product(A, B)) moves with an entry of A as dA says.  A is perturbed where 8 bits can show it: its values times 1 +- 1/2 stay
+    values of e4m3 (a power of two and its neighbours), so that central differences of the linear loss are exact up to fp32 sums."""
+    m, n, k = 40, 30, 256
+    g = torch.Generator().manual_seed(4)
+    pow2 = lambda *s: (2.0 ** torch.randint(-3, 4, s, generator=g) * (torch.randint(0, 2, s, generator=g) * 2 - 1)).cuda()
+    a, b, dy = pow2(m, k), pow2(n, k), pow2(m, n)  # powers of two: exact in 8 bits
+    top = 448.0
+    for x in (a, b, dy):
+        x[:, 0] = top  # every scale along rows is 1
+    at, bt = P.quantize(a.t()), P.quantize(b.t())
+    one = lambda x: P.Quantized(x.to(F8), torch.ones(x.shape[0], -(-x.shape[1] // 128), device="cuda"))
+    at, bt = one(a.t().contiguous()), one(b.t().contiguous())
+    da, db = P.product_grads(dy, at, bt)
+    dyq = values64(P.quantize(dy))
+    for i, j in ((0, 1), (7, 200), (39, 255)):
+        up, down = a.clone(), a.clone()
+        up[i, j] *= 1.5
+        down[i, j] *= 0.5
+        loss = [float((dyq * P.product(one(x), one(b)).double()).sum()) for x in (up, down)]
+        step = float(up[i, j] - down[i, j])
+        mag = float((dyq.abs() * (a.abs().double() @ b.abs().double().t())).sum())
+        assert abs((loss[0] - loss[1]) / step - float(da[i, j])) <= 2 * (256 + 2 * 2 + 3) * 2.0 ** -24 * mag / abs(step)
+
+
+def test_operators_refuse_a_gradient_they_do_not_record(P):
+    x = torch.ones(4, 4, device="cuda", requires_grad=True)
+    for f in (P.quantize, P.orthogonalize):
+        with pytest.raises(P.NMFkError, match="detach"):
+            f(x)
+        with torch.no_grad():
+            f(x)
+    with pytest.raises(P.NMFkError):
+        P.quantize(torch.ones(4, 4, device="cuda", dtype=torch.float64))
+    with pytest.raises(P.NMFkError):
+        P.quantize(torch.ones(4, device="cuda"))
+
+
+# ---- orthogonalize ------------------------------------------------------------------------------------------------------------
+
+def ref_ortho(x, steps, cf, dtype=torch.float64):
+    """(O, Q) of one matrix with rows <= columns; Q the factor with O = Q G"""
+    x = x.to(dtype)
+    n = torch.linalg.matrix_norm(x.double()).to(dtype)
+    q = torch.eye(x.shape[0], dtype=dtype, device=x.device) / n
+    x = x / n
+    for a, b, c in cf:
+        s = x @ x.t()
+        p = b * s + c * (s @ s)
+        x, q = a * x + p @ x, a * q + p @ q
+    return x, q
+
+
+def check_ortho(o, g, steps=5, cf=None):
+    cf = [CF] * steps if cf is None else cf
+    assert o.shape == g.shape and o.dtype == g.dtype
+    gs, os_ = g.reshape(-1, *g.shape[-2:]), o.reshape(-1, *o.shape[-2:])
+    for x, y in zip(gs, os_):
+        if x.shape[0] > x.shape[1]:
+            x, y = x.t(), y.t()
+        want, q = ref_ortho(x, steps, cf)
+        s = x.shape[0]
+        if s <= 64:
+            tol = (s + 3) * 2.0 ** -24 * (q.abs() @ x.double().abs())
+        else:
+            plain = ref_ortho(x.float(), steps, cf, torch.float32)[0].double()
+            tol = torch.full_like(want, max(4 * float((plain - want).abs().max()), 2.0 ** -22 * float(want.abs().max())))
+        tol = tol + (want.abs() + tol) * HALF[g.dtype] + TINY[g.dtype]
+        err = (y.double() - want).abs()
+        assert bool((err <= tol).all()), f"largest error / tolerance {float((err / tol).max())}"
+
+
+SMALL_SHAPES = [(1, 1), (1, 7), (5, 1), (3, 3), (2, 1000), (16, 16), (8192, 16), (17, 300), (31, 33), (64, 64), (64, 65), (500, 64), (33, 5000), (8192, 8)]
+LARGE_SHAPES = [(65, 65), (65, 1000), (100, 66), (128, 128), (129, 300), (1000, 130), (384, 384), (257, 2049), (96, 12000), (640, 520)]
+
+
+@pytest.mark.parametrize("r,c", SMALL_SHAPES + LARGE_SHAPES)
+@pytest.mark.parametrize("t", list(TYPES))
+def test_orthogonalize(P, r, c, t):
+    g = randn(r + 7 * c, r, c, t=TYPES[t])
+    o = P.orthogonalize(g)
+    check_ortho(o, g)
+    assert torch.equal(o, P.orthogonalize(g))
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 100), (7, 100, 40), (2, 3, 20, 20), (5, 70, 200), (3, 300, 80), (2, 2, 128, 129), (300, 9, 4), (1, 1, 1)])
+def test_orthogonalize_stacks(P, shape):
+    g = randn(11, *shape)
+    check_ortho(P.orthogonalize(g), g)
+
+
+@pytest.mark.parametrize("spectrum", ["nonnegative", "decaying", "rank one", "tiny", "huge", "two"])
+@pytest.mark.parametrize("r,c", [(40, 60), (200, 260), (1500, 150)])
+def test_orthogonalize_spectra(P, spectrum, r, c):
+    g = randn(12, r, c).abs() if spectrum == "nonnegative" else randn(12, r, c)
+    s = min(r, c)
+    if spectrum in ("decaying", "rank one", "two"):
+        u, _, v = torch.linalg.svd(g.double(), full_matrices=False)
+        i = torch.arange(1, s + 1, device="cuda", dtype=torch.float64)
+        sv = {"decaying": 1 / i, "rank one": torch.where(i == 1, 1.0, 1e-4), "two": torch.where(i <= 2, 1.0, 0.0)}[spectrum]
+        g = ((u * sv) @ v).float()
+    if spectrum == "tiny":
+        g = g * 2.0 ** -126
+    if spectrum == "huge":
+        g = g * 2.0 ** 120
+    check_ortho(P.orthogonalize(g), g)
+
+
+@pytest.mark.parametrize("r,c", [(30, 50), (90, 200)])
+@pytest.mark.parametrize("cf", [[CF], [(1.5, -0.5, 0.0)] * 4, [CF] * 6 + [(1.875, -1.25, 0.375)] * 4, [(8.2, -23.0, 15.6), (4.0, -2.9, 0.55), CF], [(0.0, 1.0, 0.0)], [(2.0, 0.0, 0.0)] * 3])
+def test_orthogonalize_coefficients(P, r, c, cf):
+    g = randn(13, r, c)
+    check_ortho(P.orthogonalize(g, steps=len(cf), coefficients=cf), g, len(cf), cf)
+
+
+@pytest.mark.parametrize("r,c", [(50, 3000), (300, 200)])
+def test_orthogonalize_to_orthonormal(P, r, c):
+    cf = [CF] * 8 + [(1.875, -1.25, 0.375)] * 4
+    o = P.orthogonalize(torch.randn(r, c, device="cuda"), len(cf), cf).double()
+    o = o if r <= c else o.t()
+    assert float((o @ o.t() - torch.eye(min(r, c), device="cuda")).abs().max()) < 1e-5  # 32-bit entries: s * u and the split's 2^-22
+
+
+def test_orthogonalize_layouts(P):
+    for s, l in ((20, 90), (90, 200)):
+        x = randn(14, 3, l + 5, s + 3)
+        for g in (x[:, :l, :s], x[:, :l, :s].mT, x.permute(1, 2, 0)[:l, :s, 1].contiguous().t(), x[:, ::2, ::2], x[0, :l, :s].expand(2, l, s)):
+            o = P.orthogonalize(g)
+            check_ortho(o, g)
+        out = torch.full((3, l + 5, s + 3), 5.0, device="cuda")
+        P.orthogonalize(x[:, :l, :s], out=out[:, 2:l + 2, 1:s + 1])
+        check_ortho(out[:, 2:l + 2, 1:s + 1], x[:, :l, :s])
+        out[:, 2:l + 2, 1:s + 1] = 5.0
+        assert bool((out == 5.0).all())
+
+
+@pytest.mark.parametrize("r,c", [(20, 40), (100, 130)])
+def test_orthogonalize_special(P, r, c):
+    g = randn(15, 5, r, c)
+    g[1] = 0
+    g[2, 3, 4] = float("nan")
+    g[3, 0, 0] = float("inf")
+    o = P.orthogonalize(g)
+    assert bool((o[1] == 0).all()) and bool(torch.isnan(o[2]).all()) and bool(torch.isnan(o[3]).all())
+    check_ortho(o[[0, 4]], g[[0, 4]])
+    assert P.orthogonalize(torch.empty(0, 3, device="cuda")).shape == (0, 3)
+    assert P.orthogonalize(torch.empty(0, 3, 5, device="cuda")).shape == (0, 3, 5)
+    for bad in (dict(steps=0), dict(steps=33), dict(coefficients=(1, 2)), dict(coefficients=[CF] * 4), dict(coefficients=(100, 0, 0)), dict(steps=3, coefficients=[(8.2, -23.0, 17.0), (4.0, -2.9, 0.55), CF]), dict(out=torch.empty(5, c, r, device="cuda"))):
+        with pytest.raises(P.NMFkError):
+            P.orthogonalize(g, **bad)
+
+
+# ---- as they are used together --------------------------------------------------------------------------------------------------
+
+def test_rangebasis(P):
+    n, m, k = 3000, 700, 12
+    g = torch.Generator().manual_seed(1)
+    u, v = torch.linalg.qr(torch.randn(n, k, generator=g).double())[0], torch.linalg.qr(torch.randn(m, k, generator=g).double())[0]
+    sv = torch.linspace(10, 4, k).double()
+    X = ((u * sv) @ v.t() + 1e-4 * torch.randn(n, m, generator=g).double()).float()
+    Q, B, sigma = P.rangebasis(X.cuda(), k)
+    assert Q.shape == (n, k) and B.shape == (k, m)
+    assert float((Q.t().double() @ Q.double() - torch.eye(k, device="cuda")).abs().max()) < 1e-5
+    # 8-bit entries are off by 2^-4 of themselves at most, at random: |noise| is below 2^-4 |X| / sqrt(min(n, m)) in a direction
+    noise = 2.0 ** -4 * float(X.norm()) / m ** 0.5
+    assert float((sigma.cpu().double() - sv).abs().max()) < noise
+    assert float((Q.double() @ B.double() - X.cuda().double()).norm()) < noise * k ** 0.5
+    host = P.rangebasis(X.numpy(), k)
+    assert all(isinstance(a, np.ndarray) and np.array_equal(a, b.cpu().numpy()) for a, b in zip(host, (Q, B, sigma)))
+    bad = X.clone()
+    bad[3, 3] = float("nan")
+    for call in (lambda: P.rangebasis(X.cuda(), 0), lambda: P.rangebasis(X.cuda(), 701), lambda: P.rangebasis(bad.cuda(), 3)):
+        with pytest.raises(P.NMFkError):
+            call()
+
+
+def test_rangebasis_next_to_execute(P):
+    """the rank a sweep finds is where the singular values that rangebasis reports end"""
+    g = np.random.default_rng(0)
+    X = (g.random((300, 3)) @ g.random((3, 120))).astype(np.float32)
+    sigma = P.rangebasis(X, 8)[2]
+    assert sigma[2] > 3 * sigma[3]
+    kopt = P.execute(X, range(2, 5), 4, load=False, save=False, quiet=True, seed=1)[5]
+    assert kopt == 3
+
+
+def test_training_step_of_a_linear_map(P):
+    """forward, backward and an orthogonal update of the weight, all in these operators"""
+    m, n, k = 200, 96, 160
+    A, W, target = torch.randn(m, k, device="cuda"), torch.randn(n, k, device="cuda") * 0.1, torch.randn(m, n, device="cuda")
+    (a8, at), (w8, wt) = P.quantize(A, both=True), P.quantize(W, tiles=True, both=True)
+    y = P.product(a8, w8)
+    dA, dW = P.product_grads(y - target, at, wt)
+    step = P.orthogonalize(dW)
+    check_ortho(step, dW)
+    w2 = W - 0.01 * step
+    y2 = P.product(a8, P.quantize(w2, tiles=True))
+    assert dA.shape == A.shape and bool(torch.isfinite(y2).all())
+
+
+# ---- streams, graphs ---------------------------------------------------------------------------------------------------------------
+
+def test_operators_run_on_the_current_stream(P):
+    x, b, g, h = randn(1, 600, 4000), randn(2, 64, 4000), randn(3, 4, 2000, 24), randn(4, 200, 300)
+    want = (P.product(P.quantize(x), P.quantize(b)), P.orthogonalize(g), P.orthogonalize(h))
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for rep in range(3):
+        for s in (s1, s2):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):  # the input is made late on this stream: a kernel on another one would read it too early
+                y = torch.zeros_like(x)
+                for _ in range(20):
+                    y = y * 0.5
+                y = y + x
+                outs.append((P.product(P.quantize(y), P.quantize(b)), P.orthogonalize(g), P.orthogonalize(h)))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(a, w) for a, w in zip(o, want))
+
+
+def test_two_captured_graphs_and_eager_calls(P):
+    """each graph keeps its own workspace: replays in any order, with eager calls between them, give the eager bits on the inputs of the moment"""
+    x, b, g, h = randn(1, 130, 9000), randn(2, 40, 9000), randn(3, 3, 900, 20), randn(4, 200, 1500)
+
+    def step():
+        q, t = P.quantize(x, both=True)
+        b8, bt = P.quantize(b, tiles=True, both=True)
+        y = P.product(q, b8)
+        return (y, *P.product_grads(y, t, bt), P.orthogonalize(g), P.orthogonalize(h))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        cg = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(cg):
+            out = step()
+        graphs.append((cg, out))
+    for rep in range(4):
+        for v in (x, b, g, h):
+            v.copy_(torch.roll(v, 1, 0) * 1.25)
+        want = step()
+        for cg, out in (graphs if rep % 2 else graphs[::-1]):
+            for o in out:
+                o.zero_()
+            cg.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, w) for a, w in zip(out, want))
+            step()
