@@ -26,135 +26,352 @@ template <typename T>
 __device__ __forceinline__ float read_at(const Strided &g, int64_t b, int64_t i, int64_t j) {
   return to_f32(((const T *)g.p)[b * g.batch + i * g.row + j * g.col]);
 }
-template <typename T>
-__device__ __forceinline__ void write_at(const Strided &g, int64_t b, int64_t i, int64_t j, float x) {
-  ((T *)g.p)[b * g.batch + i * g.row + j * g.col] = from_f32<T>(x);
-}
 
 // ---- s <= 64 ---------------------------------------------------------------------------------------------------------------------
+//
+// The fp64 matrix instruction (16 x 16 x 4) leaves entry [4 r + g][c] of its result in register r of lane 16 g + c, and takes, for its k-th step,
+// entry [c][4 k + g] of the first and [4 k + g][c] of the second operand there.  All matrices of the iteration are polynomials of S, hence
+// symmetric and commuting: register r of a result IS the operand of step r, on either side.  Products chain without moving an entry.
 
 struct SmallArgs {
   Strided g, o;
   double *part;  // [batch][chunks][s][s]
-  float *q;      // [batch][s][s]
+  float *q;      // [batch][s][s], s > 16
   int64_t b0;
   int s, chunks, steps;
   int64_t l, chunk;  // entries of l per workgroup
-  const double *coef;
+  int gvec, ovec;    // four entries along the contiguous side may be loaded / stored at once
 };
 
 struct Coefs {
   double v[3 * 32];
 };
 
-// partial S over a chunk of l: 64 columns of X at a time in LDS, a pair (i, j) a thread
-template <typename T>
+template <typename T, bool WIDE>
+__device__ __forceinline__ void small_load4(const Strided &g, const T *p, int s, int64_t l, int vec, int i, int64_t j, float (&out)[4]) {
+  const T *q = p + i * g.row + j * g.col;
+  const bool whole = WIDE ? i < s && j + 4 <= l : j < l && i + 4 <= s;
+  if (vec && whole) {
+    const vec4<T> v = *(const vec4<T> *)q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = to_f32(v.v[e]);
+  } else {
+    const int64_t step = WIDE ? g.col : g.row;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = (WIDE ? i < s && j + e < l : j < l && i + e < s) ? to_f32(q[e * step]) : 0.f;
+  }
+}
+
+// Partial S over a chunk of l, in 64 bits.  What bounds it is the read of G, so a lane holds an entry in the place where the matrix
+// instruction wants it on both sides, straight from memory.  With s <= 8 the instruction's 16 rows take 16 / s columns of X at once (the
+// diagonal blocks of the result add up to S).
+template <typename T, int TT, bool WIDE>
 __global__ __launch_bounds__(256) void small_gram_kernel(SmallArgs a) {
-  __shared__ float x[64][SMALL + 1];
+  __shared__ double sum[4][256];
   const int64_t b = a.b0 + blockIdx.y;
   const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
-  const int s = a.s, t = threadIdx.x;
-  double acc[SMALL * SMALL / 256];
+  const int s = a.s, t = threadIdx.x, w = t >> 6, lane = t & 63, c = lane & 15, g = lane >> 4;
+  const int packed = TT == 1 ? max(1, 16 / s) : 1, grp = TT == 1 ? c / s : 0, row = TT == 1 ? c - grp * s : c;
+  const bool live = grp < packed;
+  const T *p = (const T *)a.g.p + b * a.g.batch;
+  f64x4 acc[TT * (TT + 1) / 2];
 #pragma unroll
-  for (int k = 0; k < SMALL * SMALL / 256; ++k) acc[k] = 0;
-  for (int64_t base = l0; base < l1; base += 64) {
-    const int w = (int)min((int64_t)64, l1 - base);
-    for (int e = t; e < 64 * s; e += 256) {  // along whichever side is contiguous
-      const int i = a.g.row == 1 ? e % s : e / 64, j = a.g.row == 1 ? e / s : e % 64;
-      x[j][i] = j < w ? read_at<T>(a.g, b, i, base + j) : 0.f;
+  for (int k = 0; k < TT * (TT + 1) / 2; ++k) acc[k] = (f64x4){0, 0, 0, 0};
+  constexpr int U = TT == 1 ? 8 : TT == 2 ? 4 : 2;  // loads in flight
+  if (WIDE) {
+    constexpr int UW = TT == 1 ? 4 : TT == 2 ? 2 : 1;
+    const int span = 16 * packed;
+    for (int64_t base = l0 + (int64_t)w * UW * span; base < l1; base += 4 * UW * span) {
+      float x[UW][TT][4];
+#pragma unroll
+      for (int u = 0; u < UW; ++u)
+#pragma unroll
+        for (int k = 0; k < TT; ++k) small_load4<T, true>(a.g, p, live ? s : 0, l1, a.gvec, 16 * k + row, base + u * span + grp * 16 + 4 * g, x[u][k]);
+#pragma unroll
+      for (int u = 0; u < UW; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          double v[TT];
+#pragma unroll
+          for (int k = 0; k < TT; ++k) v[k] = (double)x[u][k][e];
+#pragma unroll
+          for (int i = 0; i < TT; ++i)
+#pragma unroll
+            for (int j = 0; j <= i; ++j) acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[i], v[j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+        }
     }
-    __syncthreads();
+  } else {
+    const int span = 4 * packed;
+    for (int64_t base = l0 + (int64_t)w * U * span; base < l1; base += 4 * U * span) {
+      float x[U][TT];
 #pragma unroll
-    for (int k = 0; k < SMALL * SMALL / 256; ++k) {
-      const int e = t + k * 256;
-      if (e < s * s) {
-        const int i = e / s, j = e % s;
-        double v = acc[k];
-        for (int c = 0; c < 64; ++c) v = fma((double)x[c][i], (double)x[c][j], v);
-        acc[k] = v;
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = base + u * span + g * packed + grp;
+#pragma unroll
+        for (int k = 0; k < TT; ++k) x[u][k] = live && j < l1 && 16 * k + row < s ? to_f32(p[(16 * k + row) * a.g.row + j * a.g.col]) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        double v[TT];
+#pragma unroll
+        for (int k = 0; k < TT; ++k) v[k] = (double)x[u][k];
+#pragma unroll
+        for (int i = 0; i < TT; ++i)
+#pragma unroll
+          for (int j = 0; j <= i; ++j) acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[i], v[j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
       }
     }
-    __syncthreads();
   }
+  double *out = a.part + ((int64_t)blockIdx.y * a.chunks + blockIdx.x) * s * s;
 #pragma unroll
-  for (int k = 0; k < SMALL * SMALL / 256; ++k) {
-    const int e = t + k * 256;
-    if (e < s * s) a.part[((int64_t)blockIdx.y * a.chunks + blockIdx.x) * s * s + e] = acc[k];
-  }
+  for (int i = 0; i < TT; ++i)
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[w][(4 * r + g) * 16 + c] = acc[i * (i + 1) / 2 + j][r];
+      __syncthreads();
+      if (TT == 1) {
+        if (t < s * s) {
+          const int y = t / s, x = t - y * s;
+          double v = 0;
+          for (int k = 0; k < packed; ++k) {
+            const int e = (k * s + y) * 16 + k * s + x;
+            v += (sum[0][e] + sum[1][e]) + (sum[2][e] + sum[3][e]);
+          }
+          out[t] = v;
+        }
+      } else {
+        const int y = 16 * i + (t >> 4), x = 16 * j + (t & 15);
+        const double v = (sum[0][t] + sum[1][t]) + (sum[2][t] + sum[3][t]);
+        if (y < s && x < s) {
+          out[y * s + x] = v;
+          if (i != j) out[x * s + y] = v;
+        }
+      }
+      __syncthreads();
+    }
 }
 
-__device__ __forceinline__ double dot_row(const double *x, const double *y, int s, int i, int j) {
-  double v = 0;
-  for (int k = 0; k < s; ++k) v = fma(x[i * s + k], y[k * s + j], v);
-  return v;
+// 1 / |G|^2 and 1 / |G| as the iteration uses them: 0 for a matrix of zeros, NaN for one that is not finite
+__device__ __forceinline__ void small_norm(double norm2, double &inv2, double &inv) {
+  const double nan = __longlong_as_double(0x7ff8000000000000ll);
+  const bool finite = norm2 <= 1.7e308;
+  inv2 = !finite ? nan : norm2 > 0 ? 1.0 / norm2 : 0.0;
+  inv = !finite ? nan : norm2 > 0 ? 1.0 / sqrt(norm2) : 0.0;
 }
 
-// the iteration on s x s matrices: one workgroup per matrix
-__global__ __launch_bounds__(256) void small_iterate_kernel(SmallArgs a, Coefs cf) {
+__device__ __forceinline__ f64x4 sym_product(f64x4 x, f64x4 y) {
+  f64x4 d = {0, 0, 0, 0};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) d = __builtin_amdgcn_mfma_f64_16x16x4f64(x[r], y[r], d, 0, 0, 0);
+  return d;
+}
+
+// 16 < s <= 64: the iteration by one workgroup per matrix, a wave per 16 x 16 tile, the matrices in LDS as registers of lanes
+template <int TT>
+__global__ __launch_bounds__(64 * TT * TT) void small_iterate_kernel(SmallArgs a, Coefs cf) {
   extern __shared__ double mats[];
-  const int s = a.s, n = s * s, t = threadIdx.x;
-  double *S = mats, *P = S + n, *Q = P + n, *U = Q + n;
-  const double *part = a.part + (int64_t)blockIdx.x * a.chunks * n;
-  for (int e = t; e < n; e += 256) {
-    double v = 0;
-    for (int c = 0; c < a.chunks; ++c) v += part[(int64_t)c * n + e];
-    S[e] = v;
-    Q[e] = (e / s == e % s) ? 1.0 : 0.0;
-  }
+  constexpr int N = TT * TT * 256;
+  const int s = a.s, w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, ti = w / TT, tj = w % TT;
+  double *S = mats, *P = S + N, *Q = P + N, *U = Q + N;
+  const double *part = a.part + (int64_t)blockIdx.x * a.chunks * s * s;
+  const int x = 16 * tj + c;
+  f64x4 v = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int k = 0; k < a.chunks; ++k)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int y = 16 * ti + 4 * r + g;
+      if (y < s && x < s) v[r] += part[(int64_t)k * s * s + y * s + x];
+    }
+  auto put = [&](double *m, f64x4 d) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m[(w * 4 + r) * 64 + lane] = d[r];
+  };
+  auto product = [&](const double *m, const double *n) {  // of this wave's tile
+    f64x4 d = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < TT; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        d = __builtin_amdgcn_mfma_f64_16x16x4f64(m[((k * TT + ti) * 4 + r) * 64 + lane], n[((k * TT + tj) * 4 + r) * 64 + lane], d, 0, 0, 0);
+    return d;
+  };
+  put(S, v);
   __syncthreads();
   double norm2 = 0;
-  for (int i = 0; i < s; ++i) norm2 += S[i * s + i];
+  for (int i = 0; i < s; ++i) {  // [i][i]: tile (i / 16, i / 16), register (i % 16) / 4, lane 16 (i % 4) + i % 16
+    const int k = i >> 4, e = i & 15;
+    norm2 += S[((k * TT + k) * 4 + (e >> 2)) * 64 + 16 * (e & 3) + e];
+  }
+  double inv2, inv;
+  small_norm(norm2, inv2, inv);
   __syncthreads();
-  const bool finite = norm2 <= 1.7e308;
-  const double scale = !finite ? __longlong_as_double(0x7ff8000000000000ll) : norm2 > 0 ? 1.0 / norm2 : 0.0;
-  for (int e = t; e < n; e += 256) S[e] *= scale;
+  f64x4 sv = v * inv2, q = {0, 0, 0, 0};
+  put(S, sv);
   __syncthreads();
   for (int k = 0; k < a.steps; ++k) {
-    const double ca = cf.v[3 * k], cb = cf.v[3 * k + 1], cc = cf.v[3 * k + 2];
-    for (int e = t; e < n; e += 256) P[e] = cb * S[e] + cc * dot_row(S, S, s, e / s, e % s) + ((e / s == e % s) ? ca : 0.0);
+    f64x4 p = cf.v[3 * k + 1] * sv + cf.v[3 * k + 2] * product(S, S);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (ti == tj && 4 * r + g == c) p[r] += cf.v[3 * k];
+    put(P, p);
     __syncthreads();
-    for (int e = t; e < n; e += 256) U[e] = dot_row(Q, P, s, e / s, e % s);
+    q = k == 0 ? p : product(Q, P);
+    if (k + 1 < a.steps) put(U, product(S, P));
     __syncthreads();
-    double *sw = Q;
-    Q = U;
-    U = sw;
     if (k + 1 < a.steps) {
-      for (int e = t; e < n; e += 256) U[e] = dot_row(S, P, s, e / s, e % s);
-      __syncthreads();
-      for (int e = t; e < n; e += 256) S[e] = dot_row(U, P, s, e / s, e % s);
+      put(Q, q);
+      sv = product(U, P);
+      put(S, sv);
       __syncthreads();
     }
   }
-  const double inv = !finite ? __longlong_as_double(0x7ff8000000000000ll) : norm2 > 0 ? 1.0 / sqrt(norm2) : 0.0;
-  for (int e = t; e < n; e += 256) a.q[(int64_t)blockIdx.x * n + e] = (float)(Q[e] * inv);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int y = 16 * ti + 4 * r + g;
+    if (y < s && x < s) a.q[(int64_t)blockIdx.x * s * s + y * s + x] = (float)(q[r] * inv);
+  }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a) {
-  __shared__ float x[64][SMALL + 1], q[SMALL * SMALL], y[64][SMALL + 1];
+// O = Q X over a chunk of l, on the fp32 matrix pipe (16 x 16 x 4: entry [c][.] of the first, [.][c] of the second operand in lane 16 g + c, result
+// [4 g + r][c] in register r).  Which four of the sum's entries a step takes is free: a lane's four consecutive entries of X serve four steps,
+// or four columns, and its four results stand next to each other in O.  s <= 16: every workgroup iterates for itself, in registers (about
+// 2 microseconds, less than a launch); the waves share the sum over the chunks.
+template <typename T, int TT, bool WIDE>
+__global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf) {
+  __shared__ double sum[4][256];
+  __shared__ float qs[16][17];
   const int64_t b = a.b0 + blockIdx.y;
-  const int s = a.s, t = threadIdx.x;
-  for (int e = t; e < s * s; e += 256) q[e] = a.q[(int64_t)blockIdx.y * s * s + e];
   const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
-  for (int64_t base = l0; base < l1; base += 64) {
-    const int w = (int)min((int64_t)64, l1 - base);
-    for (int e = t; e < 64 * s; e += 256) {
-      const int i = a.g.row == 1 ? e % s : e / 64, j = a.g.row == 1 ? e / s : e % 64;
-      x[j][i] = j < w ? read_at<T>(a.g, b, i, base + j) : 0.f;
+  const int s = a.s, t = threadIdx.x, w = t >> 6, lane = t & 63, c = lane & 15, g = lane >> 4;
+  float q[TT][TT][4];
+  if (TT == 1) {
+    const double *part = a.part + (int64_t)blockIdx.y * a.chunks * s * s;
+    const int y = t >> 4, x = t & 15;
+    double v[4] = {0, 0, 0, 0};
+    if (y < s && x < s) {
+      const double *e = part + y * s + x;
+      int k = 0;
+      for (; k + 4 <= a.chunks; k += 4)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += e[(int64_t)(k + r) * s * s];
+      for (; k < a.chunks; ++k) v[0] += e[(int64_t)k * s * s];
+    }
+    sum[0][t] = (v[0] + v[1]) + (v[2] + v[3]);
+    __syncthreads();
+    f64x4 S, P, Q = {0, 0, 0, 0};
+    double norm2 = 0, inv2, inv;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) S[r] = sum[0][(4 * r + g) * 16 + c];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) norm2 += sum[0][i * 17];
+    small_norm(norm2, inv2, inv);
+    S *= inv2;
+    for (int k = 0; k < a.steps; ++k) {
+      P = cf.v[3 * k + 1] * S + cf.v[3 * k + 2] * sym_product(S, S);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * r + g == c) P[r] += cf.v[3 * k];
+      if (k + 1 < a.steps) S = sym_product(sym_product(S, P), P);
+      Q = k == 0 ? P : sym_product(Q, P);
+    }
+    if (w == 0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) qs[4 * r + g][c] = (float)(Q[r] * inv);
     }
     __syncthreads();
-    for (int e = t; e < 64 * s; e += 256) {
-      const int j = e & 63, i = e >> 6;
-      float v = 0.f;
-      for (int k = 0; k < s; ++k) v = fmaf(q[i * s + k], x[j][k], v);
-      y[j][i] = v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[0][0][k] = qs[c][WIDE ? 4 * k + g : 4 * g + k];
+  } else {
+    const float *m = a.q + (int64_t)blockIdx.y * s * s;
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int j = 0; j < TT; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int y = 16 * i + c, x = 16 * j + (WIDE ? 4 * k + g : 4 * g + k);
+          q[i][j][k] = y < s && x < s ? m[y * s + x] : 0.f;
+        }
+  }
+  const T *p = (const T *)a.g.p + b * a.g.batch;
+  T *o = (T *)a.o.p + b * a.o.batch;
+  if (WIDE) {
+    for (int64_t base = l0 + (int64_t)w * 64; base < l1; base += 256) {
+      float x[TT][4][4];
+#pragma unroll
+      for (int k = 0; k < TT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) small_load4<T, true>(a.g, p, s, l1, a.gvec, 16 * k + 4 * r + g, base + 4 * c, x[k][r]);
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        f32x4 d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < TT; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[i][k][r], x[k][r][e], d[e], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * i + 4 * g + r;
+          if (row >= s) continue;
+          const int64_t j = base + 4 * c;
+          T *z = o + row * a.o.row + j * a.o.col;
+          if (a.ovec && j + 4 <= l1) {
+            vec4<T> v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v.v[e] = from_f32<T>(d[e][r]);
+            *(vec4<T> *)z = v;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (j + e < l1) z[e * a.o.col] = from_f32<T>(d[e][r]);
+          }
+        }
+      }
     }
-    __syncthreads();
-    for (int e = t; e < 64 * s; e += 256) {
-      const int i = a.o.row == 1 ? e % s : e / 64, j = a.o.row == 1 ? e / s : e % 64;
-      if (j < w) write_at<T>(a.o, b, i, base + j, y[j][i]);
+  } else {
+    constexpr int U = TT == 1 ? 4 : TT == 2 ? 2 : 1;
+    for (int64_t base = l0 + (int64_t)w * 16 * U; base < l1; base += 64 * U) {
+      float x[U][TT][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < TT; ++k) small_load4<T, false>(a.g, p, s, l1, a.gvec, 16 * k + 4 * g, base + 16 * u + c, x[u][k]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = base + 16 * u + c;
+        f32x4 d[TT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) d[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < TT; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < TT; ++i) d[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[i][k][r], x[u][k][r], d[i], 0, 0, 0);
+        if (j >= l1) continue;
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          const int row = 16 * i + 4 * g;
+          T *z = o + row * a.o.row + j * a.o.col;
+          if (a.ovec && row + 4 <= s) {
+            vec4<T> v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v.v[r] = from_f32<T>(d[i][r]);
+            *(vec4<T> *)z = v;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (row + r < s) z[r * a.o.row] = from_f32<T>(d[i][r]);
+          }
+        }
+      }
     }
-    __syncthreads();
   }
 }
 
@@ -427,7 +644,9 @@ Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     return o;
   };
   if (y.s <= SMALL) {
-    y.chunks = std::max<int64_t>(1, std::min<int64_t>(nmfk_div_up(y.l, 64), nmfk_div_up(1024, batch)));
+    // about 2048 workgroups, each with 256 entries of l at least; the partial S of one matrix are summed by every workgroup (s <= 16) or by one
+    const int64_t most = y.s <= 16 ? 256 : 128;
+    y.chunks = std::max<int64_t>(1, std::min<int64_t>({nmfk_div_up(y.l, 256), nmfk_div_up(2048, batch), most}));
     y.chunk = nmfk_round_up(nmfk_div_up(y.l, y.chunks), 64);
     y.chunks = nmfk_div_up(y.l, y.chunk);
     y.part = take(batch * y.chunks * y.s * y.s * 8);
@@ -478,12 +697,30 @@ int exponent(double bound) {
   return std::min(15 - e, 100);
 }
 
+// four consecutive entries along the side whose stride is `unit` may be moved at once, wherever they start at a multiple of four
+template <typename T>
+int four_at_once(const Strided &g, int64_t unit, int64_t other) {
+  return unit == 1 && other % 4 == 0 && g.batch % 4 == 0 && (uintptr_t)g.p % (4 * sizeof(T)) == 0;
+}
+
+template <typename T, int TT, bool WIDE>
+void small_launch(const SmallArgs &a, const Coefs &cf, unsigned nb, hipStream_t st) {
+  const dim3 grid((unsigned)a.chunks, nb);
+  small_gram_kernel<T, TT, WIDE><<<grid, 256, 0, st>>>(a);
+  if (TT > 1) {
+    constexpr int BYTES = 4 * TT * TT * 256 * 8;
+    static std::atomic<uint64_t> done{0};
+    nmfk_allow_dynamic_lds((const void *)small_iterate_kernel<TT>, done, BYTES);
+    small_iterate_kernel<TT><<<dim3(nb), 64 * TT * TT, BYTES, st>>>(a, cf);
+  }
+  small_apply_kernel<T, TT, WIDE><<<grid, 256, 0, st>>>(a, cf);
+}
+
 template <typename T>
 int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, const double *coef, char *work, hipStream_t st) {
   Coefs cf = {};
   for (int k = 0; k < 3 * steps; ++k) cf.v[k] = coef[k];
-  static std::atomic<uint64_t> done{0};
-  nmfk_allow_dynamic_lds((const void *)small_iterate_kernel, done, 4 * SMALL * SMALL * 8);
+  const bool wide = g.col == 1 && g.row != 1;
   for (int64_t b0 = 0; b0 < y.batch; b0 += 32768) {
     const unsigned nb = (unsigned)std::min<int64_t>(32768, y.batch - b0);
     SmallArgs a = {};
@@ -497,9 +734,18 @@ int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, 
     a.steps = steps;
     a.l = y.l;
     a.chunk = y.chunk;
-    small_gram_kernel<T><<<dim3((unsigned)y.chunks, nb), 256, 0, st>>>(a);
-    small_iterate_kernel<<<dim3(nb), 256, 4 * y.s * y.s * 8, st>>>(a, cf);
-    small_apply_kernel<T><<<dim3((unsigned)y.chunks, nb), 256, 0, st>>>(a);
+    a.gvec = wide ? four_at_once<T>(g, g.col, g.row) : four_at_once<T>(g, g.row, g.col);
+    a.ovec = wide ? four_at_once<T>(o, o.col, o.row) : four_at_once<T>(o, o.row, o.col);
+#define NMFK_SMALL(TT) (wide ? small_launch<T, TT, true>(a, cf, nb, st) : small_launch<T, TT, false>(a, cf, nb, st))
+    if (y.s <= 16)
+      NMFK_SMALL(1);
+    else if (y.s <= 32)
+      NMFK_SMALL(2);
+    else if (y.s <= 48)
+      NMFK_SMALL(3);
+    else
+      NMFK_SMALL(4);
+#undef NMFK_SMALL
   }
   return nmfk_launched("nmfk_orthogonalize");
 }
