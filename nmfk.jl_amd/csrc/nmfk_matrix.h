@@ -106,4 +106,11 @@ __device__ __forceinline__ int xcd_order(int id, int total) {
   return x * per + (x < rest ? x : rest) + i;
 }
 
+// ... and walk the tiles in bands of `band` tile rows, column by column, so that the tiles which an XCD has in work at a time share rows of both operands
+__device__ __forceinline__ void tile_at(int id, int tiles_m, int tiles_n, int band, int &tm, int &tn) {
+  const int per = band * tiles_n, k = id / per, first = k * band, rows = min(band, tiles_m - first), in = id - k * per;
+  tn = in / rows;
+  tm = first + in - tn * rows;
+}
+
 }  // namespace nmfk_mat

@@ -414,23 +414,34 @@ __device__ __forceinline__ f32x4 get4(const char *row, int col) {
   return v;
 }
 
-constexpr int NORM_PARTS = 64;
+constexpr int NORM_PARTS = 256;  // one for each thread of split_kernel
 
-// |G|^2 in 64 bits, NORM_PARTS partial sums per matrix
+// |G|^2 in 64 bits, NORM_PARTS partial sums per matrix: a wave walks rows along the contiguous side, four entries a lane
 template <typename T>
-__global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s, int64_t l, double *part) {
+__global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s, int64_t l, double *part, int vec) {
   const int64_t b = b0 + blockIdx.y;
   const bool flip = g.row == 1;
   const int64_t outer = flip ? l : s, inner = flip ? s : l;
   const int64_t so = flip ? g.col : g.row, si = flip ? g.row : g.col;
   const T *p = (const T *)g.p + b * g.batch;
   double v = 0;
-  const int64_t total = outer * inner, per = (total + NORM_PARTS - 1) / NORM_PARTS;
-  const int64_t e0 = blockIdx.x * per, e1 = min(total, e0 + per);
-  for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
-    const int64_t o = e / inner;
-    const double x = to_f32(p[o * so + (e - o * inner) * si]);
-    v = fma(x, x, v);
+  const int lane = threadIdx.x & 63;
+  for (int64_t o = blockIdx.x + NORM_PARTS * (threadIdx.x >> 6); o < outer; o += 4 * NORM_PARTS) {
+    const T *q = p + o * so;
+#pragma unroll 4
+    for (int64_t e = lane * 4; e < inner; e += 256) {
+      float x[4];
+      if (vec && e + 4 <= inner) {
+        const vec4<T> u = *(const vec4<T> *)(q + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = to_f32(u.v[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = e + k < inner ? to_f32(q[(e + k) * si]) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v = fma((double)x[k], (double)x[k], v);
+    }
   }
   __shared__ double sum[4];
 #pragma unroll
@@ -446,8 +457,13 @@ __global__ __launch_bounds__(256) void split_kernel(Strided g, int64_t b0, int s
   __shared__ float tile[64][65];
   const int t = threadIdx.x;
   const int64_t b = b0 + blockIdx.z;
-  double norm2 = 0;
-  for (int k = 0; k < NORM_PARTS; ++k) norm2 += part[(int64_t)blockIdx.z * NORM_PARTS + k];
+  __shared__ double sums[4];
+  double norm2 = part[(int64_t)blockIdx.z * NORM_PARTS + t];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) norm2 += __shfl_xor(norm2, o);
+  if ((t & 63) == 0) sums[t >> 6] = norm2;
+  __syncthreads();
+  norm2 = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   const double scale = !(norm2 <= 1.7e308) ? __longlong_as_double(0x7ff8000000000000ll) : norm2 > 0 ? pow2 / sqrt(norm2) : 0.0;
   const int64_t j0 = (int64_t)blockIdx.x * 64;
   const int i0 = blockIdx.y * 64;
@@ -501,9 +517,7 @@ __global__ __launch_bounds__(256) void gemm_kernel(GemmArgs a) {
     while (ti * (ti + 1) / 2 > id) --ti;
     tj = id - ti * (ti + 1) / 2;
   } else {
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    ti = id / a.tiles_n;
-    tj = id - ti * a.tiles_n;
+    tile_at(xcd_order(blockIdx.x, gridDim.x), (a.m + 127) >> 7, a.tiles_n, 8, ti, tj);
   }
   const int i0 = ti * 128, j0 = tj * 128;
   const int64_t b = blockIdx.z;
@@ -770,7 +784,7 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
     double *norm = (double *)(work + y.norm) + b0 * NORM_PARTS;
     double u = 1.0;
     int ex = exponent(1.01 * u);
-    norm_kernel<T><<<dim3(NORM_PARTS, nb), 256, 0, st>>>(g, b0, s, l, norm);
+    norm_kernel<T><<<dim3(NORM_PARTS, nb), 256, 0, st>>>(g, b0, s, l, norm, g.row == 1 ? four_at_once<T>(g, 1, g.col) : four_at_once<T>(g, g.col, g.row));
     split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, ldexp(1.0, ex), X, XT);
     for (int k = 0; k < steps; ++k) {
       const double ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];

@@ -93,7 +93,8 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int wm = w / WN, wn = w % WN;
   const int id = xcd_order(blockIdx.x, gridDim.x);
-  const int tn = id % p.tiles_n, tm = id / p.tiles_n;
+  int tm, tn;
+  tile_at(id, p.tiles_m, p.tiles_n, BM == 256 ? 4 : 8, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
   const int kb0 = blockIdx.y * p.kb_split, kb1 = min(p.kb, kb0 + p.kb_split);
 
@@ -201,8 +202,11 @@ struct Plan {
 
 Plan prod_plan(int64_t m, int64_t n, int64_t kb) {
   Plan q;
-  q.bm = 128;
-  q.bn = n <= 64 ? 64 : 128;
+  q.bm = q.bn = 128;
+  if (n <= 64)
+    q.bn = 64;
+  else if (nmfk_div_up(m, 256) * nmfk_div_up(n, 256) >= 200)
+    q.bm = q.bn = 256;
   const int64_t tiles = nmfk_div_up(m, q.bm) * nmfk_div_up(n, q.bn);
   // Few tiles leave most of the 256 CUs without one: split the sum, as long as a workgroup keeps four blocks.
   int64_t splits = tiles >= 256 ? 1 : std::min<int64_t>(512 / tiles, nmfk_div_up(kb, 4));
@@ -240,7 +244,9 @@ int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
     prod_join_kernel<T><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
   } else {
     p.vec = p.ldy % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
-    if (q.bn == 64)
+    if (q.bn == 256)
+      prod_tile<256, 256, 2, 4, F, T, false>(p, 1, st);
+    else if (q.bn == 64)
       prod_tile<128, 64, 4, 1, F, T, false>(p, 1, st);
     else
       prod_tile<128, 128, 2, 2, F, T, false>(p, 1, st);
