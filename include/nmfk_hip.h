@@ -280,8 +280,8 @@ int nmfk_quantize(int device, void *stream, int dtype, const void *X, int64_t ro
 
 /* Y = A * B' (m x n, entry (i, j) at Y[i * ldy + j]) of two matrices in 8 bits, A m x k and B n x k, as nmfk_quantize lays them out:
  * Y[i, j] = sum over blocks b of sA[i, b] * sB[j, b] * sum of the block's a[i, t] * b[j, t], summed in fp32, rounded once to `dtype`.
- * k = 0 gives zeros.  The result does not depend on the run (no atomics).  nmfk_product_workspace: bytes of `work` for these sizes. */
-int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int64_t *bytes);
+ * lda, ldb: at most 2^23.  k = 0 gives zeros.  The result does not depend on the run (no atomics).  nmfk_product_workspace: bytes of `work` for these sizes and this type of Y. */
+int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes);
 int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, const uint8_t *A, int64_t lda, const float *sA,
                  int64_t ldsa, int a_tiles, const uint8_t *B, int64_t ldb, const float *sB, int64_t ldsb, int b_tiles, int dtype,
                  void *Y, int64_t ldy, void *work, int64_t work_bytes);

@@ -117,7 +117,7 @@ def lib():
                                    C.POINTER(C.c_int)]
     i64, ci = C.c_int64, C.c_int
     L.nmfk_quantize.argtypes = [ci, vp, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp, i64, vp, i64, vp, i64]
-    L.nmfk_product_workspace.argtypes = [i64, i64, i64, i64p]
+    L.nmfk_product_workspace.argtypes = [i64, i64, i64, ci, i64p]
     L.nmfk_product.argtypes = [ci, vp, i64, i64, i64, vp, i64, vp, i64, ci, vp, i64, vp, i64, ci, ci, vp, i64, vp, i64]
     L.nmfk_orthogonalize_workspace.argtypes = [i64, i64, i64, i64p]
     L.nmfk_orthogonalize.argtypes = [ci, vp, ci, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, ci, vp, vp, i64]

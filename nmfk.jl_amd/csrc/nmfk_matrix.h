@@ -100,6 +100,16 @@ __device__ __forceinline__ i32x4 lds_chunk(const char *lds, int row, int c) {
 // every copy into LDS that this wave started has landed
 __device__ __forceinline__ void staged() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// ... all but the last N of them
+template <int N>
+__device__ __forceinline__ void staged_but() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// The workgroup's waves meet; what a wave has read from LDS it has received.  Unlike __syncthreads this does not wait for copies in flight.
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // Workgroups are dealt to the 8 XCDs in turn, each with an L2 of its own: renumber them so that an XCD gets consecutive numbers.
 __device__ __forceinline__ int xcd_order(int id, int total) {
   const int per = total >> 3, rest = total & 7, x = id & 7, i = id >> 3;

@@ -11,6 +11,8 @@
 //     the exact one, 1/35 of half a step of fp16, 1/280 of bf16.
 //   Y in fp32: that would show, so the entries are converted to fp16 (exact) and go through four v_mfma_f32_16x16x32_f16 (a block's sum 1e-8
 //     away), at half the rate.  v_mfma_f32_16x16x32_fp8_fp8 has the rate of the latter and the error of the former.
+#include <type_traits>
+
 #include "nmfk_matrix.h"
 
 using namespace nmfk_mat;
@@ -47,11 +49,13 @@ __device__ __forceinline__ void store4(T *p, f32x4 v, int left, int vec) {
 
 // A lane's operand for a block: 32 of its row's 128 entries.
 struct Bytes {
+  static constexpr int STEPS = 1;
   i32x8 v;
   __device__ __forceinline__ Bytes() {}
   __device__ __forceinline__ Bytes(i32x4 lo, i32x4 hi) { v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 };
 struct Halves {
+  static constexpr int STEPS = 4;
   f16x8 v[4];
   __device__ __forceinline__ Halves() {}
   __device__ __forceinline__ Halves(i32x4 lo, i32x4 hi) {
@@ -65,30 +69,30 @@ struct Halves {
       }
   }
 };
-// the block's sums of TN tiles against one: the instructions of different tiles are independent and alternate
-template <int TN>
-__device__ __forceinline__ void block_products(const Bytes (&x)[TN], const Bytes &y, f32x4 (&part)[TN]) {
+// One step of a block's sum for a 16 x 16 tile: step 0 starts from zero.
+__device__ __forceinline__ f32x4 block_step(const Bytes &x, const Bytes &y, f32x4, int) {
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < TN; ++j) part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[j].v, y.v, zero, 0, 0, 0, 0, 0, 0);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x.v, y.v, zero, 0, 0, 0, 0, 0, 0);
 }
-template <int TN>
-__device__ __forceinline__ void block_products(const Halves (&x)[TN], const Halves &y, f32x4 (&part)[TN]) {
-#pragma unroll
-  for (int j = 0; j < TN; ++j) part[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[j].v[q], y.v[q], part[j], 0, 0, 0);
+__device__ __forceinline__ f32x4 block_step(const Halves &x, const Halves &y, f32x4 part, int q) {
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(x.v[q], y.v[q], q ? part : zero, 0, 0, 0);
 }
 
+// Which scales change inside a wave's part of a tile: with tiles of 128 x 128 on one side that side's scale is one number, and a block costs one
+// vector instruction for an output instead of two.
+enum { ROWS_ROWS = 0, B_TILES = 1, A_TILES = 2 };
+
 // A workgroup's tile of BM x BN outputs over its range of blocks: WM x WN waves, each (BM / WM) x (BN / WN).
-// Two buffers of 128-byte rows in LDS; the copies into one are in flight while the other is multiplied.
+// Two buffers of 128-byte rows in LDS; the copies into one are in flight while the other is multiplied.  A wave holds B's operands of a block in
+// registers, so B's half of a buffer is free after the first row of tiles and A's before the last one: at these two places the waves meet and
+// start the copies of the block after the next.  The operands of the next block are read while the matrix pipe is still busy with the last row of this one.
 // The first operand of the matrix instruction is B, so that a lane's four outputs are neighbours in a row of Y.
-template <int BM, int BN, int WM, int WN, typename F, typename T, bool SPLIT>
+template <int BM, int BN, int WM, int WN, int MODE, typename F, typename T, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int STAGE = (BM + BN) * 128, SC = (BM + BN) * 4;
+  static_assert(TM >= 4 && TN >= 2 && BM / WM <= 128 && BN / WN <= 128, "B is copied between row 1 and row TM - 2, the scales behind the last use of the old ones");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int wm = w / WN, wn = w % WN;
@@ -98,71 +102,155 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
   const int m0 = tm * BM, n0 = tn * BN;
   const int kb0 = blockIdx.y * p.kb_split, kb1 = min(p.kb, kb0 + p.kb_split);
 
-  // this wave's share of the copies; rows behind the last one repeat it (their outputs are not stored)
+  // this wave's share of the copies; rows behind the last one repeat it (their outputs are not stored).  A lane's offset from its tile's
+  // first row fits 32 bits: 256 rows of at most 2^23 bytes.
   const int lr = lane >> 3, lc = ((lane & 7) ^ lr) << 4;
-  const char *src[(BM + BN) / 8 / WAVES];
+  constexpr int CA = BM / 8 / WAVES, CB = BN / 8 / WAVES;
+  static_assert(CA * 8 * WAVES == BM && CB * 8 * WAVES == BN, "");
+  const char *pa = p.a + (int64_t)m0 * p.lda + (int64_t)kb0 * 128, *pb = p.b + (int64_t)n0 * p.ldb + (int64_t)kb0 * 128;
+  uint32_t off_a[CA], off_b[CB];
 #pragma unroll
-  for (int i = 0; i < (BM + BN) / 8 / WAVES; ++i) {
-    const int row = (i * WAVES + w) * 8;
-    src[i] = row < BM ? p.a + (int64_t)min(m0 + row + lr, p.m - 1) * p.lda + lc : p.b + (int64_t)min(n0 + row - BM + lr, p.n - 1) * p.ldb + lc;
+  for (int i = 0; i < CA; ++i) off_a[i] = (uint32_t)min((i * WAVES + w) * 8 + lr, p.m - 1 - m0) * (uint32_t)p.lda + lc;
+#pragma unroll
+  for (int i = 0; i < CB; ++i) off_b[i] = (uint32_t)min((i * WAVES + w) * 8 + lr, p.n - 1 - n0) * (uint32_t)p.ldb + lc;
+  // scales of rows: 64 at a time, by the waves in turn (a wave without a share of its own repeats another's)
+  constexpr int CS = ((BM + BN) / 64 + WAVES - 1) / WAVES;
+  const float *ps[CS];
+  int64_t ps_ld[CS];
+  int ps_row[CS];
+#pragma unroll
+  for (int i = 0; i < CS; ++i) {
+    const int row = (i * WAVES + w) % ((BM + BN) / 64) * 64;
+    const bool is_a = row < BM;
+    ps_row[i] = row;
+    ps_ld[i] = is_a ? p.ldsa : p.ldsb;
+    ps[i] = (is_a ? p.sa + (min(m0 + row + lane, p.m - 1) >> p.ashift) : p.sb + (min(n0 + row - BM + lane, p.n - 1) >> p.bshift)) + kb0 * ps_ld[i];
   }
-  constexpr int SW = (BM + BN) / 64;  // waves' worth of scales
-  auto stage = [&](int kb, int buf) {
-    char *base = lds + buf * STAGE;
+  auto stage_b = [&](int buf) {  // the next block in order
 #pragma unroll
-    for (int i = 0; i < (BM + BN) / 8 / WAVES; ++i) stage8(src[i] + (int64_t)kb * 128, base + (i * WAVES + w) * 1024);
+    for (int i = 0; i < CB; ++i) stage8(pb + off_b[i], lds + buf * STAGE + BM * 128 + (i * WAVES + w) * 1024);
+    pb += 128;
+  };
+  auto stage_a = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < CA; ++i) stage8(pa + off_a[i], lds + buf * STAGE + (i * WAVES + w) * 1024);
+    pa += 128;
     float *sc = (float *)(lds + 2 * STAGE + buf * SC);
 #pragma unroll
-    for (int i = w; i < SW; i += WAVES) {
-      const int row = i * 64;
-      const float *g = row < BM ? p.sa + kb * p.ldsa + (min(m0 + row + lane, p.m - 1) >> p.ashift)
-                                : p.sb + kb * p.ldsb + (min(n0 + row - BM + lane, p.n - 1) >> p.bshift);
-      stage_f32(g, sc + row);
+    for (int i = 0; i < CS; ++i) {
+      stage_f32(ps[i], sc + ps_row[i]);
+      ps[i] += ps_ld[i];
     }
   };
+  const int fr = lane & 15, fg = lane >> 4;
+  const int rm = wm * (BM / WM) + fr, rn = wn * (BN / WN) + fr;
+  auto scales = [&](int buf) { return (const float *)(lds + 2 * STAGE + buf * SC); };
+  // the scale that is one number in this wave's part (through LDS like the others: a wait for a load into a register would be a wait for
+  // the copies that started after it, too)
+  auto one = [&](int buf) { return scales(buf)[MODE == B_TILES ? BM + wn * (BN / WN) : wm * (BM / WM)]; };
+  auto frag_a = [&](int buf, int i) {
+    const char *la = lds + buf * STAGE;
+    return F(lds_chunk(la, rm + i * 16, fg), lds_chunk(la, rm + i * 16, fg + 4));
+  };
+  auto frag_b = [&](int buf, int j) {
+    const char *lb = lds + buf * STAGE + BM * 128;
+    return F(lds_chunk(lb, rn + j * 16, fg), lds_chunk(lb, rn + j * 16, fg + 4));
+  };
+  auto scale_b = [&](int buf, int j) { return *(const f32x4 *)(scales(buf) + BM + wn * (BN / WN) + j * 16 + fg * 4); };
 
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
-  if (kb0 < kb1) {
-    stage(kb0, 0);
+  const int blocks = kb1 - kb0;
+  if (blocks > 0) {
+    stage_a(0);
+    stage_b(0);
     staged();
-  }
-  __syncthreads();
-  const int fr = lane & 15, fg = lane >> 4;
-  for (int kb = kb0, buf = 0; kb < kb1; ++kb, buf ^= 1) {
-    if (kb + 1 < kb1) stage(kb + 1, buf ^ 1);
-    const char *la = lds + buf * STAGE, *lb = la + BM * 128;
-    const float *sc = (const float *)(lds + 2 * STAGE + buf * SC);
-    F fb[TN];
-    f32x4 sb[TN];
+    meet();
+    if (blocks > 1) {
+      stage_a(1);
+      stage_b(1);
+    }
+    // The matrix instructions of a block are one sequence n = i * TN + j.  The vector instructions add the tile LAG places behind the one the
+    // matrix pipe has begun, and the operands of row i + 2 are requested when row i begins.
+    constexpr int LAG = 2, LEN = TM * TN;
+    F fb[TN], fa[3];
+    f32x4 sb[TN], part[LEN];
+    float sa[3] = {0.f, 0.f, 0.f}, so = 0.f, so_next = 0.f, s_old = 0.f;
+    if (MODE != ROWS_ROWS) so = one(0);
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int row = wn * (BN / WN) + j * 16;
-      fb[j] = F(lds_chunk(lb, row + fr, fg), lds_chunk(lb, row + fr, fg + 4));
-      sb[j] = *(const f32x4 *)(sc + BM + row + fg * 4);
+      fb[j] = frag_b(0, j);
+      if (MODE != B_TILES) sb[j] = MODE == A_TILES ? so * scale_b(0, j) : scale_b(0, j);
     }
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int row = wm * (BM / WM) + i * 16;
-      const F fa(lds_chunk(la, row + fr, fg), lds_chunk(la, row + fr, fg + 4));
-      const float sa = sc[row + fr];
-      f32x4 part[TN];
-      block_products<TN>(fb, fa, part);
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(part[j][r], sa * sb[j][r], acc[i][j][r]);
+    for (int i = 0; i < 2; ++i) {
+      fa[i] = frag_a(0, i);
+      if (MODE != A_TILES) sa[i] = scales(0)[rm + i * 16];
     }
-    staged();
-    __syncthreads();
+#pragma unroll
+    for (int n = LEN - LAG; n < LEN; ++n) part[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    int buf = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {  // (behind the last block the operands of "the next" are whatever stands in LDS, unused)
+      const bool copy = kb + 2 < kb1;
+      if (MODE == B_TILES) sa[0] *= so;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if (i == 1 && copy) {
+          meet();
+          stage_b(buf);
+        }
+        if (i == TM - 2) {
+          if (copy) {
+            staged_but<CB>();  // of the block after the next, B may still be on its way
+            meet();
+            stage_a(buf);
+          } else {
+            staged();
+            meet();
+          }
+          if (MODE != ROWS_ROWS) so_next = one(buf ^ 1);
+        }
+        const int from = i + 2 < TM ? buf : buf ^ 1, row = (i + 2) % TM;
+        fa[2] = frag_a(from, row);
+        if (MODE != A_TILES) sa[2] = scales(from)[rm + row * 16];
+#pragma unroll
+        for (int u = 0; u < TN * F::STEPS; ++u) {
+          const int j = u % TN, q = u / TN, n = i * TN + j;
+          part[n] = block_step(fb[j], fa[0], part[n], q);
+          if (q < F::STEPS - 1) continue;
+          if (i == TM - 1) fb[j] = frag_b(buf ^ 1, j);
+          const int o = (n + LEN - LAG) % LEN, oi = o / TN, oj = o % TN;
+          const float s = oi == i ? sa[0] : s_old;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[oi][oj][r] = fmaf(part[o][r], MODE == B_TILES ? s : MODE == A_TILES ? sb[oj][r] : s * sb[oj][r], acc[oi][oj][r]);
+          asm volatile("" : "+v"(acc[oi][oj]));  // the additions do not move behind a branch
+          if (MODE != B_TILES && oi == TM - 1) {  // the last use of this scale: the next block's
+            const f32x4 v = scale_b(i == 0 ? buf : buf ^ 1, oj);
+            sb[oj] = MODE == A_TILES ? (i == 0 ? so : so_next) * v : v;
+          }
+        }
+        s_old = sa[0];
+        sa[0] = MODE == B_TILES && i < TM - 1 ? sa[1] * so : sa[1];
+        sa[1] = sa[2];
+        fa[0] = fa[1];
+        fa[1] = fa[2];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      so = so_next;
+      buf ^= 1;
+    }
+#pragma unroll
+    for (int n = LEN - LAG; n < LEN; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[TM - 1][n % TN][r] = fmaf(part[n][r], MODE == B_TILES ? s_old : MODE == A_TILES ? sb[n % TN][r] : s_old * sb[n % TN][r], acc[TM - 1][n % TN][r]);
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int m = m0 + wm * (BM / WM) + i * 16 + fr;
+    const int m = m0 + rm + i * 16;
     if (m >= p.m) continue;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -200,12 +288,12 @@ struct Plan {
   int splits, kb_split;
 };
 
-Plan prod_plan(int64_t m, int64_t n, int64_t kb) {
+Plan prod_plan(int64_t m, int64_t n, int64_t kb, bool bytes) {
   Plan q;
   q.bm = q.bn = 128;
   if (n <= 64)
     q.bn = 64;
-  else if (nmfk_div_up(m, 256) * nmfk_div_up(n, 256) >= 200)
+  else if (bytes && nmfk_div_up(m, 256) * nmfk_div_up(n, 256) >= 200)
     q.bm = q.bn = 256;
   const int64_t tiles = nmfk_div_up(m, q.bm) * nmfk_div_up(n, q.bn);
   // Few tiles leave most of the 256 CUs without one: split the sum, as long as a workgroup keeps four blocks.
@@ -215,12 +303,22 @@ Plan prod_plan(int64_t m, int64_t n, int64_t kb) {
   return q;
 }
 
-template <int BM, int BN, int WM, int WN, typename F, typename T, bool SPLIT>
-void prod_tile(const ProdArgs &p, int splits, hipStream_t st) {
+template <int BM, int BN, int WM, int WN, int MODE, typename F, typename T, bool SPLIT>
+void prod_tile_mode(const ProdArgs &p, int splits, hipStream_t st) {
   constexpr int BYTES = 2 * (BM + BN) * 132;
   static std::atomic<uint64_t> done{0};
-  nmfk_allow_dynamic_lds((const void *)prod_tile_kernel<BM, BN, WM, WN, F, T, SPLIT>, done, BYTES);
-  prod_tile_kernel<BM, BN, WM, WN, F, T, SPLIT><<<dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)splits), 64 * WM * WN, BYTES, st>>>(p);
+  nmfk_allow_dynamic_lds((const void *)prod_tile_kernel<BM, BN, WM, WN, MODE, F, T, SPLIT>, done, BYTES);
+  prod_tile_kernel<BM, BN, WM, WN, MODE, F, T, SPLIT><<<dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)splits), 64 * WM * WN, BYTES, st>>>(p);
+}
+
+template <int BM, int BN, int WM, int WN, typename F, typename T, bool SPLIT>
+void prod_tile(const ProdArgs &p, int splits, hipStream_t st) {
+  if (p.bshift)
+    prod_tile_mode<BM, BN, WM, WN, B_TILES, F, T, SPLIT>(p, splits, st);
+  else if (p.ashift)
+    prod_tile_mode<BM, BN, WM, WN, A_TILES, F, T, SPLIT>(p, splits, st);
+  else
+    prod_tile_mode<BM, BN, WM, WN, ROWS_ROWS, F, T, SPLIT>(p, splits, st);
 }
 
 template <typename F, typename T>
@@ -238,16 +336,19 @@ int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
     p.y = work;
     p.vec = p.n % 4 == 0;
     if (q.bn == 64)
-      prod_tile<128, 64, 4, 1, F, float, true>(p, q.splits, st);
+      prod_tile<128, 64, 2, 2, F, float, true>(p, q.splits, st);
     else
       prod_tile<128, 128, 2, 2, F, float, true>(p, q.splits, st);
     prod_join_kernel<T><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
   } else {
     p.vec = p.ldy % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
-    if (q.bn == 256)
-      prod_tile<256, 256, 2, 4, F, T, false>(p, 1, st);
-    else if (q.bn == 64)
-      prod_tile<128, 64, 4, 1, F, T, false>(p, 1, st);
+    if constexpr (std::is_same<F, Bytes>::value)
+      if (q.bn == 256) {
+        prod_tile<256, 256, 2, 4, F, T, false>(p, 1, st);
+        return nmfk_launched("nmfk_product");
+      }
+    if (q.bn == 64)
+      prod_tile<128, 64, 2, 2, F, T, false>(p, 1, st);
     else
       prod_tile<128, 128, 2, 2, F, T, false>(p, 1, st);
   }
@@ -264,12 +365,13 @@ int prod_sizes(int64_t m, int64_t n, int64_t k, const char *who) {
 
 }  // namespace
 
-NMFK_EXPORT int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int64_t *bytes) {
+NMFK_EXPORT int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes) {
   if (!bytes) return fail(NMFK_ERR_BAD_ARG, "nmfk_product_workspace: null pointer");
   if (int rc = prod_sizes(m, n, k, "nmfk_product_workspace")) return rc;
+  if (dtype < NMFK_F32 || dtype > NMFK_F16) return fail(NMFK_ERR_BAD_ARG, "nmfk_product_workspace: dtype must be NMFK_F32, NMFK_BF16 or NMFK_F16");
   *bytes = 0;
   if (m == 0 || n == 0 || k == 0) return NMFK_OK;
-  const Plan q = prod_plan(m, n, nmfk_div_up(k, 128));
+  const Plan q = prod_plan(m, n, nmfk_div_up(k, 128), dtype != NMFK_F32);
   if (q.splits > 1) *bytes = (int64_t)q.splits * m * n * 4;
   return NMFK_OK;
 }
@@ -284,12 +386,12 @@ NMFK_EXPORT int nmfk_product(int device, void *stream, int64_t m, int64_t n, int
   if (!Y || ldy < n) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: Y is needed, with ldy >= n");
   if (kb > 0) {
     if (!A || !B || !sA || !sB) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: null pointer");
-    if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)lda | (uintptr_t)ldb) & 15 || lda < kb * 128 || ldb < kb * 128)
-      return fail(NMFK_ERR_BAD_ARG, "nmfk_product: rows must be 16-byte aligned and hold whole blocks of 128");
+    if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)lda | (uintptr_t)ldb) & 15 || lda < kb * 128 || ldb < kb * 128 || lda > ((int64_t)1 << 23) || ldb > ((int64_t)1 << 23))
+      return fail(NMFK_ERR_BAD_ARG, "nmfk_product: rows must be 16-byte aligned, hold whole blocks of 128 and be at most 2^23 bytes apart");
     if (ldsa < (a_tiles ? nmfk_div_up(m, 128) : m) || ldsb < (b_tiles ? nmfk_div_up(n, 128) : n))
       return fail(NMFK_ERR_BAD_ARG, "nmfk_product: the leading dimension of the scales is too small");
   }
-  const Plan q = prod_plan(m, n, std::max<int64_t>(1, kb));
+  const Plan q = prod_plan(m, n, std::max<int64_t>(1, kb), dtype != NMFK_F32);
   if (kb > 0 && q.splits > 1 && (!work || work_bytes < (int64_t)q.splits * m * n * 4 || (uintptr_t)work % 16))
     return fail(NMFK_ERR_BAD_ARG, "nmfk_product: the workspace is too small or not 16-byte aligned (nmfk_product_workspace)");
   NmfkDeviceGuard guard(device);

@@ -150,7 +150,7 @@ def product(A, B, dtype=None, out=None):
             raise _bad(f"out must be {m} x {n} on {dev} with contiguous rows")
     L = _lib.lib()
     nb = C.c_int64()
-    _check(L.nmfk_product_workspace(m, n, k, C.byref(nb)))
+    _check(L.nmfk_product_workspace(m, n, k, _TYPES[out.dtype], C.byref(nb)))
     work = torch.empty(nb.value, dtype=torch.uint8, device=dev) if nb.value else None
     _check(L.nmfk_product(dev.index, _stream(dev), m, n, k, A._v.data_ptr(), A._v.shape[1], A._s.data_ptr(), A._s.shape[1], int(A.tiles),
                           B._v.data_ptr(), B._v.shape[1], B._s.data_ptr(), B._s.shape[1], int(B.tiles), _TYPES[out.dtype],

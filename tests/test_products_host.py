@@ -61,11 +61,11 @@ def test_product_of_nothing_sizes_and_workspace(NMFk):
     assert L.nmfk_product(*{**PROD, "m": 0}.values()) == 0
     assert L.nmfk_product(*{**PROD, "n": (1 << 22) + 1, "ldy": 1 << 23}.values()) == 6
     nb = C.c_int64()
-    assert L.nmfk_product_workspace(10, 20, 0, C.byref(nb)) == 0 and nb.value == 0
-    assert L.nmfk_product_workspace(10, 20, -1, C.byref(nb)) == 1
-    assert L.nmfk_product_workspace(10, 20, 5, None) == 1
+    assert L.nmfk_product_workspace(10, 20, 0, 0, C.byref(nb)) == 0 and nb.value == 0
+    assert L.nmfk_product_workspace(10, 20, -1, 0, C.byref(nb)) == 1
+    assert L.nmfk_product_workspace(10, 20, 5, 0, None) == 1
     # a long sum of few outputs is split: the workspace is asked for, and a call without it refused
-    assert L.nmfk_product_workspace(16, 64, 65536, C.byref(nb)) == 0 and nb.value > 0
+    assert L.nmfk_product_workspace(16, 64, 65536, 0, C.byref(nb)) == 0 and nb.value > 0
     big = {**PROD, "m": 16, "n": 64, "k": 65536, "lda": 65536, "ldb": 65536, "ldsa": 16, "ldsb": 64, "ldy": 64}
     for w in (dict(work=None), dict(wb=nb.value - 1), dict(work=PTR + 4)):
         assert L.nmfk_product(*{**big, **w}.values()) == 1
