@@ -501,79 +501,127 @@ struct GemmArgs {
   int vec;
 };
 
-// 128 x 128 outputs a workgroup, 64 x 64 a wave; two buffers of 128-byte rows in LDS.  The results of GRAM and POLY are symmetric: only the
-// tiles on and below the diagonal are computed, each is written to both places.
-template <int MODE, typename T>
-__global__ __launch_bounds__(256) void gemm_kernel(GemmArgs a) {
-  constexpr int STAGE = 256 * 128;
+// BM x BN outputs a workgroup, WM x WN waves.  The results of GRAM and POLY are symmetric: only the tiles on and below the diagonal are computed,
+// each is written to both places.
+// What bounds it is the matrix pipes: per block of 32 a 16 x 16 tile takes three instructions of 16 cycles.  Two buffers of 128-byte rows in LDS;
+// a wave holds Q's operands of a block in registers, so Q's half of a buffer is free after the first row of tiles and P's before the last
+// one: at these two places the waves meet and start the copies of the block after the next.  The operands of a row are requested a row ahead.
+template <int MODE, typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
+  constexpr int STAGE = (BM + BN) * 128, WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr bool SYM = MODE == GRAM || MODE == GRAM_PART || MODE == POLY;
+  static_assert(!SYM || BM == BN, "");
+  static_assert(TM >= 4, "Q is copied between row 1 and row TM - 2");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   int ti, tj;
-  constexpr bool SYM = MODE == GRAM || MODE == GRAM_PART || MODE == POLY;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
   if (SYM) {
-    const int id = blockIdx.x;
     ti = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);
     while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
     while (ti * (ti + 1) / 2 > id) --ti;
     tj = id - ti * (ti + 1) / 2;
   } else {
-    tile_at(xcd_order(blockIdx.x, gridDim.x), (a.m + 127) >> 7, a.tiles_n, 8, ti, tj);
+    tile_at(id, (a.m + BM - 1) / BM, a.tiles_n, BM == 256 ? 4 : 8, ti, tj);
   }
-  const int i0 = ti * 128, j0 = tj * 128;
+  const int i0 = ti * BM, j0 = tj * BN;
   const int64_t b = blockIdx.z;
   const int kb0 = MODE == GRAM_PART ? blockIdx.y * a.kb_split : 0, kb1 = MODE == GRAM_PART ? min(a.kb, kb0 + a.kb_split) : a.kb;
   const int lr = lane >> 3, lc = ((lane & 7) ^ lr) << 4;
-  const char *src[8];
+  // rows behind the last one repeat it (their results are not stored).  A lane's offset from its tile's first row: at most 256 rows of 2^24 + 128 bytes
+  constexpr int CP = BM / 8 / WAVES, CQ = BN / 8 / WAVES;
+  static_assert(CP * 8 * WAVES == BM && CQ * 8 * WAVES == BN, "");
+  const char *pp = a.p.p + b * a.p.batch + i0 * a.p.ld + (int64_t)kb0 * 128, *pq = a.q.p + b * a.q.batch + j0 * a.q.ld + (int64_t)kb0 * 128;
+  uint32_t off_p[CP], off_q[CQ];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int row = (k * 4 + w) * 8;
-    src[k] = row < 128 ? a.p.p + b * a.p.batch + (int64_t)min(i0 + row + lr, a.m - 1) * a.p.ld + lc
-                       : a.q.p + b * a.q.batch + (int64_t)min(j0 + row - 128 + lr, a.n - 1) * a.q.ld + lc;
-  }
-  auto stage = [&](int kb, int buf) {
+  for (int k = 0; k < CP; ++k) off_p[k] = (uint32_t)min((k * WAVES + w) * 8 + lr, a.m - 1 - i0) * (uint32_t)a.p.ld + lc;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) stage8(src[k] + (int64_t)kb * 128, lds + buf * STAGE + (k * 4 + w) * 1024);
+  for (int k = 0; k < CQ; ++k) off_q[k] = (uint32_t)min((k * WAVES + w) * 8 + lr, a.n - 1 - j0) * (uint32_t)a.q.ld + lc;
+  auto stage_p = [&](int buf) {
+#pragma unroll
+    for (int k = 0; k < CP; ++k) stage8(pp + off_p[k], lds + buf * STAGE + (k * WAVES + w) * 1024);
+    pp += 128;
   };
-  f32x4 acc[4][4];
+  auto stage_q = [&](int buf) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int k = 0; k < CQ; ++k) stage8(pq + off_q[k], lds + buf * STAGE + BM * 128 + (k * WAVES + w) * 1024);
+    pq += 128;
+  };
+  f32x4 acc[TM][TN];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const int fr = lane & 15, fg = lane >> 4, wi = (w / WN) * (BM / WM), wj = (w % WN) * (BN / WN);
+  auto frag_p = [&](int buf, int i, int half) { return __builtin_bit_cast(f16x8, lds_chunk(lds + buf * STAGE, wi + i * 16 + fr, fg + 4 * half)); };
+  auto frag_q = [&](int buf, int j, int half) { return __builtin_bit_cast(f16x8, lds_chunk(lds + buf * STAGE + BM * 128, wj + j * 16 + fr, fg + 4 * half)); };
   if (kb0 < kb1) {
-    stage(kb0, 0);
+    stage_p(0);
+    stage_q(0);
     staged();
-  }
-  __syncthreads();
-  const int fr = lane & 15, fg = lane >> 4, wi = (w >> 1) * 64, wj = (w & 1) * 64;
-  for (int kb = kb0, buf = 0; kb < kb1; ++kb, buf ^= 1) {
-    if (kb + 1 < kb1) stage(kb + 1, buf ^ 1);
-    const char *lp = lds + buf * STAGE, *lq = lp + 128 * 128;
-    f16x8 qh[4], ql[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      qh[j] = __builtin_bit_cast(f16x8, lds_chunk(lq, wj + j * 16 + fr, fg));
-      ql[j] = __builtin_bit_cast(f16x8, lds_chunk(lq, wj + j * 16 + fr, fg + 4));
+    meet();
+    if (kb0 + 1 < kb1) {
+      stage_p(1);
+      stage_q(1);
     }
+    f16x8 qh[TN], ql[TN], ph = frag_p(0, 0, 0), pl = frag_p(0, 0, 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f16x8 ph = __builtin_bit_cast(f16x8, lds_chunk(lp, wi + i * 16 + fr, fg));
-      const f16x8 pl = __builtin_bit_cast(f16x8, lds_chunk(lp, wi + i * 16 + fr, fg + 4));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph, acc[i][j], 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph, acc[i][j], 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl, acc[i][j], 0, 0, 0);
+    for (int j = 0; j < TN; ++j) {
+      qh[j] = frag_q(0, j, 0);
+      ql[j] = frag_q(0, j, 1);
     }
-    staged();
-    __syncthreads();
+    int buf = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {  // (behind the last block the operands of "the next" are whatever stands in LDS, unused)
+      const bool copy = kb + 2 < kb1;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if (i == 1 && copy) {
+          meet();
+          stage_q(buf);
+        }
+        f16x8 ph_next, pl_next;
+        if (i < TM - 1) {
+          ph_next = frag_p(buf, i + 1, 0);
+          pl_next = frag_p(buf, i + 1, 1);
+        } else {
+          if (copy) {
+            staged_but<CQ>();  // of the block after the next, Q may still be on its way
+            meet();
+            stage_p(buf);
+          } else {
+            staged();
+            meet();
+          }
+          ph_next = frag_p(buf ^ 1, 0, 0);
+          pl_next = frag_p(buf ^ 1, 0, 1);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph, acc[i][j], 0, 0, 0);
+        if (i == TM - 1) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) ql[j] = frag_q(buf ^ 1, j, 1);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl, acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph, acc[i][j], 0, 0, 0);
+        if (i == TM - 1) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) qh[j] = frag_q(buf ^ 1, j, 0);
+        }
+        ph = ph_next;
+        pl = pl_next;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      buf ^= 1;
+    }
   }
   const int mp = (a.m + 31) & ~31, np = (a.n + 31) & ~31;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < TM; ++i) {
     const int m = i0 + wi + i * 16 + fr;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < TN; ++j) {
       const int n = j0 + wj + j * 16 + fg * 4;
       f32x4 v = acc[i][j];
       if (MODE == GRAM_PART) {
@@ -764,18 +812,36 @@ int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, 
   return nmfk_launched("nmfk_orthogonalize");
 }
 
-template <int MODE, typename T>
-void gemm(const GemmArgs &a, dim3 grid, hipStream_t st) {
-  constexpr int BYTES = 2 * 256 * 128;
+template <int MODE, typename T, int BM, int BN, int WM, int WN>
+void gemm_tile(const GemmArgs &a, dim3 grid, hipStream_t st) {
+  constexpr int BYTES = 2 * (BM + BN) * 128;
   static std::atomic<uint64_t> done{0};
-  nmfk_allow_dynamic_lds((const void *)gemm_kernel<MODE, T>, done, BYTES);
-  gemm_kernel<MODE, T><<<grid, 256, BYTES, st>>>(a);
+  nmfk_allow_dynamic_lds((const void *)gemm_kernel<MODE, T, BM, BN, WM, WN>, done, BYTES);
+  gemm_kernel<MODE, T, BM, BN, WM, WN><<<grid, 64 * WM * WN, BYTES, st>>>(a);
+}
+
+// S or its polynomial: the tiles on and below the diagonal
+template <int MODE>
+void gemm_sym(const GemmArgs &a, unsigned splits, unsigned batch, hipStream_t st) {
+  const unsigned tm = (unsigned)nmfk_div_up(a.m, 128);
+  gemm_tile<MODE, float, 128, 128, 2, 2>(a, dim3(tm * (tm + 1) / 2, splits, batch), st);
+}
+
+template <int MODE, typename T>
+void gemm_full(GemmArgs a, unsigned batch, hipStream_t st) {
+  const int64_t big = nmfk_div_up(a.m, 256) * nmfk_div_up(a.n, 256);
+  if (big * batch >= 200) {
+    a.tiles_n = (int)nmfk_div_up(a.n, 256);
+    gemm_tile<MODE, T, 256, 256, 2, 4>(a, dim3((unsigned)big, 1, batch), st);
+  } else {
+    a.tiles_n = (int)nmfk_div_up(a.n, 128);
+    gemm_tile<MODE, T, 128, 128, 2, 2>(a, dim3((unsigned)(nmfk_div_up(a.m, 128) * a.tiles_n), 1, batch), st);
+  }
 }
 
 template <typename T>
 int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, const double *coef, char *work, hipStream_t st) {
   const int s = (int)y.s, l = (int)y.l;
-  const unsigned tm = (unsigned)nmfk_div_up(s, 128), tl = (unsigned)nmfk_div_up(l, 128), sym = tm * (tm + 1) / 2;
   const int64_t bx = y.s * y.ldx, bt = y.l * y.ldt, bs = y.s * y.ldt;
   for (int64_t b0 = 0; b0 < y.batch; b0 += 32768) {
     const unsigned nb = (unsigned)std::min<int64_t>(32768, y.batch - b0);
@@ -795,22 +861,21 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
       a.kb = (int)nmfk_div_up(l, 32);
       a.mul = (float)ldexp(1.0, es - 2 * ex);
       a.out = a.out_t = S;
-      a.tiles_n = (int)tm;
       a.splits = (int)y.splits;
       a.kb_split = (int)y.kb_split;
       if (y.splits > 1) {
         a.part = (float *)(work + y.part) + b0 * y.splits * y.s * y.s;
-        gemm<GRAM_PART, T>(a, dim3(sym, (unsigned)y.splits, nb), st);
+        gemm_sym<GRAM_PART>(a, (unsigned)y.splits, nb, st);
         gram_join_kernel<<<dim3((unsigned)nmfk_div_up((int64_t)s * (y.ldt / 4), 1024), 1, nb), 256, 0, st>>>(a);
       } else {
-        gemm<GRAM, T>(a, dim3(sym, 1, nb), st);
+        gemm_sym<GRAM>(a, 1, nb, st);
       }
       a.p = a.q = a.d = S;
       a.kb = (int)nmfk_div_up(s, 32);
       a.add = (float)(cb * ldexp(1.0, eb - es));
       a.mul = (float)(cc * ldexp(1.0, eb - 2 * es));
       a.out = a.out_t = B;
-      gemm<POLY, T>(a, dim3(sym, 1, nb), st);
+      gemm_sym<POLY>(a, 1, nb, st);
       u = std::max(peak(ca, cb, cc, u, true), 1e-3);
       const bool last = k + 1 == steps;
       const int nx = last ? 0 : exponent(1.02 * u);
@@ -818,7 +883,6 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
       a.q = XT;
       a.d = X;
       a.n = l;
-      a.tiles_n = (int)tl;
       a.add = (float)(ca * ldexp(1.0, nx - ex));
       a.mul = (float)ldexp(1.0, nx - eb - ex);
       a.out = X;  // the entry [i, j] of X is read by the lane that overwrites it, and by no other
@@ -827,9 +891,9 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
         a.o = o;
         a.b0 = b0;
         a.vec = o.col == 1 && o.row % 4 == 0 && o.batch % 4 == 0 && (uintptr_t)o.p % (4 * sizeof(T)) == 0;
-        gemm<LAST, T>(a, dim3(tm * tl, 1, nb), st);
+        gemm_full<LAST, T>(a, nb, st);
       } else {
-        gemm<APPLY, T>(a, dim3(tm * tl, 1, nb), st);
+        gemm_full<APPLY, float>(a, nb, st);
       }
       std::swap(XT, NT);
       ex = nx;
