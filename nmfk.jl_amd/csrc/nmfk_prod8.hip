@@ -264,15 +264,99 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
   }
 }
 
+// Few rows of A (m <= 16 TA): what bounds it is the one read of B.  A workgroup owns 16 TB columns of Y; its eight waves take the blocks of the sum in
+// turn, the operands go from memory straight into registers (a row's 128 bytes are read by four lanes), and the waves' sums are added in
+// their order through LDS.  One row against 4096 x 4096: @@ONE@@
+template <int TA, int TB, typename F, typename T, bool SPLIT>
+__global__ __launch_bounds__(512) void prod_rows_kernel(ProdArgs p) {
+  __shared__ __attribute__((aligned(16))) float sum[8][TA * TB * 256];
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, fr = lane & 15, fg = lane >> 4;
+  const int n0 = blockIdx.x * 16 * TB;
+  const int kb0 = blockIdx.y * p.kb_split, kb1 = min(p.kb, kb0 + p.kb_split);
+  const char *pa[TA], *pb[TB];
+  const float *sa[TA], *sb[TB][4];
+#pragma unroll
+  for (int i = 0; i < TA; ++i) {
+    const int r = min(16 * i + fr, p.m - 1);
+    pa[i] = p.a + (int64_t)r * p.lda + fg * 16;
+    sa[i] = p.sa + (r >> p.ashift);
+  }
+#pragma unroll
+  for (int j = 0; j < TB; ++j) {
+    pb[j] = p.b + (int64_t)min(n0 + 16 * j + fr, p.n - 1) * p.ldb + fg * 16;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sb[j][r] = p.sb + (min(n0 + 16 * j + fg * 4 + r, p.n - 1) >> p.bshift);
+  }
+  f32x4 acc[TA][TB];
+#pragma unroll
+  for (int i = 0; i < TA; ++i)
+#pragma unroll
+    for (int j = 0; j < TB; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll(TA * TB <= 2 ? 4 : 2)
+  for (int kb = kb0 + w; kb < kb1; kb += 8) {
+    const int64_t o = (int64_t)kb * 128;
+    F fb[TB];
+    float s[TB][4];
+#pragma unroll
+    for (int j = 0; j < TB; ++j) {
+      fb[j] = F(*(const i32x4 *)(pb[j] + o), *(const i32x4 *)(pb[j] + o + 64));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[j][r] = sb[j][r][kb * p.ldsb];
+    }
+#pragma unroll
+    for (int i = 0; i < TA; ++i) {
+      const F fa(*(const i32x4 *)(pa[i] + o), *(const i32x4 *)(pa[i] + o + 64));
+      const float x = sa[i][kb * p.ldsa];
+#pragma unroll
+      for (int j = 0; j < TB; ++j) {
+        f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < F::STEPS; ++q) part = block_step(fb[j], fa, part, q);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(part[r], x * s[j][r], acc[i][j][r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TA; ++i)
+#pragma unroll
+    for (int j = 0; j < TB; ++j) *(f32x4 *)&sum[w][((i * TB + j) * 64 + lane) * 4] = acc[i][j];
+  __syncthreads();
+  for (int e = t; e < TA * TB * 64; e += 512) {
+    f32x4 v = *(const f32x4 *)&sum[0][e * 4];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += *(const f32x4 *)&sum[k][e * 4];
+    const int l = e & 63, i = (e >> 6) / TB, j = (e >> 6) % TB;
+    const int m = 16 * i + (l & 15), n = n0 + 16 * j + (l >> 4) * 4;
+    if (m >= p.m || n >= p.n) continue;
+    if (SPLIT)
+      store4<float>((float *)p.y + ((int64_t)blockIdx.y * p.m + m) * p.n + n, v, p.n - n, p.vec);
+    else
+      store4<T>((T *)p.y + m * p.ldy + n, v, p.n - n, p.vec);
+  }
+}
+
 // sums the splits in their order: the same bits on every run
-template <typename T>
+template <typename T, int V>
 __global__ __launch_bounds__(256) void prod_join_kernel(const float *part, int splits, int64_t m, int64_t n, T *y, int64_t ldy) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= m * n) return;
-  float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[(int64_t)k * m * n + i];
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, mn = m * n;
+  if (i >= mn) return;
+  float s[V] = {};
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) {
+    const float *q = part + k * mn + i;
+    if (V == 4) {
+      const f32x4 v = *(const f32x4 *)q;
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] += v[e];
+    } else {
+      s[0] += *q;
+    }
+  }
   const int64_t r = i / n;
-  y[r * ldy + (i - r * n)] = from_f32<T>(s);
+  T *z = y + r * ldy + (i - r * n);
+#pragma unroll
+  for (int e = 0; e < V; ++e) z[e] = from_f32<T>(s[e]);
 }
 
 template <typename T>
@@ -284,20 +368,28 @@ __global__ __launch_bounds__(256) void prod_zero_kernel(T *y, int64_t m, int64_t
 }
 
 struct Plan {
-  int bm, bn;
+  int bm, bn;  // bm <= 64: prod_rows_kernel with 16 * (bm / 16) rows and bn columns a workgroup
   int splits, kb_split;
 };
 
 Plan prod_plan(int64_t m, int64_t n, int64_t kb, bool bytes) {
   Plan q;
-  q.bm = q.bn = 128;
-  if (n <= 64)
-    q.bn = 64;
-  else if (bytes && nmfk_div_up(m, 256) * nmfk_div_up(n, 256) >= 200)
-    q.bm = q.bn = 256;
-  const int64_t tiles = nmfk_div_up(m, q.bm) * nmfk_div_up(n, q.bn);
-  // Few tiles leave most of the 256 CUs without one: split the sum, as long as a workgroup keeps four blocks.
-  int64_t splits = tiles >= 256 ? 1 : std::min<int64_t>(512 / tiles, nmfk_div_up(kb, 4));
+  int64_t splits = 1;
+  if (m <= 64 && n > m) {
+    q.bm = m <= 16 ? 16 : m <= 32 ? 32 : 64;
+    q.bn = q.bm > 16 && n >= 8192 ? 32 : 16;
+    const int64_t groups = nmfk_div_up(n, q.bn);  // of eight waves: two for each CU, and at least two blocks for each wave
+    if (groups < 256) splits = std::min<int64_t>(512 / groups, kb / 16);
+  } else {
+    q.bm = q.bn = 128;
+    if (n <= 64)
+      q.bn = 64;
+    else if (bytes && nmfk_div_up(m, 256) * nmfk_div_up(n, 256) >= 200)
+      q.bm = q.bn = 256;
+    const int64_t tiles = nmfk_div_up(m, q.bm) * nmfk_div_up(n, q.bn);
+    // Few tiles leave most of the 256 CUs without one: split the sum, as long as a workgroup keeps four blocks.
+    if (tiles < 256) splits = std::min<int64_t>(512 / tiles, nmfk_div_up(kb, 4));
+  }
   q.kb_split = (int)nmfk_div_up(kb, std::max<int64_t>(1, splits));
   q.splits = (int)std::max<int64_t>(1, nmfk_div_up(kb, q.kb_split));
   return q;
@@ -321,6 +413,33 @@ void prod_tile(const ProdArgs &p, int splits, hipStream_t st) {
     prod_tile_mode<BM, BN, WM, WN, ROWS_ROWS, F, T, SPLIT>(p, splits, st);
 }
 
+template <typename F, typename T, bool SPLIT>
+void prod_launch(const ProdArgs &p, const Plan &q, hipStream_t st) {
+  if (q.bm <= 64) {
+    const dim3 grid((unsigned)nmfk_div_up(p.n, q.bn), (unsigned)q.splits);
+    if (q.bm == 16)
+      prod_rows_kernel<1, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
+    else if (q.bm == 32 && q.bn == 16)
+      prod_rows_kernel<2, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
+    else if (q.bm == 32)
+      prod_rows_kernel<2, 2, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
+    else if (q.bn == 16)
+      prod_rows_kernel<4, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
+    else
+      prod_rows_kernel<4, 2, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
+    return;
+  }
+  if constexpr (std::is_same<F, Bytes>::value && !SPLIT)
+    if (q.bn == 256) {
+      prod_tile<256, 256, 2, 4, F, T, false>(p, 1, st);
+      return;
+    }
+  if (q.bn == 64)
+    prod_tile<128, 64, 2, 2, F, T, SPLIT>(p, q.splits, st);
+  else
+    prod_tile<128, 128, 2, 2, F, T, SPLIT>(p, q.splits, st);
+}
+
 template <typename F, typename T>
 int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
   const int64_t mn = (int64_t)p.m * p.n;
@@ -335,22 +454,14 @@ int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
   if (q.splits > 1) {
     p.y = work;
     p.vec = p.n % 4 == 0;
-    if (q.bn == 64)
-      prod_tile<128, 64, 2, 2, F, float, true>(p, q.splits, st);
+    prod_launch<F, float, true>(p, q, st);
+    if (p.vec)
+      prod_join_kernel<T, 4><<<dim3((unsigned)nmfk_div_up(mn, 1024)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
     else
-      prod_tile<128, 128, 2, 2, F, float, true>(p, q.splits, st);
-    prod_join_kernel<T><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
+      prod_join_kernel<T, 1><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
   } else {
     p.vec = p.ldy % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
-    if constexpr (std::is_same<F, Bytes>::value)
-      if (q.bn == 256) {
-        prod_tile<256, 256, 2, 4, F, T, false>(p, 1, st);
-        return nmfk_launched("nmfk_product");
-      }
-    if (q.bn == 64)
-      prod_tile<128, 64, 2, 2, F, T, false>(p, 1, st);
-    else
-      prod_tile<128, 128, 2, 2, F, T, false>(p, 1, st);
+    prod_launch<F, T, false>(p, q, st);
   }
   return nmfk_launched("nmfk_product");
 }

@@ -31,8 +31,35 @@ __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;
 }
-__device__ __forceinline__ float quotient(float x, float s) {
-  return fabsf(x) <= 3.402823466e38f ? x / s : __uint_as_float(0x7fc00000u);
+// x / s rounded to nearest, for the many x of a block: with r = 1 / s rounded to nearest, q0 = x r, one correction q0 + r (x - q0 s) gives the
+// correctly rounded quotient (Markstein's theorem) unless the significand of s is all ones.  The residual has to be exact: s in [2^-80, 2^80] makes
+// it so for every quotient that does not round to zero in e4m3.  Elsewhere: the division (11 instructions instead of 3).  NaN and infinities come
+// out as NaN by themselves.
+struct Divisor {
+  float s, r;
+  bool easy;
+  __device__ __forceinline__ explicit Divisor(float scale) : s(scale), r(1.0f / scale) {
+    easy = scale >= 0x1p-80f && scale <= 0x1p80f && (__float_as_uint(scale) & 0x7fffffu) != 0x7fffffu;
+  }
+};
+__device__ __forceinline__ float quotient(float x, const Divisor &d) {
+  if (d.easy) {
+    const float q = x * d.r;
+    return fmaf(fmaf(-q, d.s, x), d.r, q);
+  }
+  return fabsf(x) <= 3.402823466e38f ? x / d.s : __uint_as_float(0x7fc00000u);
+}
+// the largest of 32 lanes, in all of them: rotations within 16 lanes on the vector unit, then one exchange
+template <int CTRL>
+__device__ __forceinline__ float rotate(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float largest32(float m) {
+  m = fmaxf(m, rotate<0x128>(m));  // row_ror:8
+  m = fmaxf(m, rotate<0x124>(m));
+  m = fmaxf(m, rotate<0x122>(m));
+  m = fmaxf(m, rotate<0x121>(m));
+  return fmaxf(m, __shfl_xor(m, 16));
 }
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -62,10 +89,9 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a, int64_t bl
   float x[4];
   load4<T>(a, r, c, x);
   float top = fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float s = block_scale(top);
-  *(uint32_t *)(a.v + r * a.ldv + c) = pack4(quotient(x[0], s), quotient(x[1], s), quotient(x[2], s), quotient(x[3], s));
+  const float s = block_scale(largest32(top));
+  const Divisor d(s);
+  *(uint32_t *)(a.v + r * a.ldv + c) = pack4(quotient(x[0], d), quotient(x[1], d), quotient(x[2], d), quotient(x[3], d));
   if ((threadIdx.x & 31) == 0) a.s[kb * a.sld + r] = s;
 }
 
@@ -103,10 +129,7 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
       for (int h = 0; h < 8; ++h) cmax[j] = fmaxf(cmax[j], ctop[h][cg * 4 + j]);
   }
   if (TILES) {
-    float m = fmaxf(fmaxf(cmax[0], cmax[1]), fmaxf(cmax[2], cmax[3]));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    tile_s = block_scale(m);
+    tile_s = block_scale(largest32(fmaxf(fmaxf(cmax[0], cmax[1]), fmaxf(cmax[2], cmax[3]))));
     if (t == 0) {
       if (a.v) a.s[(int64_t)blockIdx.x * a.sld + blockIdx.y] = tile_s;
       if (a.tv) a.ts[(int64_t)blockIdx.y * a.tsld + blockIdx.x] = tile_s;
@@ -116,14 +139,9 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
   if (a.v || TILES) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float s = tile_s;
-      if (!TILES) {
-        float m = rmax[i];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        s = block_scale(m);
-      }
-      q[i] = pack4(quotient(x[i][0], s), quotient(x[i][1], s), quotient(x[i][2], s), quotient(x[i][3], s));
+      const float s = TILES ? tile_s : block_scale(largest32(rmax[i]));
+      const Divisor d(s);
+      q[i] = pack4(quotient(x[i][0], d), quotient(x[i][1], d), quotient(x[i][2], d), quotient(x[i][3], d));
       const int64_t r = r0 + g * 16 + i;
       if (a.v && r < a.rows) {
         *(uint32_t *)(a.v + r * a.ldv + c0 + cg * 4) = q[i];
@@ -146,10 +164,11 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
       }
     } else {
       const float s = block_scale(cmax[j]);
+      const Divisor d(s);
       if (g == 0 && c0 + c < a.cols) a.ts[(int64_t)blockIdx.y * a.tsld + c0 + c] = s;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        w[k] = (int)pack4(quotient(x[k * 4][j], s), quotient(x[k * 4 + 1][j], s), quotient(x[k * 4 + 2][j], s), quotient(x[k * 4 + 3][j], s));
+        w[k] = (int)pack4(quotient(x[k * 4][j], d), quotient(x[k * 4 + 1][j], d), quotient(x[k * 4 + 2][j], d), quotient(x[k * 4 + 3][j], d));
     }
     *(i32x4 *)(turn + c * 128 + ((g ^ (cg & 7)) << 4)) = w;
   }

@@ -5,6 +5,7 @@
 The operators take and return torch tensors on the GPU; they run on torch's current stream of the tensors' device, do not wait, and can be
 captured into a graph.  `rangebasis` takes a numpy array like `execute` does, or a tensor."""
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -17,16 +18,18 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 # three more of the steps that converge (error^3 in each) make the columns orthonormal to 32 bits
 CONVERGING = (1.875, -1.25, 0.375)
 
-_TYPES = None
+_TYPES = _U8 = _F8 = _F32 = _TORCH = None
 
 
 def _torch():
-    global _TYPES
-    import torch
+    """torch, imported when the first of these operators is called (the rest of the package does without)"""
+    global _TYPES, _U8, _F8, _F32, _TORCH
+    if _TORCH is None:
+        import torch
 
-    if _TYPES is None:
         _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    return torch
+        _U8, _F8, _F32, _TORCH = torch.uint8, torch.float8_e4m3fn, torch.float32, torch
+    return _TORCH
 
 
 def _bad(msg):
@@ -35,11 +38,11 @@ def _bad(msg):
 
 def _tensor(x, name, ndim=2):
     torch = _torch()
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise _bad(f"{name} must be a torch tensor on the GPU")
     if x.dtype not in _TYPES:
         raise _bad(f"{name} must be float32, bfloat16 or float16, not {x.dtype}")
-    if x.dim() < ndim or (ndim == 2 and x.dim() != 2):
+    if ndim and x.dim() != ndim:
         raise _bad(f"{name} must be a matrix")
     if x.requires_grad and torch.is_grad_enabled():
         raise _bad(f"{name} requires a gradient, which this operator does not record: pass {name}.detach()")
@@ -47,7 +50,33 @@ def _tensor(x, name, ndim=2):
 
 
 def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+    raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)  # (a tenth of the time that a Stream object takes to make)
+    return raw(device.index) if raw else _torch().cuda.current_stream(device).cuda_stream
+
+
+@functools.lru_cache(4096)
+def _product_workspace(m, n, k, t):
+    nb = C.c_int64()
+    _check(_lib.lib().nmfk_product_workspace(m, n, k, t, C.byref(nb)))
+    return nb.value
+
+
+@functools.lru_cache(4096)
+def _orthogonalize_workspace(b, r, c):
+    nb = C.c_int64()
+    _check(_lib.lib().nmfk_orthogonalize_workspace(b, r, c, C.byref(nb)))
+    return nb.value
+
+
+@functools.lru_cache(64)
+def _coefficients(key, steps):
+    cf = np.asarray(key, dtype=np.float64)
+    if cf.shape == (3,):
+        cf = np.broadcast_to(cf, (steps, 3))
+    if cf.shape != (steps, 3):
+        raise _bad(f"coefficients must be (a, b, c) or {steps} such triples")
+    cf = np.ascontiguousarray(cf)
+    return cf, cf.ctypes.data
 
 
 class Quantized:
@@ -57,7 +86,7 @@ class Quantized:
     scales   float32 (rows, ceil(cols / 128)), tiles: (ceil(rows / 128), ceil(cols / 128))
     The matrix is values * scales.  Quantized(values, scales, tiles) takes a matrix quantized elsewhere and lays it out once."""
 
-    __slots__ = ("shape", "tiles", "_v", "_s", "__weakref__")
+    __slots__ = ("shape", "tiles", "device", "_buf", "_ldv", "_lds", "_pv", "_ps")
 
     def __init__(self, values, scales, tiles=False):
         torch = _torch()
@@ -70,38 +99,41 @@ class Quantized:
         if tuple(scales.shape) != ((-(-r // 128) if tiles else r), kb):
             raise _bad(f"{'tiles' if tiles else 'rows'} of a {r} x {c} matrix have {(-(-r // 128) if tiles else r)} x {kb} scales, not {tuple(scales.shape)}")
         self._make(r, c, bool(tiles), values.device)
-        self._v[:, :c].copy_(values.view(torch.uint8))
-        if c < self._v.shape[1]:
-            self._v[:, c:].zero_()
-        self._s.copy_(scales.t())
+        v = self._values()
+        v[:, :c].copy_(values.view(torch.uint8))
+        if c < self._ldv:
+            v[:, c:].zero_()
+        self.scales.copy_(scales)
 
     def _make(self, r, c, tiles, device):
-        torch = _torch()
+        # one allocation: r rows of whole blocks, then the scales block by block (kb x r, or kb x tiles)
         kb = -(-c // 128)
-        self.shape, self.tiles = (r, c), tiles
-        self._v = torch.empty((r, kb * 128), dtype=torch.uint8, device=device)
-        self._s = torch.empty((kb, -(-r // 128) if tiles else r), dtype=torch.float32, device=device)
+        self.shape, self.tiles, self.device = (r, c), tiles, device
+        self._ldv, self._lds = kb * 128, -(-r // 128) if tiles else r
+        self._buf = _torch().empty(r * self._ldv + 4 * kb * self._lds, dtype=_U8, device=device)
+        self._pv = self._buf.data_ptr()
+        self._ps = self._pv + r * self._ldv
         return self
+
+    def _values(self):
+        return self._buf[: self.shape[0] * self._ldv].view(self.shape[0], self._ldv)
 
     @property
     def values(self):
-        return self._v.view(_torch().float8_e4m3fn)[:, : self.shape[1]]
+        r, c = self.shape
+        return self._buf.view(_F8).as_strided((r, c), (self._ldv, 1))
 
     @property
     def scales(self):
-        return self._s.t()
-
-    @property
-    def device(self):
-        return self._v.device
+        r = self.shape[0]
+        return self._buf[r * self._ldv:].view(_F32).as_strided((self._lds, self._ldv // 128), (1, self._lds))
 
     def dequantize(self, dtype=None):
         """the matrix that values and scales stand for (float32 unless told otherwise)"""
-        torch = _torch()
-        s = self._s.t().repeat_interleave(128, 1)[:, : self.shape[1]]
+        s = self.scales.repeat_interleave(128, 1)[:, : self.shape[1]]
         if self.tiles:
             s = s.repeat_interleave(128, 0)[: self.shape[0]]
-        return (self.values.float() * s).to(dtype or torch.float32)
+        return (self.values.float() * s).to(dtype or _F32)
 
 
 def quantize(X, tiles=False, both=False):
@@ -115,13 +147,14 @@ def quantize(X, tiles=False, both=False):
     if not (sc == 1 and (sr >= c or r == 1)) and not (sr == 1 and (sc >= r or c == 1)):
         X = X.contiguous()
         sr, sc = X.stride()
-    q = Quantized.__new__(Quantized)._make(r, c, bool(tiles), X.device)
-    t = Quantized.__new__(Quantized)._make(c, r, bool(tiles), X.device) if both else None
-    _check(_lib.lib().nmfk_quantize(X.device.index, _stream(X.device), _TYPES[X.dtype], X.data_ptr(), r, c, sr, sc, int(q.tiles),
-                                    q._v.data_ptr(), q._v.shape[1], q._s.data_ptr(), q._s.shape[1],
-                                    t._v.data_ptr() if both else None, t._v.shape[1] if both else 0,
-                                    t._s.data_ptr() if both else None, t._s.shape[1] if both else 0))
-    return (q, t) if both else q
+    dev, tiles = X.device, bool(tiles)
+    q = Quantized.__new__(Quantized)._make(r, c, tiles, dev)
+    if not both:
+        _check(_lib.lib().nmfk_quantize(dev.index, _stream(dev), _TYPES[X.dtype], X.data_ptr(), r, c, sr, sc, tiles, q._pv, q._ldv, q._ps, q._lds, None, 0, None, 0))
+        return q
+    t = Quantized.__new__(Quantized)._make(c, r, tiles, dev)
+    _check(_lib.lib().nmfk_quantize(dev.index, _stream(dev), _TYPES[X.dtype], X.data_ptr(), r, c, sr, sc, tiles, q._pv, q._ldv, q._ps, q._lds, t._pv, t._ldv, t._ps, t._lds))
+    return q, t
 
 
 def _quantized(x, name):
@@ -148,13 +181,11 @@ def product(A, B, dtype=None, out=None):
         _tensor(out, "out")
         if tuple(out.shape) != (m, n) or out.device != dev or (dtype is not None and out.dtype != dtype) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
             raise _bad(f"out must be {m} x {n} on {dev} with contiguous rows")
-    L = _lib.lib()
-    nb = C.c_int64()
-    _check(L.nmfk_product_workspace(m, n, k, _TYPES[out.dtype], C.byref(nb)))
-    work = torch.empty(nb.value, dtype=torch.uint8, device=dev) if nb.value else None
-    _check(L.nmfk_product(dev.index, _stream(dev), m, n, k, A._v.data_ptr(), A._v.shape[1], A._s.data_ptr(), A._s.shape[1], int(A.tiles),
-                          B._v.data_ptr(), B._v.shape[1], B._s.data_ptr(), B._s.shape[1], int(B.tiles), _TYPES[out.dtype],
-                          out.data_ptr(), out.stride(0) if m > 1 else n, work.data_ptr() if work is not None else None, nb.value))
+    t = _TYPES[out.dtype]
+    nb = _product_workspace(m, n, k, t)
+    work = torch.empty(nb, dtype=_U8, device=dev) if nb else None
+    _check(_lib.lib().nmfk_product(dev.index, _stream(dev), m, n, k, A._pv, A._ldv, A._ps, A._lds, A.tiles, B._pv, B._ldv, B._ps, B._lds, B.tiles, t,
+                                   out.data_ptr(), out.stride(0) if m > 1 else n, work.data_ptr() if nb else None, nb))
     return out
 
 
@@ -186,12 +217,12 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
     steps = int(steps)
     if steps < 1 or steps > 32:
         raise _bad("1 to 32 steps")
-    cf = np.asarray(COEFFICIENTS if coefficients is None else coefficients, dtype=np.float64)
-    if cf.shape == (3,):
-        cf = np.broadcast_to(cf, (steps, 3))
-    if cf.shape != (steps, 3):
-        raise _bad(f"coefficients must be (a, b, c) or {steps} such triples")
-    cf = np.ascontiguousarray(cf)
+    if coefficients is None:
+        key = COEFFICIENTS
+    else:
+        cf = np.asarray(coefficients, dtype=np.float64)
+        key = tuple(cf.tolist()) if cf.ndim == 1 else tuple(map(tuple, cf.tolist())) if cf.ndim == 2 else ()
+    cf, cf_at = _coefficients(key, steps)
     if out is None:
         out = torch.empty_like(G)
     else:
@@ -201,12 +232,10 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
     g = G if G.dim() == 3 else G.unsqueeze(0) if G.dim() == 2 else G.reshape(-1, *G.shape[-2:])
     o = out if out.dim() == 3 else out.unsqueeze(0) if out.dim() == 2 else out.view(-1, *out.shape[-2:])
     b, r, c = g.shape
-    L = _lib.lib()
-    nb = C.c_int64()
-    _check(L.nmfk_orthogonalize_workspace(b, r, c, C.byref(nb)))
-    work = torch.empty(nb.value, dtype=torch.uint8, device=G.device) if nb.value else None
-    _check(L.nmfk_orthogonalize(G.device.index, _stream(G.device), _TYPES[G.dtype], b, r, c, g.data_ptr(), *g.stride(), o.data_ptr(), *o.stride(),
-                                steps, cf.ctypes.data, work.data_ptr() if work is not None else None, nb.value))
+    dev, nb = G.device, _orthogonalize_workspace(b, r, c)
+    work = torch.empty(nb, dtype=_U8, device=dev) if nb else None
+    _check(_lib.lib().nmfk_orthogonalize(dev.index, _stream(dev), _TYPES[G.dtype], b, r, c, g.data_ptr(), *g.stride(), o.data_ptr(), *o.stride(),
+                                         steps, cf_at, work.data_ptr() if nb else None, nb))
     return out
 
 

@@ -67,7 +67,7 @@ def check_quantized(q, x, tiles):
     nan = (want & 0x7F) == 0x7F  # a NaN of either sign
     assert torch.equal((got & 0x7F) == 0x7F, nan)
     assert torch.equal(torch.where(nan, 0, got), torch.where(nan, 0, want))
-    assert int(q._v[:, q.shape[1]:].sum()) == 0  # whole blocks of 128, filled with zeros
+    assert int(q._values()[:, q.shape[1]:].sum()) == 0  # whole blocks of 128, filled with zeros
 
 
 @pytest.mark.parametrize("t", list(TYPES))
@@ -222,7 +222,7 @@ def test_quantized_from_parts(P):
     for tiles in (False, True):
         q = P.quantize(x, tiles=tiles)
         p = P.Quantized(q.values.contiguous(), q.scales.contiguous(), tiles=tiles)
-        assert torch.equal(p._v, q._v) and torch.equal(p._s, q._s)
+        assert torch.equal(p._values(), q._values()) and torch.equal(p.scales, q.scales)
         assert torch.allclose(q.dequantize(), x, rtol=2.0 ** -4, atol=float(x.abs().max()) * 2.0 ** -9)
     with pytest.raises(P.NMFkError):
         P.Quantized(q.values, q.scales, tiles=False)
