@@ -76,11 +76,27 @@ __device__ __forceinline__ bf16 from_f32<bf16>(float x) {
   return r;
 }
 
-// Four consecutive entries, loaded or stored at once (p aligned to four entries).
+// Four consecutive entries, loaded or stored at once.  The GPU takes them at any address that suits one entry.
 template <typename T>
-struct alignas(4 * sizeof(T)) vec4 {
+struct vec4 {
   T v[4];
 };
+template <typename T>
+__device__ __forceinline__ void read4(const T *p, float (&out)[4]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) raw {
+    uint32_t w[sizeof(T)];
+  };
+  const vec4<T> q = __builtin_bit_cast(vec4<T>, *(const raw *)p);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = to_f32(q.v[e]);
+}
+template <typename T>
+__device__ __forceinline__ void write4(T *p, float a, float b, float c, float d) {
+  struct __attribute__((packed, aligned(sizeof(T)))) raw {
+    uint32_t w[sizeof(T)];
+  };
+  *(raw *)p = __builtin_bit_cast(raw, (vec4<T>{from_f32<T>(a), from_f32<T>(b), from_f32<T>(c), from_f32<T>(d)}));
+}
 
 typedef __attribute__((address_space(1))) const void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;

@@ -41,7 +41,7 @@ struct SmallArgs {
   int64_t b0;
   int s, chunks, steps;
   int64_t l, chunk;  // entries of l per workgroup
-  int gvec, ovec;    // four entries along the contiguous side may be loaded / stored at once
+  int gvec, ovec;    // the side that is walked is contiguous: four entries at once
 };
 
 struct Coefs {
@@ -53,9 +53,7 @@ __device__ __forceinline__ void small_load4(const Strided &g, const T *p, int s,
   const T *q = p + i * g.row + j * g.col;
   const bool whole = WIDE ? i < s && j + 4 <= l : j < l && i + 4 <= s;
   if (vec && whole) {
-    const vec4<T> v = *(const vec4<T> *)q;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = to_f32(v.v[e]);
+    read4(q, out);
   } else {
     const int64_t step = WIDE ? g.col : g.row;
 #pragma unroll
@@ -323,10 +321,7 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
           const int64_t j = base + 4 * c;
           T *z = o + row * a.o.row + j * a.o.col;
           if (a.ovec && j + 4 <= l1) {
-            vec4<T> v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v.v[e] = from_f32<T>(d[e][r]);
-            *(vec4<T> *)z = v;
+            write4(z, d[0][r], d[1][r], d[2][r], d[3][r]);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -361,10 +356,7 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
           const int row = 16 * i + 4 * g;
           T *z = o + row * a.o.row + j * a.o.col;
           if (a.ovec && row + 4 <= s) {
-            vec4<T> v;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v.v[r] = from_f32<T>(d[i][r]);
-            *(vec4<T> *)z = v;
+            write4(z, d[i][0], d[i][1], d[i][2], d[i][3]);
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -433,9 +425,7 @@ __global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s,
     for (int64_t e = lane * 4; e < inner; e += 256) {
       float x[4];
       if (vec && e + 4 <= inner) {
-        const vec4<T> u = *(const vec4<T> *)(q + e);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = to_f32(u.v[k]);
+        read4(q + e, x);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = e + k < inner ? to_f32(q[(e + k) * si]) : 0.f;
@@ -498,7 +488,7 @@ struct GemmArgs {
   int tiles_n;
   // SYM: the workgroups from `whole` on are the rest of the tiles, `splits` workgroups for each; partial sums as [tile of the rest][split][128][128]
   float *part;
-  int tiles, whole, splits, kb_split;
+  int tiles, whole, rest, splits, kb_split;
   Strided o;  // LAST
   int64_t b0;
   int vec;
@@ -526,17 +516,21 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
   int ti, tj, kb0 = 0, kb1 = a.kb;
   int64_t b = blockIdx.z;
   bool partial = false;
+  int slot = 0;
   if (MODE == SYM) {
     int id = blockIdx.x;
     if (id < a.whole) {
       id = xcd_order(id, a.whole);
     } else {
-      id -= a.whole;
-      const int split = id % a.splits;
+      // an XCD gets tiles of one matrix and one part of the sum: they share rows
+      id = xcd_order(id - a.whole, a.rest * a.splits);
+      const int k = id / (a.tiles * a.splits), left = id - k * a.tiles * a.splits, here = min(a.tiles, a.rest - k * a.tiles), split = left / here;
+      const int tile = k * a.tiles + left - split * here;
       partial = a.splits > 1;
+      slot = tile * a.splits + split;
       kb0 = split * a.kb_split;
       kb1 = min(a.kb, kb0 + a.kb_split);
-      id = a.whole + id / a.splits;
+      id = a.whole + tile;
     }
     b = id / a.tiles;
     sym_tile(id - (int)b * a.tiles, ti, tj);
@@ -642,7 +636,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
       const int n = j0 + wj + j * 16 + fg * 4;
       f32x4 v = acc[i][j];
       if (MODE == SYM && partial) {
-        *(f32x4 *)(a.part + (int64_t)(blockIdx.x - a.whole) * (BM * BN) + (m - i0) * BN + (n - j0)) = v;
+        *(f32x4 *)(a.part + (int64_t)slot * (BM * BN) + (m - i0) * BN + (n - j0)) = v;
         continue;
       }
       f32x4 d = {0.f, 0.f, 0.f, 0.f};
@@ -653,10 +647,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
         if (m >= a.m || n >= a.n) continue;
         T *q = (T *)a.o.p + (a.b0 + b) * a.o.batch + m * a.o.row + (int64_t)n * a.o.col;
         if (a.vec && n + 4 <= a.n) {
-          vec4<T> u;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) u.v[r] = from_f32<T>(v[r]);
-          *(vec4<T> *)q = u;
+          write4(q, v[0], v[1], v[2], v[3]);
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -805,12 +796,6 @@ int exponent(double bound) {
   return std::min(15 - e, 100);
 }
 
-// four consecutive entries along the side whose stride is `unit` may be moved at once, wherever they start at a multiple of four
-template <typename T>
-int four_at_once(const Strided &g, int64_t unit, int64_t other) {
-  return unit == 1 && other % 4 == 0 && g.batch % 4 == 0 && (uintptr_t)g.p % (4 * sizeof(T)) == 0;
-}
-
 template <typename T, int TT, bool WIDE>
 void small_launch(const SmallArgs &a, const Coefs &cf, unsigned nb, hipStream_t st) {
   const dim3 grid((unsigned)a.chunks, nb);
@@ -842,8 +827,8 @@ int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, 
     a.steps = steps;
     a.l = y.l;
     a.chunk = y.chunk;
-    a.gvec = wide ? four_at_once<T>(g, g.col, g.row) : four_at_once<T>(g, g.row, g.col);
-    a.ovec = wide ? four_at_once<T>(o, o.col, o.row) : four_at_once<T>(o, o.row, o.col);
+    a.gvec = wide || g.row == 1;
+    a.ovec = (wide ? o.col : o.row) == 1;
 #define NMFK_SMALL(TT) (wide ? small_launch<T, TT, true>(a, cf, nb, st) : small_launch<T, TT, false>(a, cf, nb, st))
     if (y.s <= 16)
       NMFK_SMALL(1);
@@ -874,6 +859,7 @@ void gemm_sym(GemmArgs a, unsigned batch, hipStream_t st) {
   a.tiles = (int)(tm * (tm + 1) / 2);
   const SymPlan q = sym_plan((int64_t)a.tiles * batch, a.kb);
   a.whole = q.whole;
+  a.rest = q.rest;
   a.splits = q.splits;
   a.kb_split = q.kb_split;
   gemm_tile<SYM, float, 128, 128, 2, 2>(a, dim3((unsigned)(q.whole + q.rest * q.splits)), st);
@@ -906,7 +892,7 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
     double *norm = (double *)(work + y.norm) + b0 * NORM_PARTS;
     double u = 1.0;  // bound of the singular values of X; e?: the power of two a matrix is scaled by
     int ex = exponent(1.01 * u);
-    norm_kernel<T><<<dim3(NORM_PARTS, nb), 256, 0, st>>>(g, b0, s, l, norm, g.row == 1 ? four_at_once<T>(g, 1, g.col) : four_at_once<T>(g, g.col, g.row));
+    norm_kernel<T><<<dim3(NORM_PARTS, nb), 256, 0, st>>>(g, b0, s, l, norm, g.row == 1 || g.col == 1);
     split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, ldexp(1.0, ex), X, XT);
     for (int k = 0; k < steps; ++k) {
       const double ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
@@ -939,7 +925,7 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
       if (last) {
         a.o = o;
         a.b0 = b0;
-        a.vec = o.col == 1 && o.row % 4 == 0 && o.batch % 4 == 0 && (uintptr_t)o.p % (4 * sizeof(T)) == 0;
+        a.vec = o.col == 1;
         gemm_full<LAST, T>(a, nb, st);
       } else {
         gemm_full<APPLY, float>(a, nb, st);

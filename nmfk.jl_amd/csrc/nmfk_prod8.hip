@@ -30,16 +30,12 @@ struct ProdArgs {
   int m, n, kb;     // blocks of 128
   int kb_split;     // blocks per workgroup along the sum
   int tiles_m, tiles_n;
-  int vec;          // four outputs may be stored at once
 };
 
 template <typename T>
-__device__ __forceinline__ void store4(T *p, f32x4 v, int left, int vec) {
-  if (left >= 4 && vec) {
-    vec4<T> q;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) q.v[r] = from_f32<T>(v[r]);
-    *(vec4<T> *)p = q;
+__device__ __forceinline__ void store4(T *p, f32x4 v, int left) {
+  if (left >= 4) {
+    write4(p, v[0], v[1], v[2], v[3]);
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -257,9 +253,9 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
       const int n = n0 + wn * (BN / WN) + j * 16 + fg * 4;
       if (n >= p.n) continue;
       if (SPLIT)
-        store4<float>((float *)p.y + ((int64_t)blockIdx.y * p.m + m) * p.n + n, acc[i][j], p.n - n, p.vec);
+        store4<float>((float *)p.y + ((int64_t)blockIdx.y * p.m + m) * p.n + n, acc[i][j], p.n - n);
       else
-        store4<T>((T *)p.y + m * p.ldy + n, acc[i][j], p.n - n, p.vec);
+        store4<T>((T *)p.y + m * p.ldy + n, acc[i][j], p.n - n);
     }
   }
 }
@@ -330,9 +326,9 @@ __global__ __launch_bounds__(512) void prod_rows_kernel(ProdArgs p) {
     const int m = 16 * i + (l & 15), n = n0 + 16 * j + (l >> 4) * 4;
     if (m >= p.m || n >= p.n) continue;
     if (SPLIT)
-      store4<float>((float *)p.y + ((int64_t)blockIdx.y * p.m + m) * p.n + n, v, p.n - n, p.vec);
+      store4<float>((float *)p.y + ((int64_t)blockIdx.y * p.m + m) * p.n + n, v, p.n - n);
     else
-      store4<T>((T *)p.y + m * p.ldy + n, v, p.n - n, p.vec);
+      store4<T>((T *)p.y + m * p.ldy + n, v, p.n - n);
   }
 }
 
@@ -368,7 +364,7 @@ __global__ __launch_bounds__(256) void prod_zero_kernel(T *y, int64_t m, int64_t
 }
 
 struct Plan {
-  int bm, bn;  // bm <= 64: prod_rows_kernel with 16 * (bm / 16) rows and bn columns a workgroup
+  int bm, bn;  // bn <= 32: prod_rows_kernel, bm rows and bn columns a workgroup; otherwise prod_tile_kernel
   int splits, kb_split;
 };
 
@@ -386,9 +382,12 @@ Plan prod_plan(int64_t m, int64_t n, int64_t kb, bool bytes) {
       q.bn = 64;
     else if (bytes && nmfk_div_up(m, 256) * nmfk_div_up(n, 256) >= 200)
       q.bm = q.bn = 256;
+    // Tiles of 64 x 64 where those of 128 x 128 would not give every CU one
+    if (q.bn == 128 && nmfk_div_up(m, 128) * nmfk_div_up(n, 128) < 256) q.bm = q.bn = 64;
     const int64_t tiles = nmfk_div_up(m, q.bm) * nmfk_div_up(n, q.bn);
-    // Few tiles leave most of the 256 CUs without one: split the sum, as long as a workgroup keeps four blocks.
-    if (tiles < 256) splits = std::min<int64_t>(512 / tiles, nmfk_div_up(kb, 4));
+    // Few tiles leave many of the 256 CUs without one: split the sum, as long as a workgroup keeps six blocks (about 5 microseconds; the join of
+    // the partial sums costs 4).
+    if (tiles < 192) splits = std::min<int64_t>(512 / tiles, kb / 6);
   }
   q.kb_split = (int)nmfk_div_up(kb, std::max<int64_t>(1, splits));
   q.splits = (int)std::max<int64_t>(1, nmfk_div_up(kb, q.kb_split));
@@ -415,7 +414,7 @@ void prod_tile(const ProdArgs &p, int splits, hipStream_t st) {
 
 template <typename F, typename T, bool SPLIT>
 void prod_launch(const ProdArgs &p, const Plan &q, hipStream_t st) {
-  if (q.bm <= 64) {
+  if (q.bn <= 32) {
     const dim3 grid((unsigned)nmfk_div_up(p.n, q.bn), (unsigned)q.splits);
     if (q.bm == 16)
       prod_rows_kernel<1, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
@@ -434,7 +433,9 @@ void prod_launch(const ProdArgs &p, const Plan &q, hipStream_t st) {
       prod_tile<256, 256, 2, 4, F, T, false>(p, 1, st);
       return;
     }
-  if (q.bn == 64)
+  if (q.bm == 64)
+    prod_tile<64, 64, 1, 2, F, T, SPLIT>(p, q.splits, st);
+  else if (q.bn == 64)
     prod_tile<128, 64, 2, 2, F, T, SPLIT>(p, q.splits, st);
   else
     prod_tile<128, 128, 2, 2, F, T, SPLIT>(p, q.splits, st);
@@ -453,14 +454,12 @@ int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
   p.kb_split = q.kb_split;
   if (q.splits > 1) {
     p.y = work;
-    p.vec = p.n % 4 == 0;
     prod_launch<F, float, true>(p, q, st);
-    if (p.vec)
+    if (p.n % 4 == 0)
       prod_join_kernel<T, 4><<<dim3((unsigned)nmfk_div_up(mn, 1024)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
     else
       prod_join_kernel<T, 1><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
   } else {
-    p.vec = p.ldy % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
     prod_launch<F, T, false>(p, q, st);
   }
   return nmfk_launched("nmfk_product");
@@ -507,7 +506,7 @@ NMFK_EXPORT int nmfk_product(int device, void *stream, int64_t m, int64_t n, int
     return fail(NMFK_ERR_BAD_ARG, "nmfk_product: the workspace is too small or not 16-byte aligned (nmfk_product_workspace)");
   NmfkDeviceGuard guard(device);
   if (guard.status) return guard.status;
-  ProdArgs p = {(const char *)A, (const char *)B, lda, ldb, sA, sB, ldsa, ldsb, a_tiles ? 7 : 0, b_tiles ? 7 : 0, Y, ldy, (int)m, (int)n, (int)kb, 0, 0, 0, 0};
+  ProdArgs p = {(const char *)A, (const char *)B, lda, ldb, sA, sB, ldsa, ldsb, a_tiles ? 7 : 0, b_tiles ? 7 : 0, Y, ldy, (int)m, (int)n, (int)kb, 0, 0, 0};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == NMFK_F32) return prod_run<Halves, float>(p, q, work, st);
   if (dtype == NMFK_BF16) return prod_run<Bytes, bf16>(p, q, work, st);

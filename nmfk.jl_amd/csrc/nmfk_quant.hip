@@ -23,7 +23,6 @@ struct QuantArgs {
   int64_t ldtv;
   float *ts;
   int64_t tsld;
-  int vec;  // four entries may be loaded at once
 };
 
 __device__ __forceinline__ float block_scale(float top) { return fmaxf(top / 448.0f, 1.17549435e-38f); }
@@ -31,23 +30,27 @@ __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;
 }
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
 // x / s rounded to nearest, for the many x of a block: with r = 1 / s rounded to nearest, q0 = x r, one correction q0 + r (x - q0 s) gives the
 // correctly rounded quotient (Markstein's theorem) unless the significand of s is all ones.  The residual has to be exact: s in [2^-80, 2^80] makes
-// it so for every quotient that does not round to zero in e4m3.  Elsewhere: the division (11 instructions instead of 3).  NaN and infinities come
-// out as NaN by themselves.
-struct Divisor {
-  float s, r;
-  bool easy;
-  __device__ __forceinline__ explicit Divisor(float scale) : s(scale), r(1.0f / scale) {
-    easy = scale >= 0x1p-80f && scale <= 0x1p80f && (__float_as_uint(scale) & 0x7fffffu) != 0x7fffffu;
+// it so for every quotient that does not round to zero in e4m3.  Elsewhere (EASY = false; a wave takes that path as a whole): the division, 11
+// instructions instead of 3.  NaN and infinities come out of the short form as NaN by themselves.
+__device__ __forceinline__ bool easy_divisor(float s) { return s >= 0x1p-80f && s <= 0x1p80f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu; }
+template <bool EASY>
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+  if (EASY) {
+    const float q = x * r;
+    return fmaf(fmaf(-q, s, x), r, q);
   }
-};
-__device__ __forceinline__ float quotient(float x, const Divisor &d) {
-  if (d.easy) {
-    const float q = x * d.r;
-    return fmaf(fmaf(-q, d.s, x), d.r, q);
-  }
-  return fabsf(x) <= 3.402823466e38f ? x / d.s : __uint_as_float(0x7fc00000u);
+  return fabsf(x) <= 3.402823466e38f ? x / s : __uint_as_float(0x7fc00000u);
+}
+template <bool EASY>
+__device__ __forceinline__ uint32_t quotients(float a, float b, float c, float d, float s, float r) {
+  return pack4(quotient<EASY>(a, s, r), quotient<EASY>(b, s, r), quotient<EASY>(c, s, r), quotient<EASY>(d, s, r));
 }
 // the largest of 32 lanes, in all of them: rotations within 16 lanes on the vector unit, then one exchange
 template <int CTRL>
@@ -61,18 +64,11 @@ __device__ __forceinline__ float largest32(float m) {
   m = fmaxf(m, rotate<0x121>(m));
   return fmaxf(m, __shfl_xor(m, 16));
 }
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-}
-
 template <typename T>
-__device__ __forceinline__ void load4(const QuantArgs &a, int64_t r, int64_t c, float out[4]) {
+__device__ __forceinline__ void load4(const QuantArgs &a, int64_t r, int64_t c, float (&out)[4]) {
   const T *p = (const T *)a.x + r * a.ld + c;
-  if (r < a.rows && c + 4 <= a.cols && a.vec) {
-    const vec4<T> q = *(const vec4<T> *)p;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = to_f32(q.v[j]);
+  if (r < a.rows && c + 4 <= a.cols) {
+    read4(p, out);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = r < a.rows && c + j < a.cols ? to_f32(p[j]) : 0.f;
@@ -89,24 +85,68 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a, int64_t bl
   float x[4];
   load4<T>(a, r, c, x);
   float top = fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
-  const float s = block_scale(largest32(top));
-  const Divisor d(s);
-  *(uint32_t *)(a.v + r * a.ldv + c) = pack4(quotient(x[0], d), quotient(x[1], d), quotient(x[2], d), quotient(x[3], d));
+  const float s = block_scale(largest32(top)), inv = 1.0f / s;
+  *(uint32_t *)(a.v + r * a.ldv + c) = __all(easy_divisor(s)) ? quotients<true>(x[0], x[1], x[2], x[3], s, inv) : quotients<false>(x[0], x[1], x[2], x[3], s, inv);
   if ((threadIdx.x & 31) == 0) a.s[kb * a.sld + r] = s;
 }
 
-// A 128 x 128 tile per workgroup of 256: lane group g = thread / 32 owns the rows 16 g .. 16 g + 15, thread % 32 four columns.
+// A 128 x 128 tile per workgroup of 256: lane group g = thread / 32 owns the rows 16 g .. 16 g + 15, thread % 32 four columns.  `rs`, `cs`: the scales of
+// the thread's rows and columns and their reciprocals (TILES: the one of the tile).
+template <bool TILES, bool EASY>
+__device__ __forceinline__ void quant_tile_values(const QuantArgs &a, const float (&x)[16][4], const float (&rs)[TILES ? 1 : 16], const float (&rr)[TILES ? 1 : 16],
+                                                  const float (&cs)[TILES ? 1 : 4], const float (&cr)[TILES ? 1 : 4], char *turn, int64_t r0, int64_t c0) {
+  const int t = threadIdx.x, g = t >> 5, cg = t & 31;
+  uint32_t q[16];  // TILES: the values serve both orientations
+  if (a.v || TILES) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      q[i] = quotients<EASY>(x[i][0], x[i][1], x[i][2], x[i][3], rs[TILES ? 0 : i], rr[TILES ? 0 : i]);
+      if (a.v && r0 + g * 16 + i < a.rows) *(uint32_t *)(a.v + (r0 + g * 16 + i) * a.ldv + c0 + cg * 4) = q[i];
+    }
+  }
+  if (!a.tv) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    i32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (TILES) {  // byte j of four rows: two permutations of register pairs, then one of the halves
+        const uint32_t sel = 0x0c0c0400u + 0x0101u * j;
+        const uint32_t lo = __builtin_amdgcn_perm(q[4 * k + 1], q[4 * k], sel), hi = __builtin_amdgcn_perm(q[4 * k + 3], q[4 * k + 2], sel);
+        w[k] = (int)(lo | hi << 16);
+      } else {
+        w[k] = (int)quotients<EASY>(x[4 * k][j], x[4 * k + 1][j], x[4 * k + 2][j], x[4 * k + 3][j], cs[TILES ? 0 : j], cr[TILES ? 0 : j]);
+      }
+    }
+    *(i32x4 *)(turn + (cg * 4 + j) * 128 + ((g ^ (cg & 7)) << 4)) = w;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = i * 32 + (t >> 3), slot = t & 7;
+    if (c0 + c < a.cols)
+      *(i32x4 *)(a.tv + (c0 + c) * a.ldtv + r0 + slot * 16) = *(const i32x4 *)(turn + c * 128 + ((slot ^ ((c >> 2) & 7)) << 4));
+  }
+}
+
 template <typename T, bool TILES>
 __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
   __shared__ __attribute__((aligned(16))) char turn[128 * 128];
   __shared__ float ctop[8][128];
+  __shared__ int hard;
   const int t = threadIdx.x, g = t >> 5, cg = t & 31;
   const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
   float x[16][4];
+  if (t == 0) hard = 0;
+  if (r0 + 128 <= a.rows && c0 + 128 <= a.cols) {
+    const T *p = (const T *)a.x + (r0 + g * 16) * a.ld + c0 + cg * 4;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) load4<T>(a, r0 + g * 16 + i, c0 + cg * 4, x[i]);
-  float cmax[4] = {0.f, 0.f, 0.f, 0.f};
-  float rmax[16];
+    for (int i = 0; i < 16; ++i) read4(p + i * a.ld, x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) load4<T>(a, r0 + g * 16 + i, c0 + cg * 4, x[i]);
+  }
+  float cmax[4] = {0.f, 0.f, 0.f, 0.f}, rmax[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float m = 0.f;
@@ -118,67 +158,51 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
     }
     rmax[i] = m;
   }
-  float tile_s = 1.f;
-  if (TILES || a.tv) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) ctop[g][cg * 4 + j] = cmax[j];
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int h = 0; h < 8; ++h) cmax[j] = fmaxf(cmax[j], ctop[h][cg * 4 + j]);
-  }
-  if (TILES) {
-    tile_s = block_scale(largest32(fmaxf(fmaxf(cmax[0], cmax[1]), fmaxf(cmax[2], cmax[3]))));
-    if (t == 0) {
-      if (a.v) a.s[(int64_t)blockIdx.x * a.sld + blockIdx.y] = tile_s;
-      if (a.tv) a.ts[(int64_t)blockIdx.y * a.tsld + blockIdx.x] = tile_s;
-    }
-  }
-  uint32_t q[16];  // TILES: the values serve both orientations
-  if (a.v || TILES) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float s = TILES ? tile_s : block_scale(largest32(rmax[i]));
-      const Divisor d(s);
-      q[i] = pack4(quotient(x[i][0], d), quotient(x[i][1], d), quotient(x[i][2], d), quotient(x[i][3], d));
-      const int64_t r = r0 + g * 16 + i;
-      if (a.v && r < a.rows) {
-        *(uint32_t *)(a.v + r * a.ldv + c0 + cg * 4) = q[i];
-        if (!TILES && cg == 0) a.s[(int64_t)blockIdx.x * a.sld + r] = s;
-      }
-    }
-  }
-  if (!a.tv) return;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = cg * 4 + j;
-    i32x4 w;
-    if (TILES) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t o = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o |= ((q[k * 4 + i] >> (8 * j)) & 255u) << (8 * i);
-        w[k] = (int)o;
-      }
-    } else {
-      const float s = block_scale(cmax[j]);
-      const Divisor d(s);
-      if (g == 0 && c0 + c < a.cols) a.ts[(int64_t)blockIdx.y * a.tsld + c0 + c] = s;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        w[k] = (int)pack4(quotient(x[k * 4][j], d), quotient(x[k * 4 + 1][j], d), quotient(x[k * 4 + 2][j], d), quotient(x[k * 4 + 3][j], d));
-    }
-    *(i32x4 *)(turn + c * 128 + ((g ^ (cg & 7)) << 4)) = w;
-  }
+  *(f32x4 *)&ctop[g][cg * 4] = (f32x4){cmax[0], cmax[1], cmax[2], cmax[3]};
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = i * 32 + (t >> 3), slot = t & 7;
-    if (c0 + c < a.cols)
-      *(i32x4 *)(a.tv + (c0 + c) * a.ldtv + r0 + slot * 16) = *(const i32x4 *)(turn + c * 128 + ((slot ^ ((c >> 2) & 7)) << 4));
+  for (int h = 0; h < 8; ++h) {
+    const f32x4 v = *(const f32x4 *)&ctop[h][cg * 4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) cmax[j] = fmaxf(cmax[j], v[j]);
   }
+  float rs[TILES ? 1 : 16], rr[TILES ? 1 : 16], cs[TILES ? 1 : 4], cr[TILES ? 1 : 4];
+  bool easy = true;
+  if (TILES) {
+    rs[0] = cs[0] = block_scale(largest32(fmaxf(fmaxf(cmax[0], cmax[1]), fmaxf(cmax[2], cmax[3]))));
+    rr[0] = cr[0] = 1.0f / rs[0];
+    easy = easy_divisor(rs[0]);
+    if (t == 0) {
+      if (a.v) a.s[(int64_t)blockIdx.x * a.sld + blockIdx.y] = rs[0];
+      if (a.tv) a.ts[(int64_t)blockIdx.y * a.tsld + blockIdx.x] = rs[0];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      rs[TILES ? 0 : i] = block_scale(largest32(rmax[i]));
+      rr[TILES ? 0 : i] = 1.0f / rs[TILES ? 0 : i];
+      easy = easy && easy_divisor(rs[TILES ? 0 : i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      cs[TILES ? 0 : j] = block_scale(cmax[j]);
+      cr[TILES ? 0 : j] = 1.0f / cs[TILES ? 0 : j];
+      easy = easy && easy_divisor(cs[TILES ? 0 : j]);
+      if (a.tv && g == 0 && c0 + cg * 4 + j < a.cols) a.ts[(int64_t)blockIdx.y * a.tsld + c0 + cg * 4 + j] = cs[TILES ? 0 : j];
+    }
+    if (a.v && cg < 16 && r0 + g * 16 + cg < a.rows) {
+      float s = rs[0];  // this lane's row, without indexing registers
+#pragma unroll
+      for (int i = 1; i < 16; ++i) s = cg == i ? rs[TILES ? 0 : i] : s;
+      a.s[(int64_t)blockIdx.x * a.sld + r0 + g * 16 + cg] = s;
+    }
+  }
+  if (!easy) hard = 1;
+  __syncthreads();
+  if (hard)
+    quant_tile_values<TILES, false>(a, x, rs, rr, cs, cr, turn, r0, c0);
+  else
+    quant_tile_values<TILES, true>(a, x, rs, rr, cs, cr, turn, r0, c0);
 }
 
 template <typename T>
@@ -221,11 +245,9 @@ NMFK_EXPORT int nmfk_quantize(int device, void *stream, int dtype, const void *X
   const bool as_is = col_stride == 1 && (row_stride >= cols || rows == 1);
   a.x = X;
   if (as_is)
-    a = {X, rows, cols, rows == 1 ? cols : row_stride, values, ldv, scales, lds, tvalues, ldtv, tscales, ldts, 0};
+    a = {X, rows, cols, rows == 1 ? cols : row_stride, values, ldv, scales, lds, tvalues, ldtv, tscales, ldts};
   else
-    a = {X, cols, rows, cols == 1 ? rows : col_stride, tvalues, ldtv, tscales, ldts, values, ldv, scales, lds, 0};
-  const int64_t size = nmfk_type_size(dtype);
-  a.vec = ((uintptr_t)X % (4 * size)) == 0 && (a.ld % 4) == 0;
+    a = {X, cols, rows, cols == 1 ? rows : col_stride, tvalues, ldtv, tscales, ldts, values, ldv, scales, lds};
   if (nmfk_div_up(a.rows, 128) > 65535) return fail(NMFK_ERR_UNSUPPORTED, "nmfk_quantize: too many rows");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == NMFK_F32)

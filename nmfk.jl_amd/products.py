@@ -125,8 +125,7 @@ class Quantized:
 
     @property
     def scales(self):
-        r = self.shape[0]
-        return self._buf[r * self._ldv:].view(_F32).as_strided((self._lds, self._ldv // 128), (1, self._lds))
+        return self._buf.view(_F32).as_strided((self._lds, self._ldv // 128), (1, self._lds), self.shape[0] * self._ldv // 4)
 
     def dequantize(self, dtype=None):
         """the matrix that values and scales stand for (float32 unless told otherwise)"""
@@ -229,12 +228,18 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
         _tensor(out, "out", ndim=0)
         if out.shape != G.shape or out.dtype != G.dtype or out.device != G.device:
             raise _bad("out must have G's shape, type and GPU")
-    g = G if G.dim() == 3 else G.unsqueeze(0) if G.dim() == 2 else G.reshape(-1, *G.shape[-2:])
-    o = out if out.dim() == 3 else out.unsqueeze(0) if out.dim() == 2 else out.view(-1, *out.shape[-2:])
-    b, r, c = g.shape
+    g, o = G, out
+    if G.dim() == 2:
+        (r, c), b = G.shape, 1
+        gs, os = (0, *G.stride()), (0, *out.stride())
+    else:
+        if G.dim() > 3:
+            g, o = G.reshape(-1, *G.shape[-2:]), out.view(-1, *out.shape[-2:])
+        b, r, c = g.shape
+        gs, os = g.stride(), o.stride()
     dev, nb = G.device, _orthogonalize_workspace(b, r, c)
     work = torch.empty(nb, dtype=_U8, device=dev) if nb else None
-    _check(_lib.lib().nmfk_orthogonalize(dev.index, _stream(dev), _TYPES[G.dtype], b, r, c, g.data_ptr(), *g.stride(), o.data_ptr(), *o.stride(),
+    _check(_lib.lib().nmfk_orthogonalize(dev.index, _stream(dev), _TYPES[G.dtype], b, r, c, g.data_ptr(), *gs, o.data_ptr(), *os,
                                          steps, cf_at, work.data_ptr() if nb else None, nb))
     return out
 
