@@ -668,19 +668,20 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
 
 // The tiles whose sum was split: the partial sums in the order of the splits, then what the tile's own workgroup would have done.  32 x 32 results
 // a workgroup, turned in LDS for the place across the diagonal.
+template <int TS>
 __global__ __launch_bounds__(256) void sym_join_kernel(GemmArgs a) {
   __shared__ float turn[32][33];
   const int t = threadIdx.x, y = t >> 3, x = (t & 7) * 4;
   const int id = a.whole + blockIdx.x, b = id / a.tiles;
   int ti, tj;
   sym_tile(id - b * a.tiles, ti, tj);
-  const int u0 = (blockIdx.y >> 2) * 32, v0 = (blockIdx.y & 3) * 32;
-  const int m0 = ti * 128 + u0, n0 = tj * 128 + v0, m = m0 + y, n = n0 + x, mp = (a.m + 31) & ~31;
+  const int u0 = blockIdx.y / (TS / 32) * 32, v0 = blockIdx.y % (TS / 32) * 32;
+  const int m0 = ti * TS + u0, n0 = tj * TS + v0, m = m0 + y, n = n0 + x, mp = (a.m + 31) & ~31;
   if (m0 >= mp || n0 >= mp) return;
-  const float *p = a.part + (int64_t)blockIdx.x * a.splits * 16384 + (u0 + y) * 128 + v0 + x;
+  const float *p = a.part + (int64_t)blockIdx.x * a.splits * (TS * TS) + (u0 + y) * TS + v0 + x;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int k = 0; k < a.splits; ++k) v += *(const f32x4 *)(p + (int64_t)k * 16384);
+  for (int k = 0; k < a.splits; ++k) v += *(const f32x4 *)(p + (int64_t)k * (TS * TS));
   f32x4 d = {0.f, 0.f, 0.f, 0.f};
   if (a.add != 0.f && m < a.m) d = get4(a.d.p + b * a.d.batch + (int64_t)m * a.d.ld, n);
 #pragma unroll
@@ -696,29 +697,53 @@ __global__ __launch_bounds__(256) void sym_join_kernel(GemmArgs a) {
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 
-// The tiles of a symmetric product over the GPU's 512 places (two workgroups of 64 KB of LDS on each of 256 CUs): the last round is rarely full, so
-// the sums of its tiles are split.  Microseconds, measured: a round of whole tiles takes 1.1 for each block of 32, a partial sum 0.03 to write
-// and read again, the launch that joins them 4 (4096 x 4096, 528 tiles: the 16 of the second round in 16 parts, 226 -> 185; four of
-// 1000 x 4096, 144 tiles: three parts).
+// Which tiles a product is cut into.  Small tiles fill the 256 CUs where there is little to do, large ones read less for each operation.  The estimate, in
+// microseconds, measured: tiles of a side run `places` at a time (LDS: 128, 64, 32 KB a workgroup), such a round takes `step` for each block of 32
+// of the sum and `rest` to begin and to write.
+struct TileCost {
+  int side;
+  int64_t places;
+  double step, rest, part;  // part: a partial sum to write and read again
+};
+constexpr TileCost COST[3] = {{64, 1024, 0.85, 4, 0.008}, {128, 512, 1.4, 8, 0.03}, {256, 256, 2.6, 16, 0}};
+
+// A symmetric product: the last round of tiles is rarely full, so the sums of its tiles may be split (the launch that joins them costs 4).  4096 x 4096 with
+// 528 tiles of 128: the 16 of the second round in 16 parts, 226 -> 185.
 struct SymPlan {
+  int side;
+  int tiles;  // a matrix
   int whole, rest, splits, kb_split;
 };
 
-SymPlan sym_plan(int64_t tiles, int64_t kb) {
-  constexpr int64_t PLACES = 512;
-  SymPlan q;
-  q.whole = (int)(tiles / PLACES * PLACES);
-  q.rest = (int)(tiles - q.whole);
-  q.splits = 1;
-  double best = 1.1 * (double)kb;
-  for (int64_t s = 2; s <= 32 && s * 4 <= kb && s * q.rest <= 1536; ++s) {
-    const double cost = 1.1 * (double)(nmfk_div_up(q.rest * s, PLACES) * nmfk_div_up(kb, s)) + 0.03 * (double)(q.rest * s) + 4.0;
-    if (cost < best) best = cost, q.splits = (int)s;
+SymPlan sym_plan(int64_t m, int64_t batch, int64_t kb) {
+  SymPlan best = {};
+  double least = 1e30;
+  for (const TileCost &c : COST) {
+    if (c.side == 256) continue;
+    const int64_t tm = nmfk_div_up(m, c.side), tiles = tm * (tm + 1) / 2, total = tiles * batch;
+    if (total > 0x7fffffff / 64) continue;
+    const int64_t whole = total / c.places * c.places, rest = total - whole;
+    const double before = (double)(total / c.places) * (c.step * (double)kb + c.rest);
+    for (int64_t s = 1; s <= 64 && (s == 1 || (s * 4 <= kb && s * rest <= 3 * c.places)); ++s) {
+      const double cost = before + (double)nmfk_div_up(rest * s, c.places) * (c.step * (double)nmfk_div_up(kb, s) + c.rest) + (s > 1 ? c.part * (double)(rest * s) + 4.0 : 0.0);
+      if (cost >= least) continue;
+      least = cost;
+      best = {c.side, (int)tiles, (int)whole, (int)rest, (int)s, (int)nmfk_div_up(kb, s)};
+    }
   }
-  q.kb_split = (int)nmfk_div_up(kb, q.splits);
-  q.splits = (int)nmfk_div_up(kb, q.kb_split);
-  if (q.splits == 1) q.whole = (int)tiles, q.rest = 0;
-  return q;
+  best.splits = (int)nmfk_div_up(kb, best.kb_split);
+  if (best.splits == 1) best.whole += best.rest, best.rest = 0;
+  return best;
+}
+
+int full_side(int64_t m, int64_t n, int64_t batch, int64_t kb) {
+  int side = 0;
+  double least = 1e30;
+  for (const TileCost &c : COST) {
+    const double cost = (double)nmfk_div_up(nmfk_div_up(m, c.side) * nmfk_div_up(n, c.side) * batch, c.places) * (c.step * (double)kb + c.rest);
+    if (cost < least) least = cost, side = c.side;
+  }
+  return side;
 }
 
 struct Layout {
@@ -756,12 +781,11 @@ Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     y.xt[1] = take(batch * y.l * y.ldt);
     for (int k = 0; k < 2; ++k) y.sq[k] = take(batch * y.s * y.ldt);
     y.norm = take(batch * NORM_PARTS * 8);
-    const int64_t tm = nmfk_div_up(y.s, 128), tiles = tm * (tm + 1) / 2;
     int64_t part = 0;
     for (int64_t b0 = 0; b0 < batch; b0 += BATCH)
       for (int64_t k : {y.l, y.s}) {
-        const SymPlan q = sym_plan(tiles * std::min<int64_t>(BATCH, batch - b0), nmfk_div_up(k, 32));
-        if (q.splits > 1) part = std::max<int64_t>(part, (int64_t)q.rest * q.splits * 16384 * 4);
+        const SymPlan q = sym_plan(y.s, std::min<int64_t>(BATCH, batch - b0), nmfk_div_up(k, 32));
+        if (q.splits > 1) part = std::max<int64_t>(part, (int64_t)q.rest * q.splits * q.side * q.side * 4);
       }
     y.part = take(part);
   }
@@ -853,29 +877,37 @@ void gemm_tile(const GemmArgs &a, dim3 grid, hipStream_t st) {
 
 // a symmetric product: the tiles on and below the diagonal
 void gemm_sym(GemmArgs a, unsigned batch, hipStream_t st) {
-  const int64_t tm = nmfk_div_up(a.m, 128);
+  const SymPlan q = sym_plan(a.m, batch, a.kb);
   a.n = a.m;
   a.out_t = a.out;
-  a.tiles = (int)(tm * (tm + 1) / 2);
-  const SymPlan q = sym_plan((int64_t)a.tiles * batch, a.kb);
+  a.tiles = q.tiles;
   a.whole = q.whole;
   a.rest = q.rest;
   a.splits = q.splits;
   a.kb_split = q.kb_split;
-  gemm_tile<SYM, float, 128, 128, 2, 2>(a, dim3((unsigned)(q.whole + q.rest * q.splits)), st);
-  if (q.rest) sym_join_kernel<<<dim3((unsigned)q.rest, 16), 256, 0, st>>>(a);
+  const dim3 grid((unsigned)(q.whole + q.rest * q.splits));
+  if (q.side == 64)
+    gemm_tile<SYM, float, 64, 64, 1, 2>(a, grid, st);
+  else
+    gemm_tile<SYM, float, 128, 128, 2, 2>(a, grid, st);
+  if (!q.rest) return;
+  if (q.side == 64)
+    sym_join_kernel<64><<<dim3((unsigned)q.rest, 4), 256, 0, st>>>(a);
+  else
+    sym_join_kernel<128><<<dim3((unsigned)q.rest, 16), 256, 0, st>>>(a);
 }
 
 template <int MODE, typename T>
 void gemm_full(GemmArgs a, unsigned batch, hipStream_t st) {
-  const int64_t big = nmfk_div_up(a.m, 256) * nmfk_div_up(a.n, 256);
-  if (big * batch >= 200) {
-    a.tiles_n = (int)nmfk_div_up(a.n, 256);
-    gemm_tile<MODE, T, 256, 256, 2, 4>(a, dim3((unsigned)big, 1, batch), st);
-  } else {
-    a.tiles_n = (int)nmfk_div_up(a.n, 128);
-    gemm_tile<MODE, T, 128, 128, 2, 2>(a, dim3((unsigned)(nmfk_div_up(a.m, 128) * a.tiles_n), 1, batch), st);
-  }
+  const int side = full_side(a.m, a.n, batch, a.kb);
+  a.tiles_n = (int)nmfk_div_up(a.n, side);
+  const dim3 grid((unsigned)(nmfk_div_up(a.m, side) * a.tiles_n), 1, batch);
+  if (side == 256)
+    gemm_tile<MODE, T, 256, 256, 2, 4>(a, grid, st);
+  else if (side == 128)
+    gemm_tile<MODE, T, 128, 128, 2, 2>(a, grid, st);
+  else
+    gemm_tile<MODE, T, 64, 64, 1, 2>(a, grid, st);
 }
 
 // Each step forms S = X X', its polynomial P = b S + c S S and X <- a X + P X.  (The S of a later step could be had from the first one, S <- (a + P) S (a + P),
