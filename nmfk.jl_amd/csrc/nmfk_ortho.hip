@@ -698,14 +698,20 @@ __global__ __launch_bounds__(256) void sym_join_kernel(GemmArgs a) {
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 
 // Which tiles a product is cut into.  Small tiles fill the 256 CUs where there is little to do, large ones read less for each operation.  The estimate, in
-// microseconds, measured: tiles of a side run `places` at a time (LDS: 128, 64, 32 KB a workgroup), such a round takes `step` for each block of 32
-// of the sum and `rest` to begin and to write.
+// microseconds, measured: `places` tiles of a side run at a time (LDS: 128, 64, 32 KB a workgroup); such a round takes `step` for each block of
+// 32 of the sum, at least `alone` of that when it is not full, and `rest` to begin and to write.
 struct TileCost {
   int side;
   int64_t places;
-  double step, rest, part;  // part: a partial sum to write and read again
+  double step, alone, rest, part;  // part: a partial sum to write and read again
 };
-constexpr TileCost COST[3] = {{64, 1024, 0.85, 4, 0.008}, {128, 512, 1.4, 8, 0.03}, {256, 256, 2.6, 16, 0}};
+constexpr TileCost COST[3] = {{64, 1024, 0.95, 0.85, 4, 0.008}, {128, 512, 1.35, 0.55, 6, 0.03}, {256, 256, 2.6, 1.0, 16, 0}};
+
+double tiles_cost(const TileCost &c, int64_t tiles, int64_t kb) {
+  const int64_t full = tiles / c.places, rest = tiles - full * c.places;
+  const double fill = (double)nmfk_div_up(rest, 256) * 256.0 / (double)c.places;
+  return (double)full * (c.step * (double)kb + c.rest) + (rest ? c.step * std::max(fill, c.alone) * (double)kb + c.rest : 0.0);
+}
 
 // A symmetric product: the last round of tiles is rarely full, so the sums of its tiles may be split (the launch that joins them costs 4).  4096 x 4096 with
 // 528 tiles of 128: the 16 of the second round in 16 parts, 226 -> 185.
@@ -723,9 +729,9 @@ SymPlan sym_plan(int64_t m, int64_t batch, int64_t kb) {
     const int64_t tm = nmfk_div_up(m, c.side), tiles = tm * (tm + 1) / 2, total = tiles * batch;
     if (total > 0x7fffffff / 64) continue;
     const int64_t whole = total / c.places * c.places, rest = total - whole;
-    const double before = (double)(total / c.places) * (c.step * (double)kb + c.rest);
+    const double before = tiles_cost(c, whole, kb);
     for (int64_t s = 1; s <= 64 && (s == 1 || (s * 4 <= kb && s * rest <= 3 * c.places)); ++s) {
-      const double cost = before + (double)nmfk_div_up(rest * s, c.places) * (c.step * (double)nmfk_div_up(kb, s) + c.rest) + (s > 1 ? c.part * (double)(rest * s) + 4.0 : 0.0);
+      const double cost = before + tiles_cost(c, rest * s, nmfk_div_up(kb, s)) + (s > 1 ? c.part * (double)(rest * s) + 4.0 : 0.0);
       if (cost >= least) continue;
       least = cost;
       best = {c.side, (int)tiles, (int)whole, (int)rest, (int)s, (int)nmfk_div_up(kb, s)};
@@ -740,7 +746,7 @@ int full_side(int64_t m, int64_t n, int64_t batch, int64_t kb) {
   int side = 0;
   double least = 1e30;
   for (const TileCost &c : COST) {
-    const double cost = (double)nmfk_div_up(nmfk_div_up(m, c.side) * nmfk_div_up(n, c.side) * batch, c.places) * (c.step * (double)kb + c.rest);
+    const double cost = tiles_cost(c, nmfk_div_up(m, c.side) * nmfk_div_up(n, c.side) * batch, kb);
     if (cost < least) least = cost, side = c.side;
   }
   return side;
