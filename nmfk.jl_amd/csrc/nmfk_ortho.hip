@@ -100,26 +100,62 @@ __global__ __launch_bounds__(256) void small_gram_kernel(SmallArgs a) {
         }
     }
   } else {
-    const int span = 4 * packed;
-    for (int64_t base = l0 + (int64_t)w * U * span; base < l1; base += 4 * U * span) {
-      float x[U][TT];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t j = base + u * span + g * packed + grp;
-#pragma unroll
-        for (int k = 0; k < TT; ++k) x[u][k] = live && j < l1 && 16 * k + row < s ? to_f32(p[(16 * k + row) * a.g.row + j * a.g.col]) : 0.f;
-      }
+    // TT == 1: two sums take turns, an fp64 instruction waits for its predecessor's result otherwise
+    f64x4 odd = {0, 0, 0, 0};
+    const int span = 4 * packed, mine = g * packed + grp;
+    const int64_t step = span * a.g.col;
+    auto multiply = [&](const float (&x)[U][TT]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         double v[TT];
 #pragma unroll
         for (int k = 0; k < TT; ++k) v[k] = (double)x[u][k];
+        if (TT == 1 && (u & 1)) {
+          odd = __builtin_amdgcn_mfma_f64_16x16x4f64(v[0], v[0], odd, 0, 0, 0);
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
           for (int j = 0; j <= i; ++j) acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[i], v[j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
       }
+    };
+    int64_t base = l0 + (int64_t)w * U * span;
+    const T *q[TT];
+    bool here[TT];
+#pragma unroll
+    for (int k = 0; k < TT; ++k) {
+      here[k] = live && 16 * k + row < s;
+      q[k] = p + (here[k] ? (16 * k + row) * a.g.row + (base + mine) * a.g.col : 0);
     }
+    float x[U][TT], next[U][TT];
+    auto load = [&](float (&to)[U][TT], bool whole) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < TT; ++k) to[u][k] = here[k] && (whole || base + u * span + mine < l1) ? to_f32(q[k][u * step]) : 0.f;
+#pragma unroll
+      for (int k = 0; k < TT; ++k) q[k] += 4 * U * step;
+      base += 4 * U * span;
+    };
+    // the next entries are on their way while these are multiplied
+    if (base + U * span <= l1) {
+      load(x, true);
+      while (base + U * span <= l1) {
+        load(next, true);
+        multiply(x);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < TT; ++k) x[u][k] = next[u][k];
+      }
+      multiply(x);
+    }
+    if (base < l1) {
+      load(x, false);
+      multiply(x);
+    }
+    if (TT == 1) acc[0] += odd;
   }
   double *out = a.part + ((int64_t)blockIdx.y * a.chunks + blockIdx.x) * s * s;
 #pragma unroll
@@ -241,12 +277,13 @@ template <typename T, int TT, bool WIDE>
 __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf) {
   __shared__ double sum[4][256];
   __shared__ float qs[16][17];
-  const int64_t b = a.b0 + blockIdx.y;
+  const int by = gridDim.y - 1 - blockIdx.y;  // the matrices read last are still in the last-level cache: take them first
+  const int64_t b = a.b0 + by;
   const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
   const int s = a.s, t = threadIdx.x, w = t >> 6, lane = t & 63, c = lane & 15, g = lane >> 4;
   float q[TT][TT][4];
   if (TT == 1) {
-    const double *part = a.part + (int64_t)blockIdx.y * a.chunks * s * s;
+    const double *part = a.part + (int64_t)by * a.chunks * s * s;
     const int y = t >> 4, x = t & 15;
     double v[4] = {0, 0, 0, 0};
     if (y < s && x < s) {
@@ -283,7 +320,7 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
 #pragma unroll
     for (int k = 0; k < 4; ++k) q[0][0][k] = qs[c][WIDE ? 4 * k + g : 4 * g + k];
   } else {
-    const float *m = a.q + (int64_t)blockIdx.y * s * s;
+    const float *m = a.q + (int64_t)by * s * s;
 #pragma unroll
     for (int i = 0; i < TT; ++i)
 #pragma unroll
@@ -772,9 +809,9 @@ Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     return o;
   };
   if (y.s <= SMALL) {
-    // about 2048 workgroups, each with 256 entries of l at least; the partial S of one matrix are summed by every workgroup (s <= 16) or by one
+    // at most 2048 workgroups (all of them run at once), each with 256 entries of l at least; the partial S of one matrix are summed by every workgroup (s <= 16) or by one
     const int64_t most = y.s <= 16 ? 256 : 128;
-    y.chunks = std::max<int64_t>(1, std::min<int64_t>({nmfk_div_up(y.l, 256), nmfk_div_up(2048, batch), most}));
+    y.chunks = std::max<int64_t>(1, std::min<int64_t>({nmfk_div_up(y.l, 256), 2048 / batch, most}));
     y.chunk = nmfk_round_up(nmfk_div_up(y.l, y.chunks), 64);
     y.chunks = nmfk_div_up(y.l, y.chunk);
     y.part = take(batch * y.chunks * y.s * y.s * 8);
