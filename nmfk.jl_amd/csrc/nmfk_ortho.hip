@@ -479,9 +479,9 @@ __global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s,
   if (threadIdx.x == 0) part[(int64_t)blockIdx.y * NORM_PARTS + blockIdx.x] = ((sum[0] + sum[1]) + sum[2]) + sum[3];
 }
 
-// X = G * (1 / |G|) * 2^e, split, as s x l and as l x s.  A 64 x 64 tile per workgroup, turned in LDS.
+// X' = (G * (1 / |G|) * 2^e)', split: l rows of s entries, and rows of zeros up to a multiple of 32.  A 64 x 64 tile per workgroup, turned in LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void split_kernel(Strided g, int64_t b0, int s, int64_t l, const double *part, double pow2, Split x, Split xt) {
+__global__ __launch_bounds__(256) void split_kernel(Strided g, int64_t b0, int s, int64_t l, const double *part, double pow2, Split xt) {
   __shared__ float tile[64][65];
   const int t = threadIdx.x;
   const int64_t b = b0 + blockIdx.z;
@@ -507,23 +507,21 @@ __global__ __launch_bounds__(256) void split_kernel(Strided g, int64_t b0, int s
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int e = t + k * 256, u = e >> 4, v = (e & 15) * 4;
-    if (i0 + u < s && j0 + v < lp)
-      put4(x.p + blockIdx.z * x.batch + (i0 + u) * x.ld, (int)(j0 + v), (f32x4){tile[u][v], tile[u][v + 1], tile[u][v + 2], tile[u][v + 3]});
-    if (j0 + u < l && i0 + v < sp)
+    if (j0 + u < lp && i0 + v < sp)
       put4(xt.p + blockIdx.z * xt.batch + (j0 + u) * xt.ld, i0 + v, (f32x4){tile[v][u], tile[v + 1][u], tile[v + 2][u], tile[v + 3][u]});
   }
 }
 
-enum { SYM = 0, APPLY = 1, LAST = 2 };
+enum { GRAM = 0, SYM = 1, APPLY = 2, LAST = 3 };
 
 struct GemmArgs {
-  Split p, q;    // C[i, j] = sum_k P[i, k] Q[j, k]
+  Split p, q;    // C[i, j] = sum_k P[i, k] Q[j, k]; GRAM: sum_k P[k, i] P[k, j]
   int m, n, kb;  // kb: blocks of 32
   float mul, add;  // result = mul * C + add * D
-  Split d;           // read where add is not zero
-  Split out, out_t;  // APPLY: [i, j] and [j, i]; SYM: out
+  Split d;           // read where add is not zero; SYM: [i, j], APPLY and LAST: [j, i]
+  Split out;         // GRAM and SYM: [i, j] and [j, i], APPLY: [j, i]
   int tiles_n;
-  // SYM: the workgroups from `whole` on are the rest of the tiles, `splits` workgroups for each; partial sums as [tile of the rest][split][128][128]
+  // GRAM and SYM: the workgroups from `whole` on are the rest of the tiles, `splits` workgroups for each; partial sums as [tile of the rest][split][side][side]
   float *part;
   int tiles, whole, rest, splits, kb_split;
   Strided o;  // LAST
@@ -538,15 +536,22 @@ __device__ __forceinline__ void sym_tile(int id, int &ti, int &tj) {  // the til
   tj = id - ti * (ti + 1) / 2;
 }
 
-// BM x BN outputs a workgroup, WM x WN waves.  SYM: the result is symmetric, only the tiles on and below the diagonal are computed and each is
+// BM x BN outputs a workgroup, WM x WN waves.  GRAM and SYM: the result is symmetric, only the tiles on and below the diagonal are computed and each is
 // written to both places.
-// What bounds it is the matrix pipes: per block of 32 a 16 x 16 tile takes three instructions of 16 cycles.  Two buffers of 128-byte rows in LDS;
-// a wave holds Q's operands of a block in registers, so Q's half of a buffer is free after the first row of tiles and P's before the last
-// one: at these two places the waves meet and start the copies of the block after the next.  The operands of a row are requested a row ahead.
+// What bounds it is the matrix pipes: per block of 32 a 16 x 16 tile takes three instructions of 16 cycles (4096 x 4096: 1.1 .. 1.25 PFLOP/s of these, where a
+// large fp16 product of the vendor's library runs at 1.4 on the same card).  Two buffers in LDS; a wave holds Q's operands of a block in
+// registers, so Q's half of a buffer is free after the first row of tiles and P's before the last one: at these two places the waves meet and
+// start the copies of the block after the next.  The operands of a row are requested a row ahead.
+//
+// GRAM sums over l, and X stands as l rows of s: X is kept in this one orientation, half of the memory traffic of keeping both.  32 rows of a block are
+// copied as they are, a row's 32-byte segment q (16 hi or 16 lo parts) at segment q ^ f(row); ds_read_b64_tr_b16 turns 4 rows x 16 columns for 16
+// lanes, so that a lane gets eight entries of its column.  f takes the 16 rows that an instruction touches to 16 (at a side of 64: 8) segments.
+// APPLY: a lane's four results are neighbours along s, which is how X' stands.
 template <int MODE, typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
   constexpr int STAGE = (BM + BN) * 128, WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  static_assert(MODE != SYM || BM == BN, "");
+  constexpr bool TURNED = MODE == GRAM, HALF = MODE == GRAM || MODE == SYM;
+  static_assert(!HALF || BM == BN, "");
   static_assert(TM >= 4, "Q is copied between row 1 and row TM - 2");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
@@ -554,7 +559,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
   int64_t b = blockIdx.z;
   bool partial = false;
   int slot = 0;
-  if (MODE == SYM) {
+  if (HALF) {
     int id = blockIdx.x;
     if (id < a.whole) {
       id = xcd_order(id, a.whole);
@@ -575,25 +580,48 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
     tile_at(xcd_order(blockIdx.x, gridDim.x), (a.m + BM - 1) / BM, a.tiles_n, BM == 256 ? 4 : 8, ti, tj);
   }
   const int i0 = ti * BM, j0 = tj * BN;
-  const int lr = lane >> 3, lc = ((lane & 7) ^ lr) << 4;
-  // rows behind the last one repeat it (their results are not stored).  A lane's offset from its tile's first row: at most 256 rows of 2^24 + 128 bytes
-  constexpr int CP = BM / 8 / WAVES, CQ = BN / 8 / WAVES;
+  constexpr int CP = BM / 8 / WAVES, CQ = BN / 8 / WAVES;  // copies of 1024 bytes a wave
   static_assert(CP * 8 * WAVES == BM && CQ * 8 * WAVES == BN, "");
-  const char *pp = a.p.p + b * a.p.batch + i0 * a.p.ld + (int64_t)kb0 * 128, *pq = a.q.p + b * a.q.batch + j0 * a.q.ld + (int64_t)kb0 * 128;
+  const char *pp, *pq;
+  int64_t advance;
   uint32_t off_p[CP], off_q[CQ];
+  if (TURNED) {
+    // A copy is 1024 / (4 BM) rows.  Columns behind the last block repeat the first (their results are not stored); rows are whole blocks of 32.  An
+    // offset: at most 32 rows of 2^17 bytes.
+    constexpr int ROW = BM * 4, PER = 64 / (ROW / 16);
+    pp = a.p.p + b * a.p.batch + (int64_t)kb0 * 32 * a.p.ld;
+    pq = pp;
+    advance = 32 * a.p.ld;
+    const int row = lane / (ROW / 16), chunk = lane % (ROW / 16);
+    auto offset = [&](int k, int c0) {
+      const int r = k * PER + row, seg = (chunk >> 1) ^ (((r & 3) | ((r >> 3) & 3) << 2) & (ROW / 32 - 1));
+      const int at = c0 * 4 + seg * 32;
+      return (uint32_t)(r * (int)a.p.ld + (at < (int)a.p.ld ? at : 0) + (chunk & 1) * 16);
+    };
 #pragma unroll
-  for (int k = 0; k < CP; ++k) off_p[k] = (uint32_t)min((k * WAVES + w) * 8 + lr, a.m - 1 - i0) * (uint32_t)a.p.ld + lc;
+    for (int k = 0; k < CP; ++k) off_p[k] = offset(k * WAVES + w, i0);
 #pragma unroll
-  for (int k = 0; k < CQ; ++k) off_q[k] = (uint32_t)min((k * WAVES + w) * 8 + lr, a.n - 1 - j0) * (uint32_t)a.q.ld + lc;
+    for (int k = 0; k < CQ; ++k) off_q[k] = offset(k * WAVES + w, j0);
+  } else {
+    // rows behind the last one repeat it.  A lane's offset from its tile's first row: at most 256 rows of 2^17 bytes
+    const int lr = lane >> 3, lc = ((lane & 7) ^ lr) << 4;
+    pp = a.p.p + b * a.p.batch + i0 * a.p.ld + (int64_t)kb0 * 128;
+    pq = a.q.p + b * a.q.batch + j0 * a.q.ld + (int64_t)kb0 * 128;
+    advance = 128;
+#pragma unroll
+    for (int k = 0; k < CP; ++k) off_p[k] = (uint32_t)min((k * WAVES + w) * 8 + lr, a.m - 1 - i0) * (uint32_t)a.p.ld + lc;
+#pragma unroll
+    for (int k = 0; k < CQ; ++k) off_q[k] = (uint32_t)min((k * WAVES + w) * 8 + lr, a.n - 1 - j0) * (uint32_t)a.q.ld + lc;
+  }
   auto stage_p = [&](int buf) {
 #pragma unroll
     for (int k = 0; k < CP; ++k) stage8(pp + off_p[k], lds + buf * STAGE + (k * WAVES + w) * 1024);
-    pp += 128;
+    pp += advance;
   };
   auto stage_q = [&](int buf) {
 #pragma unroll
     for (int k = 0; k < CQ; ++k) stage8(pq + off_q[k], lds + buf * STAGE + BM * 128 + (k * WAVES + w) * 1024);
-    pq += 128;
+    pq += advance;
   };
   f32x4 acc[TM][TN];
 #pragma unroll
@@ -601,8 +629,24 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const int fr = lane & 15, fg = lane >> 4, wi = (w / WN) * (BM / WM), wj = (w % WN) * (BN / WN);
-  auto frag_p = [&](int buf, int i, int half) { return __builtin_bit_cast(f16x8, lds_chunk(lds + buf * STAGE, wi + i * 16 + fr, fg + 4 * half)); };
-  auto frag_q = [&](int buf, int j, int half) { return __builtin_bit_cast(f16x8, lds_chunk(lds + buf * STAGE + BM * 128, wj + j * 16 + fr, fg + 4 * half)); };
+  const int turn_row = 8 * fg + (fr >> 2), turn_seg = ((fr >> 2) | fg << 2) & (BM * 4 / 32 - 1), turn_at = turn_row * (BM * 4) + (fr & 3) * 8;
+  auto frag = [&](int part, int tile, int half) {  // part: byte offset of the operand in LDS, tile: its first row (GRAM: column)
+    if (TURNED) {
+      const int seg = (tile >> 5) * 4 + half * 2 + ((tile >> 4) & 1);
+      const char *q = lds + part + turn_at + ((seg ^ turn_seg) << 5);
+      typedef __attribute__((ext_vector_type(4))) __fp16 h4;
+      typedef __attribute__((address_space(3))) h4 lds_h4;
+      const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4 *)(lvoid *)q));
+      const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4 *)(lvoid *)(q + 4 * BM * 4)));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return __builtin_bit_cast(f16x8, lds_chunk(lds + part, tile + fr, fg + 4 * half));
+  };
+  auto frag_p = [&](int buf, int i, int half) { return frag(buf * STAGE, wi + i * 16, half); };
+  auto frag_q = [&](int buf, int j, int half) { return frag(buf * STAGE + BM * 128, wj + j * 16, half); };
+  auto multiply = [&](const f16x8 &p, const f16x8 &q, f32x4 c) {
+    return HALF ? __builtin_amdgcn_mfma_f32_16x16x32_f16(q, p, c, 0, 0, 0) : __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, c, 0, 0, 0);
+  };
   if (kb0 < kb1) {
     stage_p(0);
     stage_q(0);
@@ -644,15 +688,15 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
           pl_next = frag_p(buf ^ 1, 0, 1);
         }
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph, acc[i][j], 0, 0, 0);
+        for (int j = 0; j < TN; ++j) acc[i][j] = multiply(ph, ql[j], acc[i][j]);
         if (i == TM - 1) {
 #pragma unroll
           for (int j = 0; j < TN; ++j) ql[j] = frag_q(buf ^ 1, j, 1);
         }
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl, acc[i][j], 0, 0, 0);
+        for (int j = 0; j < TN; ++j) acc[i][j] = multiply(pl, qh[j], acc[i][j]);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph, acc[i][j], 0, 0, 0);
+        for (int j = 0; j < TN; ++j) acc[i][j] = multiply(ph, qh[j], acc[i][j]);
         if (i == TM - 1) {
 #pragma unroll
           for (int j = 0; j < TN; ++j) qh[j] = frag_q(buf ^ 1, j, 0);
@@ -667,37 +711,42 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
   const int mp = (a.m + 31) & ~31, np = (a.n + 31) & ~31;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int m = i0 + wi + i * 16 + fr;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = j0 + wj + j * 16 + fg * 4;
       f32x4 v = acc[i][j];
-      if (MODE == SYM && partial) {
-        *(f32x4 *)(a.part + (int64_t)slot * (BM * BN) + (m - i0) * BN + (n - j0)) = v;
-        continue;
-      }
       f32x4 d = {0.f, 0.f, 0.f, 0.f};
-      if (a.add != 0.f && m < a.m && n < np) d = get4(a.d.p + b * a.d.batch + (int64_t)m * a.d.ld, n);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = m < a.m && n + r < a.n ? fmaf(a.mul, v[r], a.add * d[r]) : 0.f;
-      if (MODE == LAST) {
-        if (m >= a.m || n >= a.n) continue;
-        T *q = (T *)a.o.p + (a.b0 + b) * a.o.batch + m * a.o.row + (int64_t)n * a.o.col;
-        if (a.vec && n + 4 <= a.n) {
-          write4(q, v[0], v[1], v[2], v[3]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < a.n) q[r * a.o.col] = from_f32<T>(v[r]);
+      if (HALF) {
+        const int m = i0 + wi + i * 16 + fr, n = j0 + wj + j * 16 + fg * 4;
+        if (partial) {
+          *(f32x4 *)(a.part + (int64_t)slot * (BM * BN) + (m - i0) * BN + (n - j0)) = v;
+          continue;
         }
-        continue;
-      }
-      if (m < a.m && n < np) put4(a.out.p + b * a.out.batch + (int64_t)m * a.out.ld, n, v);
-      if (MODE == SYM && ti == tj) continue;
-      if (m < mp) {
+        if (a.add != 0.f && m < a.m && n < np) d = get4(a.d.p + b * a.d.batch + (int64_t)m * a.d.ld, n);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = m < a.m && n + r < a.n ? fmaf(a.mul, v[r], a.add * d[r]) : 0.f;
+        if (m < a.m && n < np) put4(a.out.p + b * a.out.batch + (int64_t)m * a.out.ld, n, v);
+        if (ti == tj || m >= mp) continue;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (n + r < a.n) put1(a.out_t.p + b * a.out_t.batch + (int64_t)(n + r) * a.out_t.ld, m, v[r]);
+          if (n + r < a.n) put1(a.out.p + b * a.out.batch + (int64_t)(n + r) * a.out.ld, m, v[r]);
+      } else {
+        const int m = i0 + wi + i * 16 + fg * 4, n = j0 + wj + j * 16 + fr;
+        if (m >= mp || n >= np) continue;
+        if (n < a.n) d = get4(a.d.p + b * a.d.batch + (int64_t)n * a.d.ld, m);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = m + r < a.m && n < a.n ? fmaf(a.mul, v[r], a.add * d[r]) : 0.f;
+        if (MODE == APPLY) {
+          put4(a.out.p + b * a.out.batch + (int64_t)n * a.out.ld, m, v);
+        } else if (n < a.n) {
+          T *q = (T *)a.o.p + (a.b0 + b) * a.o.batch + m * a.o.row + (int64_t)n * a.o.col;
+          if (a.vec && m + 4 <= a.m) {
+            write4(q, v[0], v[1], v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (m + r < a.m) q[r * a.o.row] = from_f32<T>(v[r]);
+          }
+        }
       }
     }
   }
@@ -792,8 +841,8 @@ int full_side(int64_t m, int64_t n, int64_t batch, int64_t kb) {
 struct Layout {
   int64_t s, l, batch;
   int64_t chunks, chunk;                // small
-  int64_t x, xt[2], sq[2], norm, part, q;  // byte offsets
-  int64_t ldx, ldt;
+  int64_t xt[2], sq[2], norm, part, q;  // byte offsets
+  int64_t ldt, lp;
   int64_t bytes;
 };
 
@@ -817,11 +866,10 @@ Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     y.part = take(batch * y.chunks * y.s * y.s * 8);
     y.q = take(batch * y.s * y.s * 4);
   } else {
-    y.ldx = nmfk_round_up(y.l, 32) * 4;
+    y.lp = nmfk_round_up(y.l, 32);
     y.ldt = nmfk_round_up(y.s, 32) * 4;
-    y.x = take(batch * y.s * y.ldx);
-    y.xt[0] = take(batch * y.l * y.ldt);
-    y.xt[1] = take(batch * y.l * y.ldt);
+    y.xt[0] = take(batch * y.lp * y.ldt);
+    y.xt[1] = take(batch * y.lp * y.ldt);
     for (int k = 0; k < 2; ++k) y.sq[k] = take(batch * y.s * y.ldt);
     y.norm = take(batch * NORM_PARTS * 8);
     int64_t part = 0;
@@ -918,11 +966,11 @@ void gemm_tile(const GemmArgs &a, dim3 grid, hipStream_t st) {
   gemm_kernel<MODE, T, BM, BN, WM, WN><<<grid, 64 * WM * WN, BYTES, st>>>(a);
 }
 
-// a symmetric product: the tiles on and below the diagonal
+// GRAM or SYM: the tiles on and below the diagonal
+template <int MODE>
 void gemm_sym(GemmArgs a, unsigned batch, hipStream_t st) {
   const SymPlan q = sym_plan(a.m, batch, a.kb);
   a.n = a.m;
-  a.out_t = a.out;
   a.tiles = q.tiles;
   a.whole = q.whole;
   a.rest = q.rest;
@@ -930,9 +978,9 @@ void gemm_sym(GemmArgs a, unsigned batch, hipStream_t st) {
   a.kb_split = q.kb_split;
   const dim3 grid((unsigned)(q.whole + q.rest * q.splits));
   if (q.side == 64)
-    gemm_tile<SYM, float, 64, 64, 1, 2>(a, grid, st);
+    gemm_tile<MODE, float, 64, 64, 1, 2>(a, grid, st);
   else
-    gemm_tile<SYM, float, 128, 128, 2, 2>(a, grid, st);
+    gemm_tile<MODE, float, 128, 128, 2, 2>(a, grid, st);
   if (!q.rest) return;
   if (q.side == 64)
     sym_join_kernel<64><<<dim3((unsigned)q.rest, 4), 256, 0, st>>>(a);
@@ -959,53 +1007,51 @@ void gemm_full(GemmArgs a, unsigned batch, hipStream_t st) {
 template <typename T>
 int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, const double *coef, char *work, hipStream_t st) {
   const int s = (int)y.s, l = (int)y.l, ks = (int)nmfk_div_up(s, 32), kl = (int)nmfk_div_up(l, 32);
-  const int64_t bx = y.s * y.ldx, bt = y.l * y.ldt, bs = y.s * y.ldt;
+  const int64_t bt = y.lp * y.ldt, bs = y.s * y.ldt;
   for (int64_t b0 = 0; b0 < y.batch; b0 += BATCH) {
     const unsigned nb = (unsigned)std::min<int64_t>(BATCH, y.batch - b0);
-    Split X = {work + y.x + b0 * bx, bx, y.ldx}, XT = {work + y.xt[0] + b0 * bt, bt, y.ldt}, NT = {work + y.xt[1] + b0 * bt, bt, y.ldt};
+    Split X = {work + y.xt[0] + b0 * bt, bt, y.ldt}, N = {work + y.xt[1] + b0 * bt, bt, y.ldt};  // X', l rows of s
     Split S = {work + y.sq[0] + b0 * bs, bs, y.ldt}, P = {work + y.sq[1] + b0 * bs, bs, y.ldt};
     double *norm = (double *)(work + y.norm) + b0 * NORM_PARTS;
     double u = 1.0;  // bound of the singular values of X; e?: the power of two a matrix is scaled by
     int ex = exponent(1.01 * u);
     norm_kernel<T><<<dim3(NORM_PARTS, nb), 256, 0, st>>>(g, b0, s, l, norm, g.row == 1 || g.col == 1);
-    split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, ldexp(1.0, ex), X, XT);
+    split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, ldexp(1.0, ex), X);
     for (int k = 0; k < steps; ++k) {
       const double ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
       const int es = exponent(1.02 * u * u), ep = exponent(1.02 * std::max(peak(0, cb, cc, u, EVEN), 1e-3));
       GemmArgs a = {};
       a.part = (float *)(work + y.part);  // (a launch's own: the next one starts behind the join)
       a.m = s;
-      a.p = a.q = X;
+      a.p = X;
       a.kb = kl;
       a.mul = (float)ldexp(1.0, es - 2 * ex);
       a.out = S;
-      gemm_sym(a, nb, st);
+      gemm_sym<GRAM>(a, nb, st);
       a.p = a.q = a.d = S;
       a.kb = ks;
       a.mul = (float)(cc * ldexp(1.0, ep - 2 * es));
       a.add = (float)(cb * ldexp(1.0, ep - es));
       a.out = P;
-      gemm_sym(a, nb, st);
+      gemm_sym<SYM>(a, nb, st);
       u = std::max(peak(ca, cb, cc, u, ODD), 1e-3);
       const bool last = k + 1 == steps;
       const int nx = last ? 0 : exponent(1.02 * u);
       a.p = P;
-      a.q = XT;
-      a.d = X;
+      a.q = a.d = X;
       a.n = l;
       a.mul = (float)ldexp(1.0, nx - ep - ex);
       a.add = (float)(ca * ldexp(1.0, nx - ex));
-      a.out = X;  // the entry [i, j] of X is read by the lane that overwrites it, and by no other
-      a.out_t = NT;
+      a.out = N;
       if (last) {
         a.o = o;
         a.b0 = b0;
-        a.vec = o.col == 1;
+        a.vec = o.row == 1;
         gemm_full<LAST, T>(a, nb, st);
       } else {
         gemm_full<APPLY, float>(a, nb, st);
       }
-      std::swap(XT, NT);
+      std::swap(X, N);
       ex = nx;
     }
   }
