@@ -536,6 +536,41 @@ __device__ __forceinline__ void sym_tile(int id, int &ti, int &tj) {  // the til
   tj = id - ti * (ti + 1) / 2;
 }
 
+// Operands of GRAM: the hi and lo parts of a tile's columns, eight entries a lane, each out of two reads that turn 4 x 16 entries (OFF: bytes from the first
+// four rows to the next).  In assembly with their wait, because the compiler puts a wait for all copies into LDS before the builtin.
+using pair64 = __attribute__((ext_vector_type(2))) uint32_t;
+struct Turned {
+  f16x8 hi, lo;
+};
+__device__ __forceinline__ f16x8 join8(pair64 a, pair64 b) {
+  const i32x4 v = {(int)a[0], (int)a[1], (int)b[0], (int)b[1]};
+  return __builtin_bit_cast(f16x8, v);
+}
+template <int OFF>
+__device__ __forceinline__ Turned read_turned(uint32_t hi, uint32_t lo) {
+  pair64 a, b, c, d;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\tds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+      : "v"(hi), "v"(lo), "n"(OFF)
+      : "memory");
+  return {join8(a, b), join8(c, d)};
+}
+template <int OFF>
+__device__ __forceinline__ void read_turned2(uint32_t h0, uint32_t l0, uint32_t h1, uint32_t l1, Turned &x, Turned &y) {
+  pair64 a, b, c, d, e, f, g, h;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(f), "=&v"(g), "=&v"(h)
+      : "v"(h0), "v"(l0), "v"(h1), "v"(l1), "n"(OFF)
+      : "memory");
+  x = {join8(a, b), join8(c, d)};
+  y = {join8(e, f), join8(g, h)};
+}
+
 // BM x BN outputs a workgroup, WM x WN waves.  GRAM and SYM: the result is symmetric, only the tiles on and below the diagonal are computed and each is
 // written to both places.
 // What bounds it is the matrix pipes: per block of 32 a 16 x 16 tile takes three instructions of 16 cycles (4096 x 4096: 1.1 .. 1.25 PFLOP/s of these, where a
@@ -630,20 +665,30 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
     for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const int fr = lane & 15, fg = lane >> 4, wi = (w / WN) * (BM / WM), wj = (w % WN) * (BN / WN);
   const int turn_row = 8 * fg + (fr >> 2), turn_seg = ((fr >> 2) | fg << 2) & (BM * 4 / 32 - 1), turn_at = turn_row * (BM * 4) + (fr & 3) * 8;
-  auto frag = [&](int part, int tile, int half) {  // part: byte offset of the operand in LDS, tile: its first row (GRAM: column)
-    if (TURNED) {
-      const int seg = (tile >> 5) * 4 + half * 2 + ((tile >> 4) & 1);
-      const char *q = lds + part + turn_at + ((seg ^ turn_seg) << 5);
-      typedef __attribute__((ext_vector_type(4))) __fp16 h4;
-      typedef __attribute__((address_space(3))) h4 lds_h4;
-      const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4 *)(lvoid *)q));
-      const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4 *)(lvoid *)(q + 4 * BM * 4)));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    return __builtin_bit_cast(f16x8, lds_chunk(lds + part, tile + fr, fg + 4 * half));
+  auto turned = [&](int part, int tile, int half) {  // part: byte offset of the operand in LDS, tile: its first column
+    const int seg = (tile >> 5) * 4 + half * 2 + ((tile >> 4) & 1);
+    return (uint32_t)(uintptr_t)(lvoid *)(lds + part + turn_at + ((seg ^ turn_seg) << 5));
   };
-  auto frag_p = [&](int buf, int i, int half) { return frag(buf * STAGE, wi + i * 16, half); };
-  auto frag_q = [&](int buf, int j, int half) { return frag(buf * STAGE + BM * 128, wj + j * 16, half); };
+  auto read_p = [&](int buf, int i, f16x8 &h, f16x8 &l) {
+    const int part = buf * STAGE, tile = wi + i * 16;
+    if (TURNED) {
+      const Turned v = read_turned<16 * BM>(turned(part, tile, 0), turned(part, tile, 1));
+      h = v.hi, l = v.lo;
+    } else {
+      h = __builtin_bit_cast(f16x8, lds_chunk(lds + part, tile + fr, fg));
+      l = __builtin_bit_cast(f16x8, lds_chunk(lds + part, tile + fr, fg + 4));
+    }
+  };
+  auto frag_q = [&](int buf, int j, int half) { return __builtin_bit_cast(f16x8, lds_chunk(lds + buf * STAGE + BM * 128, wj + j * 16 + fr, fg + 4 * half)); };
+  auto turn_q = [&](int buf, f16x8 (&h)[TN], f16x8 (&l)[TN]) {
+    const int part = buf * STAGE + BM * 128;
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      Turned x, y;
+      read_turned2<16 * BM>(turned(part, wj + j * 16, 0), turned(part, wj + j * 16, 1), turned(part, wj + j * 16 + 16, 0), turned(part, wj + j * 16 + 16, 1), x, y);
+      h[j] = x.hi, l[j] = x.lo, h[j + 1] = y.hi, l[j + 1] = y.lo;
+    }
+  };
   auto multiply = [&](const f16x8 &p, const f16x8 &q, f32x4 c) {
     return HALF ? __builtin_amdgcn_mfma_f32_16x16x32_f16(q, p, c, 0, 0, 0) : __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, c, 0, 0, 0);
   };
@@ -656,11 +701,16 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
       stage_p(1);
       stage_q(1);
     }
-    f16x8 qh[TN], ql[TN], ph = frag_p(0, 0, 0), pl = frag_p(0, 0, 1);
+    f16x8 qh[TN], ql[TN], ph, pl;
+    read_p(0, 0, ph, pl);
+    if (TURNED) {
+      turn_q(0, qh, ql);
+    } else {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      qh[j] = frag_q(0, j, 0);
-      ql[j] = frag_q(0, j, 1);
+      for (int j = 0; j < TN; ++j) {
+        qh[j] = frag_q(0, j, 0);
+        ql[j] = frag_q(0, j, 1);
+      }
     }
     int buf = 0;
     for (int kb = kb0; kb < kb1; ++kb) {  // (behind the last block the operands of "the next" are whatever stands in LDS, unused)
@@ -673,8 +723,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
         }
         f16x8 ph_next, pl_next;
         if (i < TM - 1) {
-          ph_next = frag_p(buf, i + 1, 0);
-          pl_next = frag_p(buf, i + 1, 1);
+          read_p(buf, i + 1, ph_next, pl_next);
         } else {
           if (copy) {
             staged_but<CQ>();  // of the block after the next, Q may still be on its way
@@ -684,12 +733,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
             staged();
             meet();
           }
-          ph_next = frag_p(buf ^ 1, 0, 0);
-          pl_next = frag_p(buf ^ 1, 0, 1);
+          read_p(buf ^ 1, 0, ph_next, pl_next);
         }
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = multiply(ph, ql[j], acc[i][j]);
-        if (i == TM - 1) {
+        if (i == TM - 1 && !TURNED) {
 #pragma unroll
           for (int j = 0; j < TN; ++j) ql[j] = frag_q(buf ^ 1, j, 1);
         }
@@ -698,8 +746,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = multiply(ph, qh[j], acc[i][j]);
         if (i == TM - 1) {
+          if (TURNED) {
+            turn_q(buf ^ 1, qh, ql);
+          } else {
 #pragma unroll
-          for (int j = 0; j < TN; ++j) qh[j] = frag_q(buf ^ 1, j, 0);
+            for (int j = 0; j < TN; ++j) qh[j] = frag_q(buf ^ 1, j, 0);
+          }
         }
         ph = ph_next;
         pl = pl_next;
