@@ -81,8 +81,11 @@ enum { ROWS_ROWS = 0, B_TILES = 1, A_TILES = 2 };
 
 // A workgroup's tile of BM x BN outputs over its range of blocks: WM x WN waves, each (BM / WM) x (BN / WN).
 // Two buffers of 128-byte rows in LDS; the copies into one are in flight while the other is multiplied.  A wave holds B's operands of a block in
-// registers, so B's half of a buffer is free after the first row of tiles and A's before the last one: at these two places the waves meet and
-// start the copies of the block after the next.  The operands of the next block are read while the matrix pipe is still busy with the last row of this one.
+// registers, so B's half of a buffer is free after the first row of tiles and A's before the last two: at these two places the waves meet, and
+// the copies of the block after the next start, spread over the rows (all at once: 6 % slower).  The operands of the next block are read while the matrix
+// pipe is still busy with the last row of this one.
+// What bounds it at 8192^3 (256 x 256, 490 .. 540 microseconds, 2.0 .. 2.2 PFLOP/s on different cards): the matrix and vector instructions of a block alone, without
+// any memory, take 413, the additions about 35 of these; the copies add 100.  The same in 32 x 32 x 64 instructions: 7 % slower.
 // The first operand of the matrix instruction is B, so that a lane's four outputs are neighbours in a row of Y.
 template <int BM, int BN, int WM, int WN, int MODE, typename F, typename T, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
@@ -122,14 +125,18 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
     ps_ld[i] = is_a ? p.ldsa : p.ldsb;
     ps[i] = (is_a ? p.sa + (min(m0 + row + lane, p.m - 1) >> p.ashift) : p.sb + (min(n0 + row - BM + lane, p.n - 1) >> p.bshift)) + kb0 * ps_ld[i];
   }
-  auto stage_b = [&](int buf) {  // the next block in order
-#pragma unroll
-    for (int i = 0; i < CB; ++i) stage8(pb + off_b[i], lds + buf * STAGE + BM * 128 + (i * WAVES + w) * 1024);
-    pb += 128;
+  // the copies of the next block in order: B's one by one, A's in two halves
+  auto copy_b = [&](int buf, int i) {
+    stage8(pb + off_b[i], lds + buf * STAGE + BM * 128 + (i * WAVES + w) * 1024);
+    if (i == CB - 1) pb += 128;
   };
-  auto stage_a = [&](int buf) {
+  auto copy_a_first = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < CA; ++i) stage8(pa + off_a[i], lds + buf * STAGE + (i * WAVES + w) * 1024);
+    for (int i = 0; i < CA / 2; ++i) stage8(pa + off_a[i], lds + buf * STAGE + (i * WAVES + w) * 1024);
+  };
+  auto copy_a_second = [&](int buf) {
+#pragma unroll
+    for (int i = CA / 2; i < CA; ++i) stage8(pa + off_a[i], lds + buf * STAGE + (i * WAVES + w) * 1024);
     pa += 128;
     float *sc = (float *)(lds + 2 * STAGE + buf * SC);
 #pragma unroll
@@ -161,14 +168,16 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
     for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const int blocks = kb1 - kb0;
   if (blocks > 0) {
-    stage_a(0);
-    stage_b(0);
+    auto copy_all = [&](int buf) {
+      copy_a_first(buf);
+      copy_a_second(buf);
+#pragma unroll
+      for (int i = 0; i < CB; ++i) copy_b(buf, i);
+    };
+    copy_all(0);
     staged();
     meet();
-    if (blocks > 1) {
-      stage_a(1);
-      stage_b(1);
-    }
+    if (blocks > 1) copy_all(1);
     // The matrix instructions of a block are one sequence n = i * TN + j.  The vector instructions add the tile LAG places behind the one the
     // matrix pipe has begun, and the operands of row i + 2 are requested when row i begins.
     constexpr int LAG = 2, LEN = TM * TN;
@@ -194,21 +203,24 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
       if (MODE == B_TILES) sa[0] *= so;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        if (i == 1 && copy) {
-          meet();
-          stage_b(buf);
+        if (i == 1 && copy) meet();
+        if (i >= 1 && i < TM - 2 && copy) {  // B's copies, spread over the rows 1 .. TM - 3
+          constexpr int PER = (CB + TM - 4) / (TM - 3);
+#pragma unroll
+          for (int c = (i - 1) * PER; c < i * PER && c < CB; ++c) copy_b(buf, c);
         }
         if (i == TM - 2) {
           if (copy) {
             staged_but<CB>();  // of the block after the next, B may still be on its way
             meet();
-            stage_a(buf);
+            copy_a_first(buf);
           } else {
             staged();
             meet();
           }
           if (MODE != ROWS_ROWS) so_next = one(buf ^ 1);
         }
+        if (i == TM - 1 && copy) copy_a_second(buf);
         const int from = i + 2 < TM ? buf : buf ^ 1, row = (i + 2) % TM;
         fa[2] = frag_a(from, row);
         if (MODE != A_TILES) sa[2] = scales(from)[rm + row * 16];
@@ -223,6 +235,11 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[oi][oj][r] = fmaf(part[o][r], MODE == B_TILES ? s : MODE == A_TILES ? sb[oj][r] : s * sb[oj][r], acc[oi][oj][r]);
           asm volatile("" : "+v"(acc[oi][oj]));  // the additions do not move behind a branch
+          if (MODE != ROWS_ROWS && F::STEPS == 1) {  // a matrix instruction, a read from LDS, the additions
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+          }
           if (MODE != B_TILES && oi == TM - 1) {  // the last use of this scale: the next block's
             const f32x4 v = scale_b(i == 0 ? buf : buf ^ 1, oj);
             sb[oj] = MODE == A_TILES ? (i == 0 ? so : so_next) * v : v;
