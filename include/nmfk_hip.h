@@ -290,9 +290,9 @@ int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, cons
  * its three coefficients (a, b, c), X <- a X + (b S + c S S) X where S = X X' (rows <= cols; otherwise of the transpose).  Singular values
  * go towards one (which ones and how close is the coefficients' doing), singular vectors stay.  Accuracy of fp32 or better inside.
  * A matrix of zeros gives zeros; one with an entry that is not finite gives NaN everywhere.
- *  G, O       entry (i, j) of matrix r at G[r * g_batch + i * g_row + j * g_col]; O likewise, not overlapping G
+ *  G, O       entry (i, j) of matrix r at G[r * g_batch + i * g_row + j * g_col]; O likewise: G itself with the same strides, or not overlapping it
  *  coefficients   3 * steps doubles on the HOST (1 to 32 steps), read before the call returns; refused when they let a singular value grow beyond 64
- * The shorter side is at most 32768. */
+ * The shorter side is at most 32768, the entries of all matrices together 2^38. */
 int nmfk_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int64_t *bytes);
 int nmfk_orthogonalize(int device, void *stream, int dtype, int64_t batch, int64_t rows, int64_t cols, const void *G,
                        int64_t g_batch, int64_t g_row, int64_t g_col, void *O, int64_t o_batch, int64_t o_row, int64_t o_col,

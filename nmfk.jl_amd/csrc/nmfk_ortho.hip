@@ -17,6 +17,7 @@ namespace {
 
 constexpr int SMALL = 64;
 constexpr int64_t BATCH = 32768;  // matrices a launch
+constexpr double TINY = 1e-20;    // bounds below it are not followed any further
 
 struct Strided {
   char *p;
@@ -1071,7 +1072,7 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
     split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, ldexp(1.0, ex), X);
     for (int k = 0; k < steps; ++k) {
       const double ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
-      const int es = exponent(1.02 * u * u), ep = exponent(1.02 * std::max(peak(0, cb, cc, u, EVEN), 1e-3));
+      const int es = exponent(1.02 * u * u), ep = exponent(1.02 * std::max(peak(0, cb, cc, u, EVEN), TINY));
       GemmArgs a = {};
       a.part = (float *)(work + y.part);  // (a launch's own: the next one starts behind the join)
       a.m = s;
@@ -1086,7 +1087,7 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
       a.add = (float)(cb * ldexp(1.0, ep - es));
       a.out = P;
       gemm_sym<SYM>(a, nb, st);
-      u = std::max(peak(ca, cb, cc, u, ODD), 1e-3);
+      u = std::max(peak(ca, cb, cc, u, ODD), TINY);
       const bool last = k + 1 == steps;
       const int nx = last ? 0 : exponent(1.02 * u);
       a.p = P;
@@ -1114,6 +1115,7 @@ int ortho_sizes(int64_t batch, int64_t rows, int64_t cols, const char *who) {
   if (batch < 0 || rows < 0 || cols < 0) return fail(NMFK_ERR_BAD_ARG, std::string(who) + ": negative size");
   if (batch > ((int64_t)1 << 22) || std::max(rows, cols) > ((int64_t)1 << 22)) return fail(NMFK_ERR_UNSUPPORTED, std::string(who) + ": a size above 2^22");
   if (std::min(rows, cols) > 32768) return fail(NMFK_ERR_UNSUPPORTED, std::string(who) + ": both sides above 32768");
+  if (rows && cols && batch > ((int64_t)1 << 38) / (rows * cols)) return fail(NMFK_ERR_UNSUPPORTED, std::string(who) + ": more than 2^38 entries");
   return NMFK_OK;
 }
 

@@ -3,7 +3,7 @@
 `rangebasis`, an orthonormal basis of the leading directions of a large X.  The reference leaves such numerics to other packages.
 
 The operators take and return torch tensors on the GPU; they run on torch's current stream of the tensors' device, do not wait, and can be
-captured into a graph.  `rangebasis` takes a numpy array like `execute` does, or a tensor."""
+captured into a graph (a Quantized matrix used on another stream than its own needs what a tensor needs there: the streams ordered, the object kept).  `rangebasis` takes a numpy array like `execute` does, or a tensor."""
 import ctypes as C
 import functools
 
@@ -203,12 +203,18 @@ def product_grads(dY, At, Bt, dtype=None):
     return product(q, Bt, dtype), product(t, At, dtype)
 
 
+def _extent(x):
+    """first byte of a tensor and the one behind its last"""
+    at = x.data_ptr()
+    return at, at + (sum(st * (n - 1) for st, n in zip(x.stride(), x.shape)) + 1) * x.element_size()
+
+
 def orthogonalize(G, steps=5, coefficients=None, out=None):
     """The orthogonal factor of G (..., rows, cols), or of each matrix of a stack, by Newton-Schulz products: X = G / |G|_F, then `steps`
     times X <- a X + (b S + c S S) X, S = X X' (of the transpose where rows > cols).  coefficients: (a, b, c), or one such triple per step.
     The default five steps bring every singular value from about 0.003 |G|_F upwards to between 0.68 and 1.13, which is what an update wants;
     for orthonormal rows or columns add steps with (1.875, -1.25, 0.375).  Sums in 32 bits or more, one rounding to G's type.
-    Zeros give zeros, an entry that is not finite gives NaN in its matrix."""
+    Zeros give zeros, an entry that is not finite gives NaN in its matrix.  out: where to write, G itself or apart from it."""
     torch = _torch()
     _tensor(G, "G", ndim=0)
     if G.dim() < 2:
@@ -228,13 +234,23 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
         _tensor(out, "out", ndim=0)
         if out.shape != G.shape or out.dtype != G.dtype or out.device != G.device:
             raise _bad("out must have G's shape, type and GPU")
+        if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+            raise _bad("out must have a place for every entry")
+        if out.numel() and not (out.data_ptr() == G.data_ptr() and out.stride() == G.stride()):
+            (a0, a1), (b0, b1) = _extent(out), _extent(G)
+            if a0 < b1 and b0 < a1:
+                raise _bad("out must be G itself or not overlap it")
     g, o = G, out
     if G.dim() == 2:
         (r, c), b = G.shape, 1
         gs, os = (0, *G.stride()), (0, *out.stride())
     else:
         if G.dim() > 3:
-            g, o = G.reshape(-1, *G.shape[-2:]), out.view(-1, *out.shape[-2:])
+            try:
+                o = out.view(-1, *out.shape[-2:])
+            except RuntimeError:
+                raise _bad("the leading dimensions of out must fold into one") from None
+            g = o if out.data_ptr() == G.data_ptr() else G.reshape(-1, *G.shape[-2:])
         b, r, c = g.shape
         gs, os = g.stride(), o.stride()
     dev, nb = G.device, _orthogonalize_workspace(b, r, c)
@@ -249,6 +265,7 @@ def rangebasis(X, k, oversample=8, iterations=2, seed=0, device=None):
     orthogonalized.  Returns (Q, B, sigma): Q (n x k), B = Q' X (k x m, so X is near Q B), and sigma, the k leading singular values of X as the
     basis sees them.  Next to a sweep: sigma says where the candidate ranks end, Q and B are X compressed.  X is read once in 32 bits and kept in
     8, so sigma carries 8-bit noise: of about 3 % of |X| / sqrt(max(n, m)), below which nothing is resolved.
+    Directions that X does not have (k above its rank) come back as noise of that size, or zero.
     X: a numpy array (results are numpy arrays) or a torch tensor on the GPU (results are tensors).  NaN (missing data) is refused."""
     torch = _torch()
     host = not isinstance(X, torch.Tensor)

@@ -396,6 +396,60 @@ def test_orthogonalize_special(P, r, c):
             P.orthogonalize(g, **bad)
 
 
+@pytest.mark.parametrize("s,l", [(7, 500), (16, 64), (30, 900), (64, 200), (90, 140), (200, 300)])
+def test_orthogonalize_in_place_and_overlap(P, s, l):
+    for shape in ((3, s, l), (3, l, s)):
+        g = randn(16, *shape)
+        want = P.orthogonalize(g)
+        keep = g.clone()
+        assert P.orthogonalize(g, out=g) is g and torch.equal(g, want)
+        t = keep.mT.contiguous().mT  # the other layout
+        P.orthogonalize(t, out=t)
+        assert torch.allclose(t, want, rtol=0, atol=2.0 ** -18)
+        g4 = keep.clone()[None]
+        P.orthogonalize(g4, out=g4)
+        assert torch.equal(g4[0], want)
+        big = torch.cat([keep, keep], 0)
+        for bad in (big[1:4], big[0:1].expand(3, -1, -1), big[:3].mT.mT[:, :, :].flip(0)[:0].expand(0, *shape[1:])):
+            with pytest.raises(P.NMFkError):
+                P.orthogonalize(big[:3], out=bad)
+
+
+def test_orthogonalize_many_and_far(P):
+    """more matrices than a launch takes, and offsets beyond 2^31 entries"""
+    g = torch.randn(70000, 3, 5, device="cuda")
+    o = P.orthogonalize(g)
+    pick = [0, 1, 32767, 32768, 65535, 65536, 69999]
+    check_ortho(o[pick], g[pick])
+    g = torch.randn(33000, 65, 66, device="cuda")
+    o = P.orthogonalize(g, steps=2)
+    pick = [0, 32767, 32768, 32999]
+    check_ortho(o[pick], g[pick], 2)
+    del g, o
+    g = torch.empty(300000, 16, 512, device="cuda").uniform_(-1, 1)  # 2.5e9 entries
+    o = P.orthogonalize(g, steps=2)
+    pick = [0, 262143, 262144, 299999]
+    check_ortho(o[pick], g[pick], 2)
+    del g, o
+    big = torch.empty(2, 70, 1 << 24, device="cuda")
+    big.uniform_(-1, 1)
+    for bad in (big,):  # a side above 2^22
+        with pytest.raises(P.NMFkError) as e:
+            P.orthogonalize(bad)
+        assert e.value.code == 6
+    v = big[:, :, ::4095]  # strides far apart: 70 rows of 4098 entries, the last one 2^30 entries away
+    check_ortho(P.orthogonalize(v, steps=2), v, 2)
+
+
+def test_orthogonalize_coefficients_that_shrink(P):
+    for s in (20, 100):
+        g = randn(17, s, 150)
+        cf = [(1e-3, 0.0, 0.0), (1e-3, 1e-3, 0.0), (1e4 / 100, 0.0, 0.0)]
+        o = P.orthogonalize(g, 3, cf)
+        want, _ = ref_ortho(g, 3, cf)
+        assert float((o.double() - want).abs().max()) <= 2.0 ** -18 * float(want.abs().max())
+
+
 # ---- as they are used together --------------------------------------------------------------------------------------------------
 
 def test_rangebasis(P):
@@ -464,6 +518,33 @@ def test_operators_run_on_the_current_stream(P):
     torch.cuda.synchronize()
     for o in outs:
         assert all(torch.equal(a, w) for a, w in zip(o, want))
+
+
+def test_calls_from_two_threads(P):
+    """each thread on its own stream: nothing is shared between calls"""
+    import threading
+
+    x, b, g, h = randn(1, 60, 9000), randn(2, 70, 9000), randn(3, 2, 3000, 20), randn(4, 150, 400)
+    run = lambda: (P.product(P.quantize(x), P.quantize(b)), *P.quantize(h, both=True)[1].values.view(torch.uint8)[None], P.orthogonalize(g), P.orthogonalize(h))
+    want = run()
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = run()
+                s.synchronize()
+                if not all(torch.equal(a, w) for a, w in zip(got, want)):
+                    bad.append(1)
+
+    ts = [threading.Thread(target=work) for _ in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
 
 
 def test_two_captured_graphs_and_eager_calls(P):

@@ -104,6 +104,10 @@ def test_orthogonalize_of_nothing_and_of_too_much(NMFk):
     assert L.nmfk_orthogonalize_workspace(1, 40000, 40000, C.byref(nb)) == 6
     assert L.nmfk_orthogonalize_workspace(1, 0, 5, C.byref(nb)) == 0 and nb.value == 0
     assert L.nmfk_orthogonalize_workspace(1, 5, 5, None) == 1
+    for batch, rows, cols in ((1 << 22, 32768, 32768), (1 << 22, 64, 2048), (1 << 22, 1 << 22, 64)):  # nothing divides by zero on the way to the refusal
+        assert L.nmfk_orthogonalize_workspace(batch, rows, cols, C.byref(nb)) == 6
+    for batch, rows, cols in ((1 << 17, 1024, 2048), (256, 32768, 32768), (1, 1 << 22, 32768), (1 << 22, 256, 256), (1 << 22, 1, 1)):
+        assert L.nmfk_orthogonalize_workspace(batch, rows, cols, C.byref(nb)) == 0 and nb.value > 0
 
 
 def test_python_entry_points_refuse_what_is_not_on_the_gpu(NMFk):
