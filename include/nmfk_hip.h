@@ -286,6 +286,15 @@ int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, cons
                  int64_t ldsa, int a_tiles, const uint8_t *B, int64_t ldb, const float *sB, int64_t ldsb, int b_tiles, int dtype,
                  void *Y, int64_t ldy, void *work, int64_t work_bytes);
 
+/* The backward pass of Y = A * B' in one call: dY (m x n, entry (i, j) at dY[i * row_stride + j * col_stride], one of the strides 1) and its
+ * transpose are quantized by rows, then dA (m x k) = dY8 * (B'8)' and dB (n x k) = dY'8 * (A'8)'.  At (k x m) and Bt (k x n) are the
+ * transposes of A and B as nmfk_quantize leaves them (tvalues, tscales).  The two products run one behind the other. */
+int nmfk_product_grads_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes);
+int nmfk_product_grads(int device, void *stream, int64_t m, int64_t n, int64_t k, int dy_dtype, const void *dY, int64_t row_stride,
+                       int64_t col_stride, const uint8_t *At, int64_t ldat, const float *sAt, int64_t ldsat, int at_tiles,
+                       const uint8_t *Bt, int64_t ldbt, const float *sBt, int64_t ldsbt, int bt_tiles, int dtype, void *dA,
+                       int64_t ldda, void *dB, int64_t lddb, void *work, int64_t work_bytes);
+
 /* The orthogonal factor of each of `batch` matrices G (rows x cols) by Newton-Schulz products: X = G / |G|_F, then for every step, with
  * its three coefficients (a, b, c), X <- a X + (b S + c S S) X where S = X X' (rows <= cols; otherwise of the transpose).  Singular values
  * go towards one (which ones and how close is the coefficients' doing), singular vectors stay.  Accuracy of fp32 or better inside.

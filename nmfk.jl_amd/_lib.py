@@ -119,6 +119,8 @@ def lib():
     L.nmfk_quantize.argtypes = [ci, vp, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp, i64, vp, i64, vp, i64]
     L.nmfk_product_workspace.argtypes = [i64, i64, i64, ci, i64p]
     L.nmfk_product.argtypes = [ci, vp, i64, i64, i64, vp, i64, vp, i64, ci, vp, i64, vp, i64, ci, ci, vp, i64, vp, i64]
+    L.nmfk_product_grads_workspace.argtypes = [i64, i64, i64, ci, i64p]
+    L.nmfk_product_grads.argtypes = [ci, vp, i64, i64, i64, ci, vp, i64, i64, vp, i64, vp, i64, ci, vp, i64, vp, i64, ci, ci, vp, i64, vp, i64, vp, i64]
     L.nmfk_orthogonalize_workspace.argtypes = [i64, i64, i64, i64p]
     L.nmfk_orthogonalize.argtypes = [ci, vp, ci, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, ci, vp, vp, i64]
     _lib = L

@@ -529,3 +529,60 @@ NMFK_EXPORT int nmfk_product(int device, void *stream, int64_t m, int64_t n, int
   if (dtype == NMFK_BF16) return prod_run<Bytes, bf16>(p, q, work, st);
   return prod_run<Bytes, _Float16>(p, q, work, st);
 }
+
+// ---- the backward pass -------------------------------------------------------------------------------------------------------------
+
+namespace {
+
+struct GradLayout {
+  int64_t ldq, ldt;                   // bytes of a row of dY and of its transpose in 8 bits
+  int64_t q, qs, t, ts, work, bytes;  // byte offsets: dY in 8 bits and its scales, its transpose and its, what the two products need (in turn)
+};
+
+int grad_layout(int64_t m, int64_t n, int64_t k, int dtype, GradLayout &y) {
+  int64_t wa = 0, wb = 0;
+  if (int rc = nmfk_product_workspace(m, k, n, dtype, &wa)) return rc;
+  if (int rc = nmfk_product_workspace(n, k, m, dtype, &wb)) return rc;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += nmfk_round_up(bytes, 256);
+    return o;
+  };
+  y.ldq = nmfk_round_up(n, 128);
+  y.ldt = nmfk_round_up(m, 128);
+  y.q = take(m * y.ldq);
+  y.qs = take(4 * m * (y.ldq / 128));
+  y.t = take(n * y.ldt);
+  y.ts = take(4 * n * (y.ldt / 128));
+  y.work = take(std::max(wa, wb));
+  y.bytes = at;
+  return NMFK_OK;
+}
+
+}  // namespace
+
+NMFK_EXPORT int nmfk_product_grads_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes) {
+  if (!bytes) return fail(NMFK_ERR_BAD_ARG, "nmfk_product_grads_workspace: null pointer");
+  GradLayout y;
+  if (int rc = grad_layout(m, n, k, dtype, y)) return rc;
+  *bytes = y.bytes;
+  return NMFK_OK;
+}
+
+NMFK_EXPORT int nmfk_product_grads(int device, void *stream, int64_t m, int64_t n, int64_t k, int dy_dtype, const void *dY, int64_t row_stride,
+                                   int64_t col_stride, const uint8_t *At, int64_t ldat, const float *sAt, int64_t ldsat, int at_tiles,
+                                   const uint8_t *Bt, int64_t ldbt, const float *sBt, int64_t ldsbt, int bt_tiles, int dtype, void *dA,
+                                   int64_t ldda, void *dB, int64_t lddb, void *work, int64_t work_bytes) {
+  GradLayout y;
+  if (int rc = grad_layout(m, n, k, dtype, y)) return rc;
+  if (work_bytes < y.bytes || (y.bytes && (!work || (uintptr_t)work % 256)))
+    return fail(NMFK_ERR_BAD_ARG, "nmfk_product_grads: the workspace is too small or not 256-byte aligned (nmfk_product_grads_workspace)");
+  char *w = (char *)work;
+  uint8_t *q = (uint8_t *)(w + y.q), *t = (uint8_t *)(w + y.t);
+  float *qs = (float *)(w + y.qs), *ts = (float *)(w + y.ts);
+  if (m && n)
+    if (int rc = nmfk_quantize(device, stream, dy_dtype, dY, m, n, row_stride, col_stride, 0, q, y.ldq, qs, m, t, y.ldt, ts, n)) return rc;
+  if (int rc = nmfk_product(device, stream, m, k, n, q, y.ldq, qs, m, 0, Bt, ldbt, sBt, ldsbt, bt_tiles, dtype, dA, ldda, w + y.work, y.bytes - y.work)) return rc;
+  return nmfk_product(device, stream, n, k, m, t, y.ldt, ts, n, 0, At, ldat, sAt, ldsat, at_tiles, dtype, dB, lddb, w + y.work, y.bytes - y.work);
+}

@@ -62,6 +62,13 @@ def _product_workspace(m, n, k, t):
 
 
 @functools.lru_cache(4096)
+def _grads_workspace(m, n, k, t):
+    nb = C.c_int64()
+    _check(_lib.lib().nmfk_product_grads_workspace(m, n, k, t, C.byref(nb)))
+    return nb.value
+
+
+@functools.lru_cache(4096)
 def _orthogonalize_workspace(b, r, c):
     nb = C.c_int64()
     _check(_lib.lib().nmfk_orthogonalize_workspace(b, r, c, C.byref(nb)))
@@ -135,6 +142,15 @@ class Quantized:
         return (self.values.float() * s).to(dtype or _F32)
 
 
+def _contiguous_side(X):
+    """X and its strides: as it is if its rows or its columns are contiguous, else a copy"""
+    (r, c), (sr, sc) = X.shape, X.stride()
+    if not (sc == 1 and (sr >= c or r == 1)) and not (sr == 1 and (sc >= r or c == 1)):
+        X = X.contiguous()
+        sr, sc = X.stride()
+    return X, sr, sc
+
+
 def quantize(X, tiles=False, both=False):
     """X (a matrix of float32, bfloat16 or float16) in 8 bits with a scale for each block of 128 entries of a row, or (tiles) for each
     128 x 128 tile.  scale = max(max |x| / 448, 2^-126) over the block's finite entries, value = x / scale rounded to e4m3, ties to even; an
@@ -142,10 +158,7 @@ def quantize(X, tiles=False, both=False):
     both=True: a pair, X and its transpose (blocks along ITS rows), from one pass over X."""
     _tensor(X, "X")
     r, c = X.shape
-    sr, sc = X.stride()
-    if not (sc == 1 and (sr >= c or r == 1)) and not (sr == 1 and (sc >= r or c == 1)):
-        X = X.contiguous()
-        sr, sc = X.stride()
+    X, sr, sc = _contiguous_side(X)
     dev, tiles = X.device, bool(tiles)
     q = Quantized.__new__(Quantized)._make(r, c, tiles, dev)
     if not both:
@@ -192,6 +205,7 @@ def product_grads(dY, At, Bt, dtype=None):
     """The backward pass of Y = product(A, B): (dA, dB) = (dY * B, dY' * A), both products in 8 bits.  dY and its transpose are quantized by
     rows; At and Bt are the Quantized transposes of A and of B (quantize(..., both=True) leaves them beside the forward's).  The gradients are
     those with respect to the matrices that the 8 bits stand for."""
+    torch = _torch()
     _tensor(dY, "dY")
     _quantized(At, "At")
     _quantized(Bt, "Bt")
@@ -199,8 +213,15 @@ def product_grads(dY, At, Bt, dtype=None):
     if At.shape[1] != m or Bt.shape[1] != n or At.shape[0] != Bt.shape[0] or At.device != dY.device or Bt.device != dY.device:
         raise _bad(f"dY {m} x {n} needs At k x {m} and Bt k x {n} on its GPU, not {At.shape} on {At.device} and {Bt.shape} on {Bt.device}")
     dtype = dtype or dY.dtype
-    q, t = quantize(dY, both=True)
-    return product(q, Bt, dtype), product(t, At, dtype)
+    if dtype not in _TYPES:
+        raise _bad(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+    dY, sr, sc = _contiguous_side(dY)
+    k, dev, t = At.shape[0], dY.device, _TYPES[dtype]
+    nb = _grads_workspace(m, n, k, t)
+    dA, dB, work = torch.empty((m, k), dtype=dtype, device=dev), torch.empty((n, k), dtype=dtype, device=dev), torch.empty(nb, dtype=_U8, device=dev)
+    _check(_lib.lib().nmfk_product_grads(dev.index, _stream(dev), m, n, k, _TYPES[dY.dtype], dY.data_ptr(), sr, sc, At._pv, At._ldv, At._ps, At._lds, At.tiles,
+                                         Bt._pv, Bt._ldv, Bt._ps, Bt._lds, Bt.tiles, t, dA.data_ptr(), k, dB.data_ptr(), k, work.data_ptr(), nb))
+    return dA, dB
 
 
 def _extent(x):

@@ -244,6 +244,24 @@ def test_product_grads(P, m, n, k, t):
     check_product(db, values64(w), values64(at), TYPES[t])
 
 
+def test_product_grads_strides_sizes_and_refusals(P):
+    (a8, at), (b8, bt) = P.quantize(randn(1, 60, 90), both=True), P.quantize(randn(2, 40, 90), tiles=True, both=True)
+    dy = randn(3, 60, 40)
+    want = P.product_grads(dy, at, bt)
+    for v in (dy.t().contiguous().t(), torch.cat([dy, dy], 1)[:, :40], torch.stack([dy, dy], 2)[:, :, 1]):
+        assert all(torch.equal(x, y) for x, y in zip(P.product_grads(v, at, bt), want))
+    half = P.product_grads(dy, at, bt, dtype=torch.float16)
+    assert half[0].dtype == torch.float16 and torch.allclose(half[0].float(), want[0], rtol=2.0 ** -8, atol=2.0 ** -8 * float(want[0].abs().max()))
+    e, f = P.product_grads(torch.empty(0, 40, device="cuda"), P.quantize(torch.empty(90, 0, device="cuda")), bt)  # no rows: dB is a sum over nothing
+    assert e.shape == (0, 90) and f.shape == (40, 90) and bool((f == 0).all())
+    e, f = P.product_grads(torch.empty(60, 0, device="cuda"), at, P.quantize(torch.empty(90, 0, device="cuda")))
+    assert e.shape == (60, 90) and bool((e == 0).all()) and f.shape == (0, 90)
+    for bad in (lambda: P.product_grads(dy.t(), at, bt), lambda: P.product_grads(dy, bt, at), lambda: P.product_grads(dy, a8, b8), lambda: P.product_grads(dy, at, bt, dtype=torch.float64),
+                lambda: P.product_grads(dy, at, b8), lambda: P.product_grads(dy[0], at, bt)):
+        with pytest.raises(P.NMFkError):
+            bad()
+
+
 def test_product_grads_against_differences(P):
     """The loss sum(dY * product(A, B)) moves with an entry of A as dA says.  A is perturbed where 8 bits can show it: its values times 1 +- 1/2 stay
     values of e4m3 (a power of two and its neighbours), so that central differences of the linear loss are exact up to fp32 sums."""

@@ -72,6 +72,25 @@ def test_product_of_nothing_sizes_and_workspace(NMFk):
         assert "workspace" in _last(L)
 
 
+GRADS = dict(device=0, stream=None, m=10, n=20, k=200, dt=0, dY=PTR, rs=20, cs=1, At=PTR, ldat=128, sAt=PTR, ldsat=200, att=0, Bt=PTR, ldbt=128, sBt=PTR, ldsbt=200,
+             btt=0, dtype=0, dA=PTR, ldda=200, dB=PTR, lddb=200, work=PTR, wb=1 << 40)
+
+
+@pytest.mark.parametrize("bad", [dict(m=-1), dict(n=-1), dict(k=-1), dict(dtype=7), dict(dt=7), dict(dY=None), dict(rs=3), dict(work=None), dict(wb=100), dict(work=PTR + 64)], ids=str)
+def test_product_grads_refuses(NMFk, bad):
+    L = NMFk.lib()
+    assert L.nmfk_product_grads(*{**GRADS, **bad}.values()) == 1, bad
+    assert "nmfk_" in _last(L)
+
+
+def test_product_grads_of_nothing(NMFk):
+    L = NMFk.lib()
+    nb = C.c_int64()
+    assert L.nmfk_product_grads_workspace(0, 0, 5, 0, C.byref(nb)) == 0 and nb.value == 0
+    assert L.nmfk_product_grads_workspace(3, 4, 5, 0, None) == 1
+    assert L.nmfk_product_grads(*{**GRADS, "m": 0, "n": 0, "work": None, "wb": 0}.values()) == 0
+
+
 CF = (C.c_double * 15)(*([3.4445, -4.7750, 2.0315] * 5))
 ORTHO = dict(device=0, stream=None, dtype=0, batch=2, rows=100, cols=20, G=PTR, gb=2000, gr=20, gc=1, O=PTR, ob=2000, orow=20, oc=1, steps=5,
              cf=C.addressof(CF), work=PTR, wb=1 << 40)
