@@ -349,23 +349,24 @@ __global__ __launch_bounds__(512) void prod_rows_kernel(ProdArgs p) {
   }
 }
 
-// sums the splits in their order: the same bits on every run
+// Joins the parts of split sums: a wave adds every fourth part of 64 V results, then the four waves' sums are added in their order, so the bits are
+// the same on every run.  What bounds it is the latency of the reads, hence many small workgroups (2048 x 64 in 32 parts: 4.8 us;
+// 128 x 128 x 65536 with its join 13.3 us, with a whole sum a thread 14.9).
 template <typename T, int V>
 __global__ __launch_bounds__(256) void prod_join_kernel(const float *part, int splits, int64_t m, int64_t n, T *y, int64_t ldy) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, mn = m * n;
-  if (i >= mn) return;
-  float s[V] = {};
+  using vec = __attribute__((ext_vector_type(V))) float;
+  __shared__ vec sum[3][64];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t i = ((int64_t)blockIdx.x * 64 + lane) * V, mn = m * n;
+  vec s = 0.f;
+  if (i < mn) {
 #pragma unroll 8
-  for (int k = 0; k < splits; ++k) {
-    const float *q = part + k * mn + i;
-    if (V == 4) {
-      const f32x4 v = *(const f32x4 *)q;
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[e] += v[e];
-    } else {
-      s[0] += *q;
-    }
+    for (int k = w; k < splits; k += 4) s += *(const vec *)(part + k * mn + i);
   }
+  if (w) sum[w - 1][lane] = s;
+  __syncthreads();
+  if (w || i >= mn) return;
+  s = ((s + sum[0][lane]) + sum[1][lane]) + sum[2][lane];
   const int64_t r = i / n;
   T *z = y + r * ldy + (i - r * n);
 #pragma unroll
@@ -403,8 +404,9 @@ Plan prod_plan(int64_t m, int64_t n, int64_t kb, bool bytes) {
     if (q.bn == 128 && nmfk_div_up(m, 128) * nmfk_div_up(n, 128) < 256) q.bm = q.bn = 64;
     const int64_t tiles = nmfk_div_up(m, q.bm) * nmfk_div_up(n, q.bn);
     // Few tiles leave many of the 256 CUs without one: split the sum, as long as a workgroup keeps six blocks (about 5 microseconds; the join of
-    // the partial sums costs 4).
-    if (tiles < 192) splits = std::min<int64_t>(512 / tiles, kb / 6);
+    // the partial sums costs 3).  One workgroup for each CU, or two where both keep sixteen blocks: 1024 x 64 x 65536 in 32 parts 23 us, in 64
+    // parts 27; 4096 x 64 x 65536 in 16 parts 62, in 8 parts 67.
+    if (tiles < 192) splits = std::min<int64_t>(kb / 6, std::max<int64_t>(nmfk_div_up(256, tiles), std::min<int64_t>(512 / tiles, kb / 16)));
   }
   q.kb_split = (int)nmfk_div_up(kb, std::max<int64_t>(1, splits));
   q.splits = (int)std::max<int64_t>(1, nmfk_div_up(kb, q.kb_split));
@@ -473,9 +475,9 @@ int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
     p.y = work;
     prod_launch<F, float, true>(p, q, st);
     if (p.n % 4 == 0)
-      prod_join_kernel<T, 4><<<dim3((unsigned)nmfk_div_up(mn, 1024)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
+      prod_join_kernel<T, 4><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
     else
-      prod_join_kernel<T, 1><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
+      prod_join_kernel<T, 1><<<dim3((unsigned)nmfk_div_up(mn, 64)), 256, 0, st>>>((const float *)work, q.splits, p.m, p.n, y, p.ldy);
   } else {
     prod_launch<F, T, false>(p, q, st);
   }
