@@ -88,18 +88,17 @@ enum { ROWS_ROWS = 0, B_TILES = 1, A_TILES = 2 };
 // any memory, take 413, the additions about 35 of these; the copies add 100.  The same in 32 x 32 x 64 instructions: 7 % slower.
 // The first operand of the matrix instruction is B, so that a lane's four outputs are neighbours in a row of Y.
 template <int BM, int BN, int WM, int WN, int MODE, typename F, typename T, bool SPLIT>
-__global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
+__device__ __forceinline__ void prod_tile(const ProdArgs &p, int id, int split) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int STAGE = (BM + BN) * 128, SC = (BM + BN) * 4;
   static_assert(TM >= 4 && TN >= 2 && BM / WM <= 128 && BN / WN <= 128, "B is copied between row 1 and row TM - 2, the scales behind the last use of the old ones");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int wm = w / WN, wn = w % WN;
-  const int id = xcd_order(blockIdx.x, gridDim.x);
   int tm, tn;
   tile_at(id, p.tiles_m, p.tiles_n, BM == 256 ? 4 : 8, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  const int kb0 = blockIdx.y * p.kb_split, kb1 = min(p.kb, kb0 + p.kb_split);
+  const int kb0 = split * p.kb_split, kb1 = min(p.kb, kb0 + p.kb_split);
 
   // this wave's share of the copies; rows behind the last one repeat it (their outputs are not stored).  A lane's offset from its tile's
   // first row fits 32 bits: 256 rows of at most 2^23 bytes.
@@ -270,11 +269,32 @@ __global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
       const int n = n0 + wn * (BN / WN) + j * 16 + fg * 4;
       if (n >= p.n) continue;
       if (SPLIT)
-        store4<float>((float *)p.y + ((int64_t)blockIdx.y * p.m + m) * p.n + n, acc[i][j], p.n - n);
+        store4<float>((float *)p.y + ((int64_t)split * p.m + m) * p.n + n, acc[i][j], p.n - n);
       else
         store4<T>((T *)p.y + m * p.ldy + n, acc[i][j], p.n - n);
     }
   }
+}
+
+template <int BM, int BN, int WM, int WN, int MODE, typename F, typename T, bool SPLIT>
+__global__ __launch_bounds__(64 * WM * WN) void prod_tile_kernel(ProdArgs p) {
+  prod_tile<BM, BN, WM, WN, MODE, F, T, SPLIT>(p, xcd_order(blockIdx.x, gridDim.x), blockIdx.y);
+}
+
+// Two products that do not wait for each other in one launch, the one with the longer sums first: the second fills the CUs that the first one leaves idle
+// at its end.  The first operands have a scale for each row.
+struct ProdPair {
+  ProdArgs p[2];
+};
+template <int BM, int BN, int WM, int WN, typename F, typename T>
+__global__ __launch_bounds__(64 * WM * WN) void prod_pair_kernel(ProdPair a) {
+  const int first = a.p[0].tiles_m * a.p[0].tiles_n, which = (int)blockIdx.x >= first;
+  const ProdArgs &p = a.p[which];
+  const int id = which ? xcd_order(blockIdx.x - first, gridDim.x - first) : xcd_order(blockIdx.x, first);
+  if (p.bshift)
+    prod_tile<BM, BN, WM, WN, B_TILES, F, T, false>(p, id, 0);
+  else
+    prod_tile<BM, BN, WM, WN, ROWS_ROWS, F, T, false>(p, id, 0);
 }
 
 // Few rows of A (m <= 16 TA): what bounds it is the one read of B.  A workgroup owns 16 TB columns of Y; its eight waves take the blocks of the sum in
@@ -422,7 +442,7 @@ void prod_tile_mode(const ProdArgs &p, int splits, hipStream_t st) {
 }
 
 template <int BM, int BN, int WM, int WN, typename F, typename T, bool SPLIT>
-void prod_tile(const ProdArgs &p, int splits, hipStream_t st) {
+void prod_tile_side(const ProdArgs &p, int splits, hipStream_t st) {
   if (p.bshift)
     prod_tile_mode<BM, BN, WM, WN, B_TILES, F, T, SPLIT>(p, splits, st);
   else if (p.ashift)
@@ -449,15 +469,15 @@ void prod_launch(const ProdArgs &p, const Plan &q, hipStream_t st) {
   }
   if constexpr (std::is_same<F, Bytes>::value && !SPLIT)
     if (q.bn == 256) {
-      prod_tile<256, 256, 2, 4, F, T, false>(p, 1, st);
+      prod_tile_side<256, 256, 2, 4, F, T, false>(p, 1, st);
       return;
     }
   if (q.bm == 64)
-    prod_tile<64, 64, 1, 2, F, T, SPLIT>(p, q.splits, st);
+    prod_tile_side<64, 64, 1, 2, F, T, SPLIT>(p, q.splits, st);
   else if (q.bn == 64)
-    prod_tile<128, 64, 2, 2, F, T, SPLIT>(p, q.splits, st);
+    prod_tile_side<128, 64, 2, 2, F, T, SPLIT>(p, q.splits, st);
   else
-    prod_tile<128, 128, 2, 2, F, T, SPLIT>(p, q.splits, st);
+    prod_tile_side<128, 128, 2, 2, F, T, SPLIT>(p, q.splits, st);
 }
 
 template <typename F, typename T>
@@ -484,11 +504,63 @@ int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
   return nmfk_launched("nmfk_product");
 }
 
+template <int BM, int BN, int WM, int WN, typename F, typename T>
+int prod_pair_side(ProdPair a, hipStream_t st) {
+  constexpr int BYTES = 2 * (BM + BN) * 132;
+  static std::atomic<uint64_t> done{0};
+  nmfk_allow_dynamic_lds((const void *)prod_pair_kernel<BM, BN, WM, WN, F, T>, done, BYTES);
+  unsigned tiles = 0;
+  for (ProdArgs &p : a.p) {
+    p.tiles_m = (int)nmfk_div_up(p.m, BM);
+    p.tiles_n = (int)nmfk_div_up(p.n, BN);
+    p.kb_split = p.kb;
+    tiles += (unsigned)(p.tiles_m * p.tiles_n);
+  }
+  prod_pair_kernel<BM, BN, WM, WN, F, T><<<dim3(tiles), 64 * WM * WN, BYTES, st>>>(a);
+  return nmfk_launched("nmfk_product_grads");
+}
+
+template <typename F, typename T>
+int prod_pair(const ProdPair &a, int side, hipStream_t st) {
+  if constexpr (std::is_same<F, Bytes>::value)
+    if (side == 256) return prod_pair_side<256, 256, 2, 4, F, T>(a, st);
+  if (side == 128) return prod_pair_side<128, 128, 2, 2, F, T>(a, st);
+  return prod_pair_side<64, 64, 1, 2, F, T>(a, st);
+}
+
+// The side of the tiles with which two products go in one launch, by prod_plan's rule for both together; 0: one behind the other, because one of them
+// is better off with another kernel or a split sum
+int pair_side(int64_t m0, int64_t n0, int64_t kb0, int64_t m1, int64_t n1, int64_t kb1, bool bytes) {
+  for (const Plan &q : {prod_plan(m0, n0, kb0, bytes), prod_plan(m1, n1, kb1, bytes)})
+    if (q.splits > 1 || q.bm != q.bn || q.bm < 64) return 0;
+  auto tiles = [&](int64_t side) { return nmfk_div_up(m0, side) * nmfk_div_up(n0, side) + nmfk_div_up(m1, side) * nmfk_div_up(n1, side); };
+  return bytes && tiles(256) >= 200 ? 256 : tiles(128) >= 256 ? 128 : 64;
+}
+
 int prod_sizes(int64_t m, int64_t n, int64_t k, const char *who) {
   if (m < 0 || n < 0 || k < 0) return fail(NMFK_ERR_BAD_ARG, std::string(who) + ": negative size");
   if (m > ((int64_t)1 << 22) || n > ((int64_t)1 << 22) || k > ((int64_t)1 << 22))
     return fail(NMFK_ERR_UNSUPPORTED, std::string(who) + ": a size above 2^22");
   if (nmfk_div_up(m, 128) * nmfk_div_up(n, 64) > 0x7fffffff / 2) return fail(NMFK_ERR_UNSUPPORTED, std::string(who) + ": too many outputs");
+  return NMFK_OK;
+}
+
+// the arguments of a product, checked; m = 0 or n = 0 is nothing to do
+int prod_args(int64_t m, int64_t n, int64_t k, const uint8_t *A, int64_t lda, const float *sA, int64_t ldsa, int a_tiles, const uint8_t *B, int64_t ldb,
+              const float *sB, int64_t ldsb, int b_tiles, int dtype, void *Y, int64_t ldy, ProdArgs &p) {
+  if (int rc = prod_sizes(m, n, k, "nmfk_product")) return rc;
+  if (dtype < NMFK_F32 || dtype > NMFK_F16) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: dtype must be NMFK_F32, NMFK_BF16 or NMFK_F16");
+  if (m == 0 || n == 0) return NMFK_OK;
+  const int64_t kb = nmfk_div_up(k, 128);
+  if (!Y || ldy < n) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: Y is needed, with ldy >= n");
+  if (kb > 0) {
+    if (!A || !B || !sA || !sB) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: null pointer");
+    if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)lda | (uintptr_t)ldb) & 15 || lda < kb * 128 || ldb < kb * 128 || lda > ((int64_t)1 << 23) || ldb > ((int64_t)1 << 23))
+      return fail(NMFK_ERR_BAD_ARG, "nmfk_product: rows must be 16-byte aligned, hold whole blocks of 128 and be at most 2^23 bytes apart");
+    if (ldsa < (a_tiles ? nmfk_div_up(m, 128) : m) || ldsb < (b_tiles ? nmfk_div_up(n, 128) : n))
+      return fail(NMFK_ERR_BAD_ARG, "nmfk_product: the leading dimension of the scales is too small");
+  }
+  p = {(const char *)A, (const char *)B, lda, ldb, sA, sB, ldsa, ldsb, a_tiles ? 7 : 0, b_tiles ? 7 : 0, Y, ldy, (int)m, (int)n, (int)kb, 0, 0, 0};
   return NMFK_OK;
 }
 
@@ -508,24 +580,15 @@ NMFK_EXPORT int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int dtyp
 NMFK_EXPORT int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, const uint8_t *A, int64_t lda, const float *sA,
                              int64_t ldsa, int a_tiles, const uint8_t *B, int64_t ldb, const float *sB, int64_t ldsb, int b_tiles, int dtype,
                              void *Y, int64_t ldy, void *work, int64_t work_bytes) {
-  if (int rc = prod_sizes(m, n, k, "nmfk_product")) return rc;
-  if (dtype < NMFK_F32 || dtype > NMFK_F16) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: dtype must be NMFK_F32, NMFK_BF16 or NMFK_F16");
+  ProdArgs p;
+  if (int rc = prod_args(m, n, k, A, lda, sA, ldsa, a_tiles, B, ldb, sB, ldsb, b_tiles, dtype, Y, ldy, p)) return rc;
   if (m == 0 || n == 0) return NMFK_OK;
-  const int64_t kb = nmfk_div_up(k, 128);
-  if (!Y || ldy < n) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: Y is needed, with ldy >= n");
-  if (kb > 0) {
-    if (!A || !B || !sA || !sB) return fail(NMFK_ERR_BAD_ARG, "nmfk_product: null pointer");
-    if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)lda | (uintptr_t)ldb) & 15 || lda < kb * 128 || ldb < kb * 128 || lda > ((int64_t)1 << 23) || ldb > ((int64_t)1 << 23))
-      return fail(NMFK_ERR_BAD_ARG, "nmfk_product: rows must be 16-byte aligned, hold whole blocks of 128 and be at most 2^23 bytes apart");
-    if (ldsa < (a_tiles ? nmfk_div_up(m, 128) : m) || ldsb < (b_tiles ? nmfk_div_up(n, 128) : n))
-      return fail(NMFK_ERR_BAD_ARG, "nmfk_product: the leading dimension of the scales is too small");
-  }
+  const int64_t kb = p.kb;
   const Plan q = prod_plan(m, n, std::max<int64_t>(1, kb), dtype != NMFK_F32);
   if (kb > 0 && q.splits > 1 && (!work || work_bytes < (int64_t)q.splits * m * n * 4 || (uintptr_t)work % 16))
     return fail(NMFK_ERR_BAD_ARG, "nmfk_product: the workspace is too small or not 16-byte aligned (nmfk_product_workspace)");
   NmfkDeviceGuard guard(device);
   if (guard.status) return guard.status;
-  ProdArgs p = {(const char *)A, (const char *)B, lda, ldb, sA, sB, ldsa, ldsb, a_tiles ? 7 : 0, b_tiles ? 7 : 0, Y, ldy, (int)m, (int)n, (int)kb, 0, 0, 0};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == NMFK_F32) return prod_run<Halves, float>(p, q, work, st);
   if (dtype == NMFK_BF16) return prod_run<Bytes, bf16>(p, q, work, st);
@@ -583,8 +646,21 @@ NMFK_EXPORT int nmfk_product_grads(int device, void *stream, int64_t m, int64_t 
   char *w = (char *)work;
   uint8_t *q = (uint8_t *)(w + y.q), *t = (uint8_t *)(w + y.t);
   float *qs = (float *)(w + y.qs), *ts = (float *)(w + y.ts);
+  ProdPair pair;
+  if (int rc = prod_args(m, k, n, q, y.ldq, qs, m, 0, Bt, ldbt, sBt, ldsbt, bt_tiles, dtype, dA, ldda, pair.p[0])) return rc;
+  if (int rc = prod_args(n, k, m, t, y.ldt, ts, n, 0, At, ldat, sAt, ldsat, at_tiles, dtype, dB, lddb, pair.p[1])) return rc;
   if (m && n)
     if (int rc = nmfk_quantize(device, stream, dy_dtype, dY, m, n, row_stride, col_stride, 0, q, y.ldq, qs, m, t, y.ldt, ts, n)) return rc;
+  const int side = m && n && k ? pair_side(m, k, nmfk_div_up(n, 128), n, k, nmfk_div_up(m, 128), dtype != NMFK_F32) : 0;
+  if (side) {
+    NmfkDeviceGuard guard(device);
+    if (guard.status) return guard.status;
+    if (m > n) std::swap(pair.p[0], pair.p[1]);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == NMFK_F32) return prod_pair<Halves, float>(pair, side, st);
+    if (dtype == NMFK_BF16) return prod_pair<Bytes, bf16>(pair, side, st);
+    return prod_pair<Bytes, _Float16>(pair, side, st);
+  }
   if (int rc = nmfk_product(device, stream, m, k, n, q, y.ldq, qs, m, 0, Bt, ldbt, sBt, ldsbt, bt_tiles, dtype, dA, ldda, w + y.work, y.bytes - y.work)) return rc;
   return nmfk_product(device, stream, n, k, m, t, y.ldt, ts, n, 0, At, ldat, sAt, ldsat, at_tiles, dtype, dB, lddb, w + y.work, y.bytes - y.work);
 }
