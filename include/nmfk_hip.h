@@ -288,7 +288,7 @@ int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, cons
 
 /* The backward pass of Y = A * B' in one call: dY (m x n, entry (i, j) at dY[i * row_stride + j * col_stride], one of the strides 1) and its
  * transpose are quantized by rows, then dA (m x k) = dY8 * (B'8)' and dB (n x k) = dY'8 * (A'8)'.  At (k x m) and Bt (k x n) are the
- * transposes of A and B as nmfk_quantize leaves them (tvalues, tscales).  The two products run one behind the other. */
+ * transposes of A and B as nmfk_quantize leaves them (tvalues, tscales).  dA, dB and the other operands must not overlap. */
 int nmfk_product_grads_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes);
 int nmfk_product_grads(int device, void *stream, int64_t m, int64_t n, int64_t k, int dy_dtype, const void *dY, int64_t row_stride,
                        int64_t col_stride, const uint8_t *At, int64_t ldat, const float *sAt, int64_t ldsat, int at_tiles,

@@ -226,6 +226,72 @@ function robustkmeans(c::Context, X::Matrix{Float32}, k::Integer, repeats::Integ
 end
 
 # ---------------------------------------------------------------------------------------------------------------
+# matrix products beside the factorizations (no reference counterpart)
+# ---------------------------------------------------------------------------------------------------------------
+# Thin: device pointers (pointer(a) of an AMDGPU.jl array), sizes and strides as in include/nmfk_hip.h, work queued on `stream`.  Entry (i, j) of a
+# Julia matrix A stands at 1-based A[i, j] = memory[(i - 1) + (j - 1) * size(A, 1)]: row_stride = 1, col_stride = size(A, 1).
+const F32, BF16, F16 = Int32(0), Int32(1), Int32(2)
+
+"X (rows x cols) in e4m3 with a scale for 128 entries of a row, or (tiles) for 128 x 128; tvalues, tscales: the same of the transpose"
+function quantize!(values::Ptr{UInt8}, ldv::Integer, scales::Ptr{Float32}, lds::Integer, X::Ptr, rows::Integer, cols::Integer,
+		row_stride::Integer, col_stride::Integer; dtype::Int32=F32, tiles::Bool=false, tvalues::Ptr{UInt8}=Ptr{UInt8}(C_NULL),
+		ldtv::Integer=0, tscales::Ptr{Float32}=Ptr{Float32}(C_NULL), ldts::Integer=0, device::Integer=0, stream::Ptr{Cvoid}=C_NULL)
+	check(ccall((:nmfk_quantize, libnmfk), Cint,
+		(Cint, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Int64, Int64, Int64, Int64, Cint, Ptr{UInt8}, Int64, Ptr{Float32}, Int64, Ptr{UInt8}, Int64, Ptr{Float32}, Int64),
+		device, stream, dtype, X, rows, cols, row_stride, col_stride, tiles, values, ldv, scales, lds, tvalues, ldtv, tscales, ldts))
+end
+
+"bytes of the workspace of product!, product_grads! and orthogonalize!"
+function product_workspace(m::Integer, n::Integer, k::Integer; dtype::Int32=F32)
+	r = Ref{Int64}(0)
+	check(ccall((:nmfk_product_workspace, libnmfk), Cint, (Int64, Int64, Int64, Cint, Ref{Int64}), m, n, k, dtype, r))
+	return r[]
+end
+function product_grads_workspace(m::Integer, n::Integer, k::Integer; dtype::Int32=F32)
+	r = Ref{Int64}(0)
+	check(ccall((:nmfk_product_grads_workspace, libnmfk), Cint, (Int64, Int64, Int64, Cint, Ref{Int64}), m, n, k, dtype, r))
+	return r[]
+end
+function orthogonalize_workspace(batch::Integer, rows::Integer, cols::Integer)
+	r = Ref{Int64}(0)
+	check(ccall((:nmfk_orthogonalize_workspace, libnmfk), Cint, (Int64, Int64, Int64, Ref{Int64}), batch, rows, cols, r))
+	return r[]
+end
+
+"Y = A * B' (m x n by rows) of two quantized matrices, m x k and n x k"
+function product!(Y::Ptr, ldy::Integer, m::Integer, n::Integer, k::Integer, A::Ptr{UInt8}, lda::Integer, sA::Ptr{Float32}, ldsa::Integer,
+		B::Ptr{UInt8}, ldb::Integer, sB::Ptr{Float32}, ldsb::Integer, work::Ptr{Cvoid}, work_bytes::Integer; a_tiles::Bool=false,
+		b_tiles::Bool=false, dtype::Int32=F32, device::Integer=0, stream::Ptr{Cvoid}=C_NULL)
+	check(ccall((:nmfk_product, libnmfk), Cint,
+		(Cint, Ptr{Cvoid}, Int64, Int64, Int64, Ptr{UInt8}, Int64, Ptr{Float32}, Int64, Cint, Ptr{UInt8}, Int64, Ptr{Float32}, Int64, Cint,
+		 Cint, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64),
+		device, stream, m, n, k, A, lda, sA, ldsa, a_tiles, B, ldb, sB, ldsb, b_tiles, dtype, Y, ldy, work, work_bytes))
+end
+
+"dA = dY * B, dB = dY' * A from dY (m x n) and the quantized transposes At (k x m) and Bt (k x n)"
+function product_grads!(dA::Ptr, ldda::Integer, dB::Ptr, lddb::Integer, m::Integer, n::Integer, k::Integer, dY::Ptr, row_stride::Integer,
+		col_stride::Integer, At::Ptr{UInt8}, ldat::Integer, sAt::Ptr{Float32}, ldsat::Integer, Bt::Ptr{UInt8}, ldbt::Integer,
+		sBt::Ptr{Float32}, ldsbt::Integer, work::Ptr{Cvoid}, work_bytes::Integer; at_tiles::Bool=false, bt_tiles::Bool=false,
+		dy_dtype::Int32=F32, dtype::Int32=F32, device::Integer=0, stream::Ptr{Cvoid}=C_NULL)
+	check(ccall((:nmfk_product_grads, libnmfk), Cint,
+		(Cint, Ptr{Cvoid}, Int64, Int64, Int64, Cint, Ptr{Cvoid}, Int64, Int64, Ptr{UInt8}, Int64, Ptr{Float32}, Int64, Cint,
+		 Ptr{UInt8}, Int64, Ptr{Float32}, Int64, Cint, Cint, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64),
+		device, stream, m, n, k, dy_dtype, dY, row_stride, col_stride, At, ldat, sAt, ldsat, at_tiles, Bt, ldbt, sBt, ldsbt, bt_tiles,
+		dtype, dA, ldda, dB, lddb, work, work_bytes))
+end
+
+"The orthogonal factor of `batch` matrices by Newton-Schulz products; strides: (batch, row, col); coefficients: (a, b, c) for each step, 3 x steps"
+function orthogonalize!(O::Ptr, ostrides::NTuple{3,Integer}, G::Ptr, gstrides::NTuple{3,Integer}, batch::Integer, rows::Integer,
+		cols::Integer, coefficients::Matrix{Float64}, work::Ptr{Cvoid}, work_bytes::Integer; dtype::Int32=F32, device::Integer=0,
+		stream::Ptr{Cvoid}=C_NULL)
+	size(coefficients, 1) == 3 || throw(ArgumentError("coefficients must be 3 x steps"))
+	GC.@preserve coefficients check(ccall((:nmfk_orthogonalize, libnmfk), Cint,
+		(Cint, Ptr{Cvoid}, Cint, Int64, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Int64, Cint, Ptr{Float64}, Ptr{Cvoid}, Int64),
+		device, stream, dtype, batch, rows, cols, G, gstrides[1], gstrides[2], gstrides[3], O, ostrides[1], ostrides[2], ostrides[3],
+		size(coefficients, 2), coefficients, work, work_bytes))
+end
+
+# ---------------------------------------------------------------------------------------------------------------
 # host logic of the reference, unchanged in meaning
 # ---------------------------------------------------------------------------------------------------------------
 "getk (src/NMFkPostprocess.jl:7-41)"
