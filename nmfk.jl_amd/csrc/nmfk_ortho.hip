@@ -203,26 +203,46 @@ __device__ __forceinline__ f64x4 sym_product(f64x4 x, f64x4 y) {
   return d;
 }
 
-// 16 < s <= 64: the iteration by one workgroup per matrix, a wave per 16 x 16 tile, the matrices in LDS as registers of lanes
+// 16 < s <= 64: the chunks' partial S, added in their order and left in the place of the first
+__global__ __launch_bounds__(256) void small_join_kernel(SmallArgs a) {
+  const int ss = a.s * a.s, e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= ss) return;
+  double *part = a.part + (int64_t)blockIdx.y * a.chunks * ss + e, v = 0;
+#pragma unroll 16
+  for (int k = 0; k < a.chunks; ++k) v += part[(int64_t)k * ss];
+  *part = v;
+}
+
+// 16 < s <= 64: the iteration by one workgroup per matrix, a wave per 16 x 16 tile, the matrices in LDS as registers of lanes.  What bounds it above
+// s = 32 is the fp64 matrix instruction (64 cycles) on one CU, so there only the tiles on and below the diagonal are computed and
+// written to both places; below, the way through LDS.
+constexpr bool small_half(int tt) { return tt > 2; }
+constexpr int small_waves(int tt) { return small_half(tt) ? tt * (tt + 1) / 2 : tt * tt; }
+constexpr int SUMS = 4;  // partial S that the iteration adds itself; more of them are joined before
 template <int TT>
-__global__ __launch_bounds__(64 * TT * TT) void small_iterate_kernel(SmallArgs a, Coefs cf) {
+__global__ __launch_bounds__(64 * small_waves(TT)) void small_iterate_kernel(SmallArgs a, Coefs cf, int parts) {
   extern __shared__ double mats[];
   constexpr int N = TT * TT * 256;
-  const int s = a.s, w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, ti = w / TT, tj = w % TT;
+  const int s = a.s, w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  constexpr bool HALF = small_half(TT);
+  const int ti = !HALF ? w / TT : w < 1 ? 0 : w < 3 ? 1 : w < 6 ? 2 : 3, tj = HALF ? w - ti * (ti + 1) / 2 : w % TT;
   double *S = mats, *P = S + N, *Q = P + N, *U = Q + N;
   const double *part = a.part + (int64_t)blockIdx.x * a.chunks * s * s;
   const int x = 16 * tj + c;
   f64x4 v = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int k = 0; k < a.chunks; ++k)
+#pragma unroll
+  for (int k = 0; k < SUMS; ++k)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int y = 16 * ti + 4 * r + g;
-      if (y < s && x < s) v[r] += part[(int64_t)k * s * s + y * s + x];
+      if (k < parts && y < s && x < s) v[r] += part[(int64_t)k * s * s + y * s + x];
     }
   auto put = [&](double *m, f64x4 d) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) m[(w * 4 + r) * 64 + lane] = d[r];
+    for (int r = 0; r < 4; ++r) m[((ti * TT + tj) * 4 + r) * 64 + lane] = d[r];
+    if (!HALF || ti == tj) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m[((tj * TT + ti) * 4 + (c >> 2)) * 64 + 16 * (c & 3) + 4 * r + g] = d[r];
   };
   auto product = [&](const double *m, const double *n) {  // of this wave's tile
     f64x4 d = {0, 0, 0, 0};
@@ -236,9 +256,11 @@ __global__ __launch_bounds__(64 * TT * TT) void small_iterate_kernel(SmallArgs a
   put(S, v);
   __syncthreads();
   double norm2 = 0;
-  for (int i = 0; i < s; ++i) {  // [i][i]: tile (i / 16, i / 16), register (i % 16) / 4, lane 16 (i % 4) + i % 16
-    const int k = i >> 4, e = i & 15;
-    norm2 += S[((k * TT + k) * 4 + (e >> 2)) * 64 + 16 * (e & 3) + e];
+  {  // [i][i]: tile (i / 16, i / 16), register (i % 16) / 4, lane 16 (i % 4) + i % 16; zero behind s
+    const int k = lane >> 4, e = lane & 15;
+    if (k < TT) norm2 = S[((k * TT + k) * 4 + (e >> 2)) * 64 + 16 * (e & 3) + e];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) norm2 += __shfl_xor(norm2, o);
   }
   double inv2, inv;
   small_norm(norm2, inv2, inv);
@@ -266,22 +288,44 @@ __global__ __launch_bounds__(64 * TT * TT) void small_iterate_kernel(SmallArgs a
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int y = 16 * ti + 4 * r + g;
-    if (y < s && x < s) a.q[(int64_t)blockIdx.x * s * s + y * s + x] = (float)(q[r] * inv);
+    if (y >= s || x >= s) continue;
+    float *out = a.q + (int64_t)blockIdx.x * s * s;
+    out[y * s + x] = (float)(q[r] * inv);
+    if (HALF && ti != tj) out[x * s + y] = (float)(q[r] * inv);
   }
 }
 
 // O = Q X over a chunk of l, on the fp32 matrix pipe (16 x 16 x 4: entry [c][.] of the first, [.][c] of the second operand in lane 16 g + c, result
-// [4 g + r][c] in register r).  Which four of the sum's entries a step takes is free: a lane's four consecutive entries of X serve four steps,
-// or four columns, and its four results stand next to each other in O.  s <= 16: every workgroup iterates for itself, in registers (about
-// 2 microseconds, less than a launch); the waves share the sum over the chunks.
+// [4 g + r][c] in register r).  Which four of the sum's entries a step takes is free: a lane's four consecutive entries of X or of Q serve four steps,
+// or four columns, and its four results stand next to each other in O.  s <= 16: every workgroup iterates for itself, a wave in registers (about
+// 2 microseconds, less than a launch), while the first entries of X are on their way.
 template <typename T, int TT, bool WIDE>
 __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf) {
-  __shared__ double sum[4][256];
+  __shared__ double sum[256];
   __shared__ float qs[16][17];
   const int by = gridDim.y - 1 - blockIdx.y;  // the matrices read last are still in the last-level cache: take them first
   const int64_t b = a.b0 + by;
   const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
-  const int s = a.s, t = threadIdx.x, w = t >> 6, lane = t & 63, c = lane & 15, g = lane >> 4;
+  const int s = a.s, t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 15, g = lane >> 4;
+  const T *p = (const T *)a.g.p + b * a.g.batch;
+  T *o = (T *)a.o.p + b * a.o.batch;
+  constexpr int U = WIDE ? 4 : TT == 1 ? 4 : TT == 2 ? 2 : 1, SPAN = 16 * U;  // columns a wave takes at a time
+  float x[WIDE ? TT : U][WIDE ? 4 : TT][4];
+  auto load = [&](int64_t base) {
+    if (WIDE) {
+#pragma unroll
+      for (int k = 0; k < TT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) small_load4<T, true>(a.g, p, s, l1, a.gvec, 16 * k + 4 * g + r, base + 4 * c, x[k][r]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < TT; ++k) small_load4<T, false>(a.g, p, s, l1, a.gvec, 16 * k + 4 * g, base + 16 * u + c, x[u][k]);
+    }
+  };
+  const int64_t base0 = l0 + (int64_t)w * SPAN;
+  if (TT == 1) load(base0);  // on its way during the iteration
   float q[TT][TT][4];
   if (TT == 1) {
     const double *part = a.part + (int64_t)by * a.chunks * s * s;
@@ -290,57 +334,60 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
     if (y < s && x < s) {
       const double *e = part + y * s + x;
       int k = 0;
+      for (; k + 16 <= a.chunks; k += 16) {  // sixteen loads in flight
+        double u[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) u[r] = e[(int64_t)(k + r) * s * s];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r & 3] += u[r];
+      }
       for (; k + 4 <= a.chunks; k += 4)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] += e[(int64_t)(k + r) * s * s];
       for (; k < a.chunks; ++k) v[0] += e[(int64_t)k * s * s];
     }
-    sum[0][t] = (v[0] + v[1]) + (v[2] + v[3]);
+    sum[t] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
-    f64x4 S, P, Q = {0, 0, 0, 0};
-    double norm2 = 0, inv2, inv;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) S[r] = sum[0][(4 * r + g) * 16 + c];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) norm2 += sum[0][i * 17];
-    small_norm(norm2, inv2, inv);
-    S *= inv2;
-    for (int k = 0; k < a.steps; ++k) {
-      P = cf.v[3 * k + 1] * S + cf.v[3 * k + 2] * sym_product(S, S);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (4 * r + g == c) P[r] += cf.v[3 * k];
-      if (k + 1 < a.steps) S = sym_product(sym_product(S, P), P);
-      Q = k == 0 ? P : sym_product(Q, P);
-    }
     if (w == 0) {
+      f64x4 S, P, Q = {0, 0, 0, 0};
+      double norm2 = 0, inv2, inv;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[r] = sum[(4 * r + g) * 16 + c];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) norm2 += sum[i * 17];
+      small_norm(norm2, inv2, inv);
+      S *= inv2;
+      for (int k = 0; k < a.steps; ++k) {
+        P = cf.v[3 * k + 1] * S + cf.v[3 * k + 2] * sym_product(S, S);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (4 * r + g == c) P[r] += cf.v[3 * k];
+        if (k + 1 < a.steps) S = sym_product(sym_product(S, P), P);
+        Q = k == 0 ? P : sym_product(Q, P);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) qs[4 * r + g][c] = (float)(Q[r] * inv);
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) q[0][0][k] = qs[c][WIDE ? 4 * k + g : 4 * g + k];
+    for (int k = 0; k < 4; ++k) q[0][0][k] = qs[c][4 * g + k];
   } else {
     const float *m = a.q + (int64_t)by * s * s;
 #pragma unroll
     for (int i = 0; i < TT; ++i)
 #pragma unroll
-      for (int j = 0; j < TT; ++j)
+      for (int j = 0; j < TT; ++j) {
+        const int y = 16 * i + c, x = 16 * j + 4 * g;
+        if (y < s && x + 4 <= s)
+          read4(m + y * s + x, q[i][j]);
+        else
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int y = 16 * i + c, x = 16 * j + (WIDE ? 4 * k + g : 4 * g + k);
-          q[i][j][k] = y < s && x < s ? m[y * s + x] : 0.f;
-        }
+          for (int k = 0; k < 4; ++k) q[i][j][k] = y < s && x + k < s ? m[y * s + x + k] : 0.f;
+      }
   }
-  const T *p = (const T *)a.g.p + b * a.g.batch;
-  T *o = (T *)a.o.p + b * a.o.batch;
-  if (WIDE) {
-    for (int64_t base = l0 + (int64_t)w * 64; base < l1; base += 256) {
-      float x[TT][4][4];
-#pragma unroll
-      for (int k = 0; k < TT; ++k)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) small_load4<T, true>(a.g, p, s, l1, a.gvec, 16 * k + 4 * r + g, base + 4 * c, x[k][r]);
+  for (int64_t base = base0; base < l1; base += 4 * SPAN) {
+    if (TT > 1) load(base);
+    if (WIDE) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
         f32x4 d[4];
@@ -352,6 +399,7 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[i][k][r], x[k][r][e], d[e], 0, 0, 0);
+        if (TT == 1) load(base + 4 * SPAN);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int row = 16 * i + 4 * g + r;
@@ -367,38 +415,34 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
           }
         }
       }
-    }
-  } else {
-    constexpr int U = TT == 1 ? 4 : TT == 2 ? 2 : 1;
-    for (int64_t base = l0 + (int64_t)w * 16 * U; base < l1; base += 64 * U) {
-      float x[U][TT][4];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < TT; ++k) small_load4<T, false>(a.g, p, s, l1, a.gvec, 16 * k + 4 * g, base + 16 * u + c, x[u][k]);
+    } else {
+      f32x4 d[U][TT];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t j = base + 16 * u + c;
-        f32x4 d[TT];
 #pragma unroll
-        for (int i = 0; i < TT; ++i) d[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < TT; ++i) d[u][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < TT; ++k)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int i = 0; i < TT; ++i) d[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[i][k][r], x[u][k][r], d[i], 0, 0, 0);
+            for (int i = 0; i < TT; ++i) d[u][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[i][k][r], x[u][k][r], d[u][i], 0, 0, 0);
+      }
+      if (TT == 1) load(base + 4 * SPAN);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = base + 16 * u + c;
         if (j >= l1) continue;
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
           const int row = 16 * i + 4 * g;
           T *z = o + row * a.o.row + j * a.o.col;
           if (a.ovec && row + 4 <= s) {
-            write4(z, d[i][0], d[i][1], d[i][2], d[i][3]);
+            write4(z, d[u][i][0], d[u][i][1], d[u][i][2], d[u][i][3]);
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (row + r < s) z[r * a.o.row] = from_f32<T>(d[i][r]);
+              if (row + r < s) z[r * a.o.row] = from_f32<T>(d[u][i][r]);
           }
         }
       }
@@ -911,9 +955,12 @@ Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     return o;
   };
   if (y.s <= SMALL) {
-    // at most 2048 workgroups (all of them run at once), each with 256 entries of l at least; the partial S of one matrix are summed by every workgroup (s <= 16) or by one
+    // Workgroups a matrix.  Two for each CU while the matrices are few: what a workgroup does whatever its share (partial S, the iteration, Q) is 2 .. 6
+    // microseconds of every round (20 of 30000 x 16: 33 us, with 2048 workgroups 61; 250 of 1000 x 48: 79 and 96).  Many matrices are a stream through
+    // memory, where a short last round counts (480 of 8192 x 16 in 1920 workgroups 155, in 480 186; 600 of 3000 x 32 in 1800 244, in 600 270).
     const int64_t most = y.s <= 16 ? 256 : 128;
-    y.chunks = std::max<int64_t>(1, std::min<int64_t>({nmfk_div_up(y.l, 256), 2048 / batch, most}));
+    y.chunks = batch <= 256 ? std::min(nmfk_div_up(y.l, most), 512 / batch) : std::min(nmfk_div_up(y.l, 1024), 2048 / batch);
+    y.chunks = std::max<int64_t>(1, std::min(y.chunks, most));
     y.chunk = nmfk_round_up(nmfk_div_up(y.l, y.chunks), 64);
     y.chunks = nmfk_div_up(y.l, y.chunk);
     y.part = take(batch * y.chunks * y.s * y.s * 8);
@@ -972,7 +1019,8 @@ void small_launch(const SmallArgs &a, const Coefs &cf, unsigned nb, hipStream_t 
     constexpr int BYTES = 4 * TT * TT * 256 * 8;
     static std::atomic<uint64_t> done{0};
     nmfk_allow_dynamic_lds((const void *)small_iterate_kernel<TT>, done, BYTES);
-    small_iterate_kernel<TT><<<dim3(nb), 64 * TT * TT, BYTES, st>>>(a, cf);
+    if (a.chunks > SUMS) small_join_kernel<<<dim3((unsigned)nmfk_div_up((int64_t)a.s * a.s, 256), nb), 256, 0, st>>>(a);
+    small_iterate_kernel<TT><<<dim3(nb), 64 * small_waves(TT), BYTES, st>>>(a, cf, a.chunks > SUMS ? 1 : a.chunks);
   }
   small_apply_kernel<T, TT, WIDE><<<grid, 256, 0, st>>>(a, cf);
 }
