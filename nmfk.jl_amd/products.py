@@ -117,18 +117,18 @@ class Quantized:
         kb = -(-c // 128)
         self.shape, self.tiles, self.device = (r, c), tiles, device
         self._ldv, self._lds = kb * 128, -(-r // 128) if tiles else r
-        self._buf = _torch().empty(r * self._ldv + 4 * kb * self._lds, dtype=_U8, device=device)
+        self._buf = _TORCH.empty(r * self._ldv + 4 * kb * self._lds, dtype=_F8, device=device)
         self._pv = self._buf.data_ptr()
         self._ps = self._pv + r * self._ldv
         return self
 
     def _values(self):
-        return self._buf[: self.shape[0] * self._ldv].view(self.shape[0], self._ldv)
+        return self._buf.view(_U8).as_strided((self.shape[0], self._ldv), (self._ldv, 1))
 
     @property
     def values(self):
         r, c = self.shape
-        return self._buf.view(_F8).as_strided((r, c), (self._ldv, 1))
+        return self._buf.as_strided((r, c), (self._ldv, 1))
 
     @property
     def scales(self):

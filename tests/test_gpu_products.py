@@ -244,6 +244,20 @@ def test_product_grads(P, m, n, k, t):
     check_product(db, values64(w), values64(at), TYPES[t])
 
 
+@pytest.mark.parametrize("m,n,k", [(1500, 3000, 1000), (3000, 1500, 1000), (2500, 2600, 2700), (20000, 70, 100), (32, 2700, 441), (391, 4195, 77), (90, 130, 40)])
+@pytest.mark.parametrize("ta,tb", [(False, True), (True, False), (True, True)])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_product_grads_together_and_apart(P, m, n, k, ta, tb, t):
+    """sizes whose two products share a launch (tiles of 64, 128 and 256, either sum the longer one), split their sums or have few rows"""
+    a, b, dy = randn(1, m, k), randn(2, n, k), randn(3, m, n, t=TYPES[t])
+    at, bt = P.quantize(a.t(), tiles=ta), P.quantize(b.t(), tiles=tb)
+    da, db = P.product_grads(dy, at, bt)
+    check_product(da, values64(P.quantize(dy)), values64(bt), TYPES[t])
+    check_product(db, values64(P.quantize(dy.t())), values64(at), TYPES[t])
+    again = P.product_grads(dy, at, bt)
+    assert torch.equal(da, again[0]) and torch.equal(db, again[1])
+
+
 def test_product_grads_strides_sizes_and_refusals(P):
     (a8, at), (b8, bt) = P.quantize(randn(1, 60, 90), both=True), P.quantize(randn(2, 40, 90), tiles=True, both=True)
     dy = randn(3, 60, 40)
@@ -345,6 +359,25 @@ def test_orthogonalize(P, r, c, t):
     o = P.orthogonalize(g)
     check_ortho(o, g)
     assert torch.equal(o, P.orthogonalize(g))
+
+
+@pytest.mark.parametrize("r,c", [(33, 3000), (64, 5000), (20000, 48), (17, 700), (5, 30000)])
+def test_orthogonalize_many_parts(P, r, c):
+    """a short side whose Gram matrix comes from many parts: joined apart from the iteration, or by it"""
+    g = randn(5, r, c)
+    o = P.orthogonalize(g)
+    check_ortho(o, g)
+    assert torch.equal(o, P.orthogonalize(g))
+
+
+@pytest.mark.parametrize("shape", [(300, 20, 40), (260, 12, 2100), (300, 2200, 33), (257, 64, 64)])
+def test_orthogonalize_more_matrices_than_compute_units(P, shape):
+    g = randn(6, *shape)
+    o = P.orthogonalize(g)
+    check_ortho(o[:3], g[:3])
+    check_ortho(o[-3:], g[-3:])
+    each = torch.stack([P.orthogonalize(x) for x in g])
+    assert torch.allclose(o, each, rtol=2.0 ** -20, atol=2.0 ** -20 * float(each.abs().max()))
 
 
 @pytest.mark.parametrize("shape", [(3, 40, 100), (7, 100, 40), (2, 3, 20, 20), (5, 70, 200), (3, 300, 80), (2, 2, 128, 129), (300, 9, 4), (1, 1, 1)])
