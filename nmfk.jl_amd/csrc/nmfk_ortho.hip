@@ -5,9 +5,11 @@
 // which drives every singular value of X towards one and leaves its singular vectors.  Small singular values grow by a in each step, so
 // does a rounding error made early: everything is carried to 32-bit accuracy or better.
 //
-//   s <= 64: the polynomials of all steps are polynomials of the first S.  One pass over G makes S in 64 bits, one workgroup per matrix
-//     iterates on s x s matrices in LDS in 64 bits (S <- P S P, Q <- Q P), a second pass applies Q.  Two reads and a write of G.
-//   s > 64: products on the 16-bit matrix pipes.  An entry x is kept as two fp16 numbers, hi + lo (22 significant bits), scaled by a power of
+//   s <= 96: the polynomials of all steps are polynomials of the first S.  One pass over G makes S in 64 bits, one workgroup per matrix
+//     iterates on s x s matrices in LDS in 64 bits (S <- P S P, Q <- Q P), a second pass applies Q.  Two reads and a write of G.  (Five steps on
+//     90 x 20000: 133 us, the other form 194; 60 of 96 x 3000: 245 and 488; one of 96 x 96, where the iteration is all there is: 118 and 105.
+//     Beyond, three matrices do not fit into LDS.)
+//   s > 96: products on the 16-bit matrix pipes.  An entry x is kept as two fp16 numbers, hi + lo (22 significant bits), scaled by a power of
 //     two that the growth bound of the step allows; a product is hi hi + hi lo + lo hi, summed in 32 bits (what is dropped is 2^-22 of it).
 #include "nmfk_matrix.h"
 
@@ -15,7 +17,7 @@ using namespace nmfk_mat;
 
 namespace {
 
-constexpr int SMALL = 64;
+constexpr int SMALL = 96;
 constexpr int64_t BATCH = 32768;  // matrices a launch
 constexpr double TINY = 1e-20;    // bounds below it are not followed any further
 
@@ -29,7 +31,7 @@ __device__ __forceinline__ float read_at(const Strided &g, int64_t b, int64_t i,
   return to_f32(((const T *)g.p)[b * g.batch + i * g.row + j * g.col]);
 }
 
-// ---- s <= 64 ---------------------------------------------------------------------------------------------------------------------
+// ---- s <= 96 ---------------------------------------------------------------------------------------------------------------------
 //
 // The fp64 matrix instruction (16 x 16 x 4) leaves entry [4 r + g][c] of its result in register r of lane 16 g + c, and takes, for its k-th step,
 // entry [c][4 k + g] of the first and [4 k + g][c] of the second operand there.  All matrices of the iteration are polynomials of S, hence
@@ -64,7 +66,7 @@ __device__ __forceinline__ void small_load4(const Strided &g, const T *p, int s,
 
 // Partial S over a chunk of l, in 64 bits.  What bounds it is the read of G, so a lane holds an entry in the place where the matrix
 // instruction wants it on both sides, straight from memory.  With s <= 8 the instruction's 16 rows take 16 / s columns of X at once (the
-// diagonal blocks of the result add up to S).
+// diagonal blocks of the result add up to S).  480 of 8192 x 16 in fp32: 60 us, 4.2 TB/s.
 template <typename T, int TT, bool WIDE>
 __global__ __launch_bounds__(256) void small_gram_kernel(SmallArgs a) {
   __shared__ double sum[4][256];
@@ -203,7 +205,7 @@ __device__ __forceinline__ f64x4 sym_product(f64x4 x, f64x4 y) {
   return d;
 }
 
-// 16 < s <= 64: the chunks' partial S, added in their order and left in the place of the first
+// s > 16: the chunks' partial S, added in their order and left in the place of the first
 __global__ __launch_bounds__(256) void small_join_kernel(SmallArgs a) {
   const int ss = a.s * a.s, e = blockIdx.x * 256 + threadIdx.x;
   if (e >= ss) return;
@@ -213,92 +215,124 @@ __global__ __launch_bounds__(256) void small_join_kernel(SmallArgs a) {
   *part = v;
 }
 
-// 16 < s <= 64: the iteration by one workgroup per matrix, a wave per 16 x 16 tile, the matrices in LDS as registers of lanes.  What bounds it above
-// s = 32 is the fp64 matrix instruction (64 cycles) on one CU, so there only the tiles on and below the diagonal are computed and
-// written to both places; below, the way through LDS.
-constexpr bool small_half(int tt) { return tt > 2; }
-constexpr int small_waves(int tt) { return small_half(tt) ? tt * (tt + 1) / 2 : tt * tt; }
+// s > 16: the iteration by one workgroup per matrix.  What bounds it is the fp64 matrix instruction (64 cycles) on one CU, so only the tiles on and
+// below the diagonal are computed, by a wave each (s > 80: two), and kept in LDS: rows of a tile 17 entries apart, so that a tile can be read
+// as its transpose, too.  Above s = 80 there is no room for a fourth matrix, and U takes the place of S.  Five steps: 29 us at s = 64, 46 at 80, 82 at 96
+// (every tile computed, partial sums added by this workgroup: 76 at s = 64).
+constexpr int small_tiles(int tt) { return tt * (tt + 1) / 2; }
+constexpr int small_waves(int tt) { return tt > 5 ? (small_tiles(tt) + 1) / 2 : small_tiles(tt); }
+constexpr int small_lds(int tt) { return (tt > 5 ? 3 : 4) * small_tiles(tt) * 16 * 17 * 8; }
 constexpr int SUMS = 4;  // partial S that the iteration adds itself; more of them are joined before
 template <int TT>
 __global__ __launch_bounds__(64 * small_waves(TT)) void small_iterate_kernel(SmallArgs a, Coefs cf, int parts) {
   extern __shared__ double mats[];
-  constexpr int N = TT * TT * 256;
-  const int s = a.s, w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  constexpr bool HALF = small_half(TT);
-  const int ti = !HALF ? w / TT : w < 1 ? 0 : w < 3 ? 1 : w < 6 ? 2 : 3, tj = HALF ? w - ti * (ti + 1) / 2 : w % TT;
-  double *S = mats, *P = S + N, *Q = P + N, *U = Q + N;
+  constexpr int TILE = 16 * 17, NT = small_tiles(TT), N = NT * TILE, W = small_waves(TT), OWN = (NT + W - 1) / W;
+  constexpr bool TIGHT = TT > 5;
+  const int s = a.s, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  double *S = mats, *P = S + N, *Q = P + N, *U = TIGHT ? S : Q + N;
   const double *part = a.part + (int64_t)blockIdx.x * a.chunks * s * s;
-  const int x = 16 * tj + c;
-  f64x4 v = {0, 0, 0, 0};
+  int ti[OWN], tj[OWN];
 #pragma unroll
-  for (int k = 0; k < SUMS; ++k)
+  for (int o = 0; o < OWN; ++o) {
+    const int id = min(w + o * W, NT - 1);  // (the last tile twice: the same numbers to the same place)
+    ti[o] = id < 1 ? 0 : id < 3 ? 1 : id < 6 ? 2 : id < 10 ? 3 : id < 15 ? 4 : 5;
+    tj[o] = id - ti[o] * (ti[o] + 1) / 2;
+  }
+  const int down = 17 * g + c, across = 17 * c + g;  // entry [4 r + g][c] of a tile: 68 r further; of its transpose: 4 r further
+  auto put = [&](double *m, const f64x4 (&d)[OWN]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int y = 16 * ti + 4 * r + g;
-      if (k < parts && y < s && x < s) v[r] += part[(int64_t)k * s * s + y * s + x];
+    for (int o = 0; o < OWN; ++o)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m[(ti[o] * (ti[o] + 1) / 2 + tj[o]) * TILE + down + 68 * r] = d[o][r];
+  };
+  auto product = [&](const double *m, const double *n, f64x4 (&d)[OWN]) {
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      d[o] = (f64x4){0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < TT; ++k) {
+        const int ui = k >= ti[o] ? (k * (k + 1) / 2 + ti[o]) * TILE + down : (ti[o] * (ti[o] + 1) / 2 + k) * TILE + across, si = k >= ti[o] ? 68 : 4;
+        const int uj = k >= tj[o] ? (k * (k + 1) / 2 + tj[o]) * TILE + down : (tj[o] * (tj[o] + 1) / 2 + k) * TILE + across, sj = k >= tj[o] ? 68 : 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d[o] = __builtin_amdgcn_mfma_f64_16x16x4f64(m[ui + r * si], n[uj + r * sj], d[o], 0, 0, 0);
+      }
     }
-  auto put = [&](double *m, f64x4 d) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) m[((ti * TT + tj) * 4 + r) * 64 + lane] = d[r];
-    if (!HALF || ti == tj) return;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) m[((tj * TT + ti) * 4 + (c >> 2)) * 64 + 16 * (c & 3) + 4 * r + g] = d[r];
   };
-  auto product = [&](const double *m, const double *n) {  // of this wave's tile
-    f64x4 d = {0, 0, 0, 0};
+  f64x4 sv[OWN], p[OWN], q[OWN], u[OWN];
 #pragma unroll
-    for (int k = 0; k < TT; ++k)
+  for (int o = 0; o < OWN; ++o) {
+    sv[o] = (f64x4){0, 0, 0, 0};
+    const int x = 16 * tj[o] + c;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        d = __builtin_amdgcn_mfma_f64_16x16x4f64(m[((k * TT + ti) * 4 + r) * 64 + lane], n[((k * TT + tj) * 4 + r) * 64 + lane], d, 0, 0, 0);
-    return d;
-  };
-  put(S, v);
+    for (int k = 0; k < SUMS; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int y = 16 * ti[o] + 4 * r + g;
+        if (k < parts && y < s && x < s) sv[o][r] += part[(int64_t)k * s * s + y * s + x];
+      }
+  }
+  put(S, sv);
   __syncthreads();
   double norm2 = 0;
-  {  // [i][i]: tile (i / 16, i / 16), register (i % 16) / 4, lane 16 (i % 4) + i % 16; zero behind s
-    const int k = lane >> 4, e = lane & 15;
-    if (k < TT) norm2 = S[((k * TT + k) * 4 + (e >> 2)) * 64 + 16 * (e & 3) + e];
-#pragma unroll
-    for (int o = 32; o; o >>= 1) norm2 += __shfl_xor(norm2, o);
+  for (int i = lane; i < 16 * TT; i += 64) {  // zero behind s
+    const int k = i >> 4, e = i & 15;
+    norm2 += S[(k * (k + 1) / 2 + k) * TILE + 18 * e];
   }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) norm2 += __shfl_xor(norm2, o);
   double inv2, inv;
   small_norm(norm2, inv2, inv);
   __syncthreads();
-  f64x4 sv = v * inv2, q = {0, 0, 0, 0};
+#pragma unroll
+  for (int o = 0; o < OWN; ++o) sv[o] *= inv2;
   put(S, sv);
   __syncthreads();
   for (int k = 0; k < a.steps; ++k) {
-    f64x4 p = cf.v[3 * k + 1] * sv + cf.v[3 * k + 2] * product(S, S);
+    product(S, S, p);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (ti == tj && 4 * r + g == c) p[r] += cf.v[3 * k];
+    for (int o = 0; o < OWN; ++o) {
+      p[o] = cf.v[3 * k + 1] * sv[o] + cf.v[3 * k + 2] * p[o];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (ti[o] == tj[o] && 4 * r + g == c) p[o][r] += cf.v[3 * k];
+    }
     put(P, p);
     __syncthreads();
-    q = k == 0 ? p : product(Q, P);
-    if (k + 1 < a.steps) put(U, product(S, P));
-    __syncthreads();
-    if (k + 1 < a.steps) {
-      put(Q, q);
-      sv = product(U, P);
-      put(S, sv);
-      __syncthreads();
+    if (k == 0) {
+#pragma unroll
+      for (int o = 0; o < OWN; ++o) q[o] = p[o];
+    } else {
+      product(Q, P, q);
     }
+    if (k + 1 == a.steps) break;
+    product(S, P, u);
+    if (TIGHT) __syncthreads();
+    put(U, u);
+    __syncthreads();
+    put(Q, q);
+    product(U, P, sv);
+    if (TIGHT) __syncthreads();
+    put(S, sv);
+    __syncthreads();
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int y = 16 * ti + 4 * r + g;
-    if (y >= s || x >= s) continue;
-    float *out = a.q + (int64_t)blockIdx.x * s * s;
-    out[y * s + x] = (float)(q[r] * inv);
-    if (HALF && ti != tj) out[x * s + y] = (float)(q[r] * inv);
+  for (int o = 0; o < OWN; ++o) {
+    const int x = 16 * tj[o] + c;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int y = 16 * ti[o] + 4 * r + g;
+      if (y >= s || x >= s) continue;
+      float *out = a.q + (int64_t)blockIdx.x * s * s;
+      out[y * s + x] = (float)(q[o][r] * inv);
+      if (ti[o] != tj[o]) out[x * s + y] = (float)(q[o][r] * inv);
+    }
   }
 }
 
 // O = Q X over a chunk of l, on the fp32 matrix pipe (16 x 16 x 4: entry [c][.] of the first, [.][c] of the second operand in lane 16 g + c, result
 // [4 g + r][c] in register r).  Which four of the sum's entries a step takes is free: a lane's four consecutive entries of X or of Q serve four steps,
 // or four columns, and its four results stand next to each other in O.  s <= 16: every workgroup iterates for itself, a wave in registers (about
-// 2 microseconds, less than a launch), while the first entries of X are on their way.
+// 2 microseconds, less than a launch), while the first entries of X are on their way.  480 of 8192 x 16 in fp32: 90 us, 5.6 TB/s.
 template <typename T, int TT, bool WIDE>
 __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf) {
   __shared__ double sum[256];
@@ -450,7 +484,7 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
   }
 }
 
-// ---- s > 64 ----------------------------------------------------------------------------------------------------------------------
+// ---- s > 96 ----------------------------------------------------------------------------------------------------------------------
 //
 // A split matrix: rows of 128-byte blocks, a block = the hi parts of 32 consecutive entries, then their lo parts; zeros behind the last entry.
 
@@ -489,9 +523,9 @@ __device__ __forceinline__ f32x4 get4(const char *row, int col) {
   return v;
 }
 
-constexpr int NORM_PARTS = 256;  // one for each thread of split_kernel
+constexpr int NORM_PARTS = 256;  // at most: one for each thread of split_kernel
 
-// |G|^2 in 64 bits, NORM_PARTS partial sums per matrix: a wave walks rows along the contiguous side, four entries a lane
+// |G|^2 in 64 bits, as partial sums of gridDim.x workgroups per matrix: a wave walks rows along the contiguous side, four entries a lane
 template <typename T>
 __global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s, int64_t l, double *part, int vec) {
   const int64_t b = b0 + blockIdx.y;
@@ -501,7 +535,7 @@ __global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s,
   const T *p = (const T *)g.p + b * g.batch;
   double v = 0;
   const int lane = threadIdx.x & 63;
-  for (int64_t o = blockIdx.x + NORM_PARTS * (threadIdx.x >> 6); o < outer; o += 4 * NORM_PARTS) {
+  for (int64_t o = blockIdx.x + gridDim.x * (threadIdx.x >> 6); o < outer; o += 4 * gridDim.x) {
     const T *q = p + o * so;
 #pragma unroll 4
     for (int64_t e = lane * 4; e < inner; e += 256) {
@@ -521,17 +555,17 @@ __global__ __launch_bounds__(256) void norm_kernel(Strided g, int64_t b0, int s,
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
   if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = v;
   __syncthreads();
-  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * NORM_PARTS + blockIdx.x] = ((sum[0] + sum[1]) + sum[2]) + sum[3];
+  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = ((sum[0] + sum[1]) + sum[2]) + sum[3];
 }
 
 // X' = (G * (1 / |G|) * 2^e)', split: l rows of s entries, and rows of zeros up to a multiple of 32.  A 64 x 64 tile per workgroup, turned in LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void split_kernel(Strided g, int64_t b0, int s, int64_t l, const double *part, double pow2, Split xt) {
+__global__ __launch_bounds__(256) void split_kernel(Strided g, int64_t b0, int s, int64_t l, const double *part, int parts, double pow2, Split xt) {
   __shared__ float tile[64][65];
   const int t = threadIdx.x;
   const int64_t b = b0 + blockIdx.z;
   __shared__ double sums[4];
-  double norm2 = part[(int64_t)blockIdx.z * NORM_PARTS + t];
+  double norm2 = t < parts ? part[(int64_t)blockIdx.z * parts + t] : 0.0;
 #pragma unroll
   for (int o = 32; o; o >>= 1) norm2 += __shfl_xor(norm2, o);
   if ((t & 63) == 0) sums[t >> 6] = norm2;
@@ -1016,7 +1050,7 @@ void small_launch(const SmallArgs &a, const Coefs &cf, unsigned nb, hipStream_t 
   const dim3 grid((unsigned)a.chunks, nb);
   small_gram_kernel<T, TT, WIDE><<<grid, 256, 0, st>>>(a);
   if (TT > 1) {
-    constexpr int BYTES = 4 * TT * TT * 256 * 8;
+    constexpr int BYTES = small_lds(TT);
     static std::atomic<uint64_t> done{0};
     nmfk_allow_dynamic_lds((const void *)small_iterate_kernel<TT>, done, BYTES);
     if (a.chunks > SUMS) small_join_kernel<<<dim3((unsigned)nmfk_div_up((int64_t)a.s * a.s, 256), nb), 256, 0, st>>>(a);
@@ -1052,8 +1086,12 @@ int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, 
       NMFK_SMALL(2);
     else if (y.s <= 48)
       NMFK_SMALL(3);
-    else
+    else if (y.s <= 64)
       NMFK_SMALL(4);
+    else if (y.s <= 80)
+      NMFK_SMALL(5);
+    else
+      NMFK_SMALL(6);
 #undef NMFK_SMALL
   }
   return nmfk_launched("nmfk_orthogonalize");
@@ -1116,8 +1154,9 @@ int ortho_large(const Layout &y, const Strided &g, const Strided &o, int steps, 
     double *norm = (double *)(work + y.norm) + b0 * NORM_PARTS;
     double u = 1.0;  // bound of the singular values of X; e?: the power of two a matrix is scaled by
     int ex = exponent(1.01 * u);
-    norm_kernel<T><<<dim3(NORM_PARTS, nb), 256, 0, st>>>(g, b0, s, l, norm, g.row == 1 || g.col == 1);
-    split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, ldexp(1.0, ex), X);
+    const unsigned parts = (unsigned)std::max<int64_t>(1, std::min<int64_t>(NORM_PARTS, 2048 / nb));  // 424 of 78 x 351: 82 us with 256 parts each, 16 so
+    norm_kernel<T><<<dim3(parts, nb), 256, 0, st>>>(g, b0, s, l, norm, g.row == 1 || g.col == 1);
+    split_kernel<T><<<dim3((unsigned)nmfk_div_up(l, 64), (unsigned)nmfk_div_up(s, 64), nb), 256, 0, st>>>(g, b0, s, l, norm, (int)parts, ldexp(1.0, ex), X);
     for (int k = 0; k < steps; ++k) {
       const double ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
       const int es = exponent(1.02 * u * u), ep = exponent(1.02 * std::max(peak(0, cb, cc, u, EVEN), TINY));

@@ -387,7 +387,7 @@ def test_orthogonalize_stacks(P, shape):
 
 
 @pytest.mark.parametrize("spectrum", ["nonnegative", "decaying", "rank one", "tiny", "huge", "two"])
-@pytest.mark.parametrize("r,c", [(40, 60), (200, 260), (1500, 150)])
+@pytest.mark.parametrize("r,c", [(40, 60), (90, 150), (200, 260), (1500, 150)])
 def test_orthogonalize_spectra(P, spectrum, r, c):
     g = randn(12, r, c).abs() if spectrum == "nonnegative" else randn(12, r, c)
     s = min(r, c)
@@ -431,7 +431,7 @@ def test_orthogonalize_layouts(P):
         assert bool((out == 5.0).all())
 
 
-@pytest.mark.parametrize("r,c", [(20, 40), (100, 130)])
+@pytest.mark.parametrize("r,c", [(20, 40), (70, 90), (100, 130)])
 def test_orthogonalize_special(P, r, c):
     g = randn(15, 5, r, c)
     g[1] = 0
