@@ -916,18 +916,19 @@ __global__ __launch_bounds__(256) void sym_join_kernel(GemmArgs a) {
 
 // Which tiles a product is cut into.  Small tiles fill the 256 CUs where there is little to do, large ones read less for each operation.  The estimate, in
 // microseconds, measured: `places` tiles of a side run at a time (LDS: 128, 64, 32 KB a workgroup); such a round takes `step` for each block of
-// 32 of the sum, at least `alone` of that when it is not full, and `rest` to begin and to write.
+// 32 of the sum, and `rest` to begin and to write.  A round that is not full takes less of `step`: GRAM and SYM the part of it that is filled, but at
+// least `alone`; APPLY and LAST `base` and the filled part of what remains (1000 x 1000 in 256 tiles of 64: 18 us, in 64 tiles of 128: 27).
 struct TileCost {
   int side;
   int64_t places;
-  double step, alone, rest, part;  // part: a partial sum to write and read again
+  double step, alone, base, rest, part;  // part: a partial sum to write and read again
 };
-constexpr TileCost COST[3] = {{64, 1024, 0.95, 0.85, 4, 0.008}, {128, 512, 1.35, 0.55, 6, 0.03}, {256, 256, 2.6, 1.0, 16, 0}};
+constexpr TileCost COST[3] = {{64, 1024, 0.95, 0.85, 0.2, 4, 0.008}, {128, 512, 1.35, 0.55, 0, 6, 0.03}, {256, 256, 2.6, 1.0, 0, 16, 0}};
 
-double tiles_cost(const TileCost &c, int64_t tiles, int64_t kb) {
+double tiles_cost(const TileCost &c, int64_t tiles, int64_t kb, bool sym) {
   const int64_t full = tiles / c.places, rest = tiles - full * c.places;
-  const double fill = (double)nmfk_div_up(rest, 256) * 256.0 / (double)c.places;
-  return (double)full * (c.step * (double)kb + c.rest) + (rest ? c.step * std::max(fill, c.alone) * (double)kb + c.rest : 0.0);
+  const double filled = (double)nmfk_div_up(rest, 256) * 256.0 / (double)c.places, share = sym ? std::max(filled, c.alone) : c.base + (1 - c.base) * filled;
+  return (double)full * (c.step * (double)kb + c.rest) + (rest ? c.step * share * (double)kb + c.rest : 0.0);
 }
 
 // A symmetric product: the last round of tiles is rarely full, so the sums of its tiles may be split (the launch that joins them costs 4).  4096 x 4096 with
@@ -946,9 +947,9 @@ SymPlan sym_plan(int64_t m, int64_t batch, int64_t kb) {
     const int64_t tm = nmfk_div_up(m, c.side), tiles = tm * (tm + 1) / 2, total = tiles * batch;
     if (total > 0x7fffffff / 64) continue;
     const int64_t whole = total / c.places * c.places, rest = total - whole;
-    const double before = tiles_cost(c, whole, kb);
+    const double before = tiles_cost(c, whole, kb, true);
     for (int64_t s = 1; s <= 64 && (s == 1 || (s * 4 <= kb && s * rest <= 3 * c.places)); ++s) {
-      const double cost = before + tiles_cost(c, rest * s, nmfk_div_up(kb, s)) + (s > 1 ? c.part * (double)(rest * s) + 4.0 : 0.0);
+      const double cost = before + tiles_cost(c, rest * s, nmfk_div_up(kb, s), true) + (s > 1 ? c.part * (double)(rest * s) + 4.0 : 0.0);
       if (cost >= least) continue;
       least = cost;
       best = {c.side, (int)tiles, (int)whole, (int)rest, (int)s, (int)nmfk_div_up(kb, s)};
@@ -963,7 +964,7 @@ int full_side(int64_t m, int64_t n, int64_t batch, int64_t kb) {
   int side = 0;
   double least = 1e30;
   for (const TileCost &c : COST) {
-    const double cost = tiles_cost(c, nmfk_div_up(m, c.side) * nmfk_div_up(n, c.side) * batch, kb);
+    const double cost = tiles_cost(c, nmfk_div_up(m, c.side) * nmfk_div_up(n, c.side) * batch, kb, false);
     if (cost < least) least = cost, side = c.side;
   }
   return side;
