@@ -267,7 +267,7 @@ int nmfk_multi_sweep(nmfk_multi *mh, int nk, const int32_t *ks, int nruns, const
  * No call allocates, copies to the host or keeps anything, so all of them can be captured into a hipGraph. */
 enum { NMFK_F32 = 0, NMFK_BF16 = 1, NMFK_F16 = 2 };  /* types of the matrices that are not in 8 bits */
 
-/* X (rows x cols) in 8-bit floating point, e4m3, with a scale for each block: 128 consecutive entries of a row (tiles = 0) or a 128 x 128
+/* X (rows x cols, each at most 2^22) in 8-bit floating point, e4m3, with a scale for each block: 128 consecutive entries of a row (tiles = 0) or a 128 x 128
  * tile (tiles = 1), the last ones shorter.  scale = max(max |x| / 448, 2^-126) over the block's finite entries in fp32; value = x / scale,
  * rounded to fp32, then to e4m3, both to nearest with ties to even; NaN where x is not finite.
  *  X          entry (i, j) at X[i * row_stride + j * col_stride]; one of the strides is 1
@@ -280,7 +280,7 @@ int nmfk_quantize(int device, void *stream, int dtype, const void *X, int64_t ro
 
 /* Y = A * B' (m x n, entry (i, j) at Y[i * ldy + j]) of two matrices in 8 bits, A m x k and B n x k, as nmfk_quantize lays them out:
  * Y[i, j] = sum over blocks b of sA[i, b] * sB[j, b] * sum of the block's a[i, t] * b[j, t], summed in fp32, rounded once to `dtype`.
- * lda, ldb: at most 2^23.  k = 0 gives zeros.  The result does not depend on the run (no atomics).  nmfk_product_workspace: bytes of `work` for these sizes and this type of Y. */
+ * m, n, k: at most 2^22; lda, ldb: at most 2^23.  k = 0 gives zeros.  The result does not depend on the run (no atomics).  nmfk_product_workspace: bytes of `work` for these sizes and this type of Y. */
 int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes);
 int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, const uint8_t *A, int64_t lda, const float *sA,
                  int64_t ldsa, int a_tiles, const uint8_t *B, int64_t ldb, const float *sB, int64_t ldsb, int b_tiles, int dtype,

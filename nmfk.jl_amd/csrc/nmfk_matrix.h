@@ -1,8 +1,6 @@
 // Shared by the operators on plain matrices (nmfk_quant.hip, nmfk_prod8.hip, nmfk_ortho.hip): element types, the device guard of an entry
 // point, and the staging of 128-byte rows into LDS that the tiled products use.
 #pragma once
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -39,7 +37,6 @@ static inline int nmfk_launched(const char *what) {
 
 static inline int64_t nmfk_div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t nmfk_round_up(int64_t a, int64_t b) { return nmfk_div_up(a, b) * b; }
-static inline int nmfk_type_size(int dtype) { return dtype == NMFK_F32 ? 4 : 2; }
 
 namespace nmfk_mat {
 

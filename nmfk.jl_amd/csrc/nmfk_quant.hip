@@ -238,7 +238,6 @@ NMFK_EXPORT int nmfk_quantize(int device, void *stream, int dtype, const void *X
     a = {X, rows, cols, rows == 1 ? cols : row_stride, values, ldv, scales, lds, tvalues, ldtv, tscales, ldts};
   else
     a = {X, cols, rows, cols == 1 ? rows : col_stride, tvalues, ldtv, tscales, ldts, values, ldv, scales, lds};
-  if (nmfk_div_up(a.rows, 128) > 65535) return fail(NMFK_ERR_UNSUPPORTED, "nmfk_quantize: too many rows");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == NMFK_F32)
     quant_launch<float>(a, tiles != 0, st);
