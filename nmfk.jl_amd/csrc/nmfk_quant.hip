@@ -38,13 +38,16 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 // x / s rounded to nearest, for the many x of a block: with r = 1 / s rounded to nearest, q0 = x r, one correction q0 + r (x - q0 s) gives the
 // correctly rounded quotient (Markstein's theorem) unless the significand of s is all ones.  The residual has to be exact: s in [2^-80, 2^80] makes
 // it so for every quotient that does not round to zero in e4m3.  Elsewhere (EASY = false; a wave takes that path as a whole): the division, 11
-// instructions instead of 3.  NaN and infinities come out of the short form as NaN by themselves.
-__device__ __forceinline__ bool easy_divisor(float s) { return s >= 0x1p-80f && s <= 0x1p80f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu; }
+// instructions instead of 3.  NaN and infinities come out of the short form as NaN by themselves, zeros with their sign (so a block with
+// nothing else in it, as behind the last row, takes it, too).
+__device__ __forceinline__ bool easy_divisor(float top, float s) {
+  return top == 0.f || (s >= 0x1p-80f && s <= 0x1p80f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu);
+}
 template <bool EASY>
 __device__ __forceinline__ float quotient(float x, float s, float r) {
   if (EASY) {
     const float q = x * r;
-    return fmaf(fmaf(-q, s, x), r, q);
+    return fmaf(-fmaf(q, s, -x), r, q);
   }
   return fabsf(x) <= 3.402823466e38f ? x / s : __uint_as_float(0x7fc00000u);
 }
@@ -84,14 +87,16 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a, int64_t bl
   const int64_t c = kb * 128 + (threadIdx.x & 31) * 4;
   float x[4];
   load4<T>(a, r, c, x);
-  float top = fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
-  const float s = block_scale(largest32(top)), inv = 1.0f / s;
-  *(uint32_t *)(a.v + r * a.ldv + c) = __all(easy_divisor(s)) ? quotients<true>(x[0], x[1], x[2], x[3], s, inv) : quotients<false>(x[0], x[1], x[2], x[3], s, inv);
+  const float top = largest32(fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3]))));
+  const float s = block_scale(top), inv = 1.0f / s;
+  *(uint32_t *)(a.v + r * a.ldv + c) = __all(easy_divisor(top, s)) ? quotients<true>(x[0], x[1], x[2], x[3], s, inv) : quotients<false>(x[0], x[1], x[2], x[3], s, inv);
   if ((threadIdx.x & 31) == 0) a.s[kb * a.sld + r] = s;
 }
 
 // A 128 x 128 tile per workgroup of 1024: lane group g = thread / 32 owns the rows 4 g .. 4 g + 3, thread % 32 four columns.  (With 256 threads and 16 rows each the
-// code is four times as long, and a small matrix pays for fetching it: 35 tiles of fp32 in both orientations take 9.5 us instead of 12.3.)
+// code is four times as long, and a small matrix pays for fetching it: 35 tiles of fp32 in both orientations 12.3 us instead of 8.5.)  Scales of rows and
+// columns are made by 256 of the threads, once each: two divisions, which in every thread that needs them cost as much as the quotients (4096 x 4096 of
+// bf16 23 us instead of 16, the 35 tiles 8.5 instead of 5).
 // `rs`, `cs`: the scales of the thread's rows and columns and their reciprocals (TILES: the one of the tile).
 template <bool TILES, bool EASY>
 __device__ __forceinline__ void quant_tile_values(const QuantArgs &a, const float (&x)[4][4], const float (&rs)[4], const float (&rr)[4], const float (&cs)[4],
@@ -125,7 +130,7 @@ __device__ __forceinline__ void quant_tile_values(const QuantArgs &a, const floa
 template <typename T, bool TILES>
 __global__ __launch_bounds__(1024) void quant_tile_kernel(QuantArgs a) {
   __shared__ __attribute__((aligned(16))) char turn[128 * 128];
-  __shared__ __attribute__((aligned(16))) float ctop[16][128];
+  __shared__ __attribute__((aligned(16))) float ctop[16][128], rtop[2 * 128];
   __shared__ int hard;
   const int t = threadIdx.x, g = t >> 5, cg = t & 31;
   const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
@@ -155,44 +160,56 @@ __global__ __launch_bounds__(1024) void quant_tile_kernel(QuantArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) cmax[j] = fmaxf(cmax[j], __shfl_xor(cmax[j], 32));
   if (!(g & 1)) *(f32x4 *)&ctop[g >> 1][cg * 4] = (f32x4){cmax[0], cmax[1], cmax[2], cmax[3]};
+  if (!TILES) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rmax[i] = largest32(rmax[i]);
+    if (cg == 0) *(f32x4 *)&rtop[g * 4] = (f32x4){rmax[0], rmax[1], rmax[2], rmax[3]};
+  }
   __syncthreads();
   if (t < 128) {
     float m = ctop[0][t];
 #pragma unroll
     for (int h = 1; h < 16; ++h) m = fmaxf(m, ctop[h][t]);
-    ctop[0][t] = m;
+    if (TILES) {
+      ctop[0][t] = m;
+    } else {  // a column's scale and its reciprocal; two divisions, so once for each
+      const float s = block_scale(m);
+      ctop[0][t] = s;
+      ctop[1][t] = 1.0f / s;
+      if (!easy_divisor(m, s)) hard = 1;
+      if (a.tv && c0 + t < a.cols) a.ts[(int64_t)blockIdx.y * a.tsld + c0 + t] = s;
+    }
+  } else if (!TILES && t < 256) {
+    const int r = t - 128;
+    const float m = rtop[r], s = block_scale(m);
+    rtop[r] = s;
+    rtop[128 + r] = 1.0f / s;
+    if (!easy_divisor(m, s)) hard = 1;
+    if (a.v && r0 + r < a.rows) a.s[(int64_t)blockIdx.x * a.sld + r0 + r] = s;
   }
   __syncthreads();
-  const f32x4 top = *(const f32x4 *)&ctop[0][cg * 4];
   float rs[4], rr[4], cs[4], cr[4];
-  bool easy = true;
+  bool easy;
+  const f32x4 top = *(const f32x4 *)&ctop[0][cg * 4];
   if (TILES) {
-    rs[0] = block_scale(largest32(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))));
+    const float m = largest32(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+    rs[0] = block_scale(m);
     rr[0] = 1.0f / rs[0];
-    easy = easy_divisor(rs[0]);
+    easy = easy_divisor(m, rs[0]);  // the same for all
     if (t == 0) {
       if (a.v) a.s[(int64_t)blockIdx.x * a.sld + blockIdx.y] = rs[0];
       if (a.tv) a.ts[(int64_t)blockIdx.y * a.tsld + blockIdx.x] = rs[0];
     }
   } else {
+    const f32x4 inv = *(const f32x4 *)&ctop[1][cg * 4], row = *(const f32x4 *)&rtop[g * 4], row_inv = *(const f32x4 *)&rtop[128 + g * 4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      rs[i] = block_scale(largest32(rmax[i]));
-      rr[i] = 1.0f / rs[i];
-      cs[i] = block_scale(top[i]);
-      cr[i] = 1.0f / cs[i];
-      easy = easy && easy_divisor(rs[i]) && easy_divisor(cs[i]);
-      if (a.tv && g == 0 && c0 + cg * 4 + i < a.cols) a.ts[(int64_t)blockIdx.y * a.tsld + c0 + cg * 4 + i] = cs[i];
-    }
-    if (a.v && cg < 4 && r0 + g * 4 + cg < a.rows)
-      a.s[(int64_t)blockIdx.x * a.sld + r0 + g * 4 + cg] = cg == 0 ? rs[0] : cg == 1 ? rs[1] : cg == 2 ? rs[2] : rs[3];
+    for (int i = 0; i < 4; ++i) rs[i] = row[i], rr[i] = row_inv[i], cs[i] = top[i], cr[i] = inv[i];
+    easy = !hard;
   }
-  if (!easy) hard = 1;
-  __syncthreads();
-  if (hard)
-    quant_tile_values<TILES, false>(a, x, rs, rr, cs, cr, turn, r0, c0);
-  else
+  if (easy)
     quant_tile_values<TILES, true>(a, x, rs, rr, cs, cr, turn, r0, c0);
+  else
+    quant_tile_values<TILES, false>(a, x, rs, rr, cs, cr, turn, r0, c0);
 }
 
 template <typename T>

@@ -111,6 +111,20 @@ def test_quantize_special_values(P, tiles):
     check_quantized(w, x.t(), tiles)
 
 
+@pytest.mark.parametrize("tiles,both", [(False, False), (False, True), (True, True)])
+def test_quantize_zeros_keep_their_sign(P, tiles, both):
+    x = torch.zeros(130, 260, device="cuda")
+    x[::2, ::3] = -0.0
+    x[5, 7], x[9] = 3.0, -0.0  # blocks with an entry, and without
+    x[70, 200], x[71, 201] = float("nan"), float("inf")
+    want = x.clone()
+    for v, w in zip(P.quantize(x, tiles=tiles, both=True) if both else (P.quantize(x, tiles=tiles),), (want, want.t())):
+        v = v.values.float()
+        there = torch.isfinite(w)
+        assert torch.equal(torch.isnan(v), ~there)
+        assert torch.equal(torch.signbit(v)[there], torch.signbit(w)[there])
+
+
 def test_quantize_ties_go_to_even(P):
     steps = torch.arange(0, 127, dtype=torch.uint8).view(F8).float()  # every finite non-negative value of e4m3
     mid = (steps[1:] + steps[:-1]) / 2
