@@ -11,6 +11,8 @@
 //     Beyond, three matrices do not fit into LDS.)
 //   s > 96: products on the 16-bit matrix pipes.  An entry x is kept as two fp16 numbers, hi + lo (22 significant bits), scaled by a power of
 //     two that the growth bound of the step allows; a product is hi hi + hi lo + lo hi, summed in 32 bits (what is dropped is 2^-22 of it).
+#include <type_traits>
+
 #include "nmfk_matrix.h"
 
 using namespace nmfk_mat;
@@ -18,6 +20,7 @@ using namespace nmfk_mat;
 namespace {
 
 constexpr int SMALL = 96;
+constexpr double GROWTH32 = 512;  // up to which s <= 96 applies its factor in 32 bits: five of the default steps, 3e-5 of |G| in the directions that grow so
 constexpr int64_t BATCH = 32768;  // matrices a launch
 constexpr double TINY = 1e-20;    // bounds below it are not followed any further
 
@@ -40,9 +43,10 @@ __device__ __forceinline__ float read_at(const Strided &g, int64_t b, int64_t i,
 struct SmallArgs {
   Strided g, o;
   double *part;  // [batch][chunks][s][s]
-  float *q;      // [batch][s][s], s > 16
+  double *q;     // s > 16, [batch][small_q_size]: Q / |G| in the order in which small_apply_kernel takes it, then the exponent left out of it
   int64_t b0;
   int s, chunks, steps;
+  int q64;           // Q is applied in 64 bits
   int64_t l, chunk;  // entries of l per workgroup
   int gvec, ovec;    // the side that is walked is contiguous: four entries at once
 };
@@ -198,6 +202,25 @@ __device__ __forceinline__ void small_norm(double norm2, double &inv2, double &i
   inv = !finite ? nan : norm2 > 0 ? 1.0 / sqrt(norm2) : 0.0;
 }
 
+// Q / |G| goes up to growth / |G|, which 32 bits do not hold for a very small |G|, nor its bits for a very large one: there the power of two stays out of Q,
+// and G is multiplied by it (exactly).
+__device__ __forceinline__ int small_exponent(double norm2, int q64) {
+  const int e = (__double2hiint(norm2) >> 20) - 1023;  // (zero and what is not finite are far outside)
+  return !q64 && (e < -200 || e > 200) && e > -400 && e < 400 ? -e >> 1 : 0;
+}
+
+// Where small_apply_kernel looks for Q[y, x]: the operand of step k of tile (i, j) for lane 16 g + c at [((i TT + j) 4 + k) 64 + 16 g + c].  The fp64 instruction
+// leaves entry [4 r + g] where the fp32 one leaves [4 g + r]: its rows are dealt so that a lane gets row 4 g + r, too.
+template <int TT>
+__host__ __device__ constexpr int small_q_size() {
+  return TT * TT * 256 + 32;
+}
+template <int TT>
+__device__ __forceinline__ int small_q_at(int y, int x, int q64) {
+  const int c = q64 ? ((y & 3) << 2) + ((y >> 2) & 3) : y & 15;
+  return (((y >> 4) * TT + (x >> 4)) * 4 + (x & 3)) * 64 + ((x & 12) << 2) + c;
+}
+
 __device__ __forceinline__ f64x4 sym_product(f64x4 x, f64x4 y) {
   f64x4 d = {0, 0, 0, 0};
 #pragma unroll
@@ -315,34 +338,48 @@ __global__ __launch_bounds__(64 * small_waves(TT)) void small_iterate_kernel(Sma
     put(S, sv);
     __syncthreads();
   }
+  const int e = small_exponent(norm2, a.q64);
+  inv = ldexp(inv, -e);
+  double *out = a.q + (int64_t)blockIdx.x * small_q_size<TT>();
+  if (threadIdx.x == 0) out[TT * TT * 256] = e;
 #pragma unroll
   for (int o = 0; o < OWN; ++o) {
     const int x = 16 * tj[o] + c;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int y = 16 * ti[o] + 4 * r + g;
-      if (y >= s || x >= s) continue;
-      float *out = a.q + (int64_t)blockIdx.x * s * s;
-      out[y * s + x] = (float)(q[o][r] * inv);
-      if (ti[o] != tj[o]) out[x * s + y] = (float)(q[o][r] * inv);
+      const double v = y < s && x < s ? q[o][r] * inv : 0.0;
+      out[small_q_at<TT>(y, x, a.q64)] = v;
+      if (ti[o] != tj[o]) out[small_q_at<TT>(x, y, a.q64)] = v;
     }
   }
 }
 
-// O = Q X over a chunk of l, on the fp32 matrix pipe (16 x 16 x 4: entry [c][.] of the first, [.][c] of the second operand in lane 16 g + c, result
-// [4 g + r][c] in register r).  Which four of the sum's entries a step takes is free: a lane's four consecutive entries of X or of Q serve four steps,
-// or four columns, and its four results stand next to each other in O.  s <= 16: every workgroup iterates for itself, a wave in registers (about
-// 2 microseconds, less than a launch), while the first entries of X are on their way.  480 of 8192 x 16 in fp32: 90 us, 5.6 TB/s.
-template <typename T, int TT, bool WIDE>
-__global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf) {
-  __shared__ double sum[256];
-  __shared__ float qs[16][17];
+// O = Q G over a chunk of l, on the fp32 matrix pipe (16 x 16 x 4: entry [c][.] of the first, [.][c] of the second operand in lane 16 g + c, result
+// [4 g + r][c] in register r) or on the fp64 one.  Which four of the sum's entries a step takes is free: a lane's four consecutive entries of G or of Q
+// serve four steps, or four columns, and its four results stand next to each other in O.  s <= 16: every workgroup iterates for itself, a wave in registers
+// (about 2 microseconds, less than a launch), while the first entries of G are on their way.  480 of 8192 x 16 in fp32: 90 us, 5.6 TB/s.
+//
+// A = float: Q in registers, rounded to 32 bits, which puts an error of growth * 2^-24 |G| into O like the same steps in fp32 would.  A = double where that is
+// too much: O is off by its own rounding (to fp32, then to its type).  Q stands in LDS, which is quick enough for an instruction of 64 cycles.  60 of 96 x 3000:
+// 75 us in 32 bits, 112 in 64.
+__device__ __forceinline__ f32x4 small_multiply(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f64x4 small_multiply(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+
+template <typename T, typename O, typename A, int TT, bool WIDE>
+__global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(SmallArgs a, Coefs cf) {
+  constexpr bool Q64 = std::is_same<A, double>::value, LDS = Q64 && TT > 1;
+  using vec = typename std::conditional<Q64, f64x4, f32x4>::type;
+  __shared__ double sum[TT == 1 ? 256 : 1];
+  __shared__ A own[TT == 1 ? 256 : 1];
+  __shared__ int exponent;
+  extern __shared__ __attribute__((aligned(16))) double qs[];  // LDS: the operands of Q as in memory
   const int by = gridDim.y - 1 - blockIdx.y;  // the matrices read last are still in the last-level cache: take them first
   const int64_t b = a.b0 + by;
   const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
   const int s = a.s, t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 15, g = lane >> 4;
   const T *p = (const T *)a.g.p + b * a.g.batch;
-  T *o = (T *)a.o.p + b * a.o.batch;
+  O *o = (O *)a.o.p + b * a.o.batch;
   constexpr int U = WIDE ? 4 : TT == 1 ? 4 : TT == 2 ? 2 : 1, SPAN = 16 * U;  // columns a wave takes at a time
   float x[WIDE ? TT : U][WIDE ? 4 : TT][4];
   auto load = [&](int64_t base) {
@@ -360,8 +397,9 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
   };
   const int64_t base0 = l0 + (int64_t)w * SPAN;
   if (TT == 1) load(base0);  // on its way during the iteration
-  float q[TT][TT][4];
-  if (TT == 1) {
+  A mine[LDS ? 1 : TT][LDS ? 1 : TT][4];
+  int ex = 0;
+  if constexpr (TT == 1) {
     const double *part = a.part + (int64_t)by * a.chunks * s * s;
     const int y = t >> 4, x = t & 15;
     double v[4] = {0, 0, 0, 0};
@@ -399,68 +437,128 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
         if (k + 1 < a.steps) S = sym_product(sym_product(S, P), P);
         Q = k == 0 ? P : sym_product(Q, P);
       }
+      const int e = small_exponent(norm2, Q64);
+      inv = ldexp(inv, -e);
+      if (lane == 0) exponent = e;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) qs[4 * r + g][c] = (float)(Q[r] * inv);
+      for (int r = 0; r < 4; ++r) own[small_q_at<1>(4 * r + g, c, Q64)] = (A)(Q[r] * inv);
     }
     __syncthreads();
+    ex = __builtin_amdgcn_readfirstlane(exponent);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) q[0][0][k] = qs[c][4 * g + k];
+    for (int k = 0; k < 4; ++k) mine[0][0][k] = own[k * 64 + lane];
   } else {
-    const float *m = a.q + (int64_t)by * s * s;
+    const double *m = a.q + (int64_t)by * small_q_size<TT>();
+    if constexpr (LDS) {
+      for (int e = t; e < TT * TT * 128; e += 256) ((i32x4 *)qs)[e] = ((const i32x4 *)m)[e];
+      __syncthreads();
+    } else {
+      ex = __builtin_amdgcn_readfirstlane((int)m[TT * TT * 256]);
 #pragma unroll
-    for (int i = 0; i < TT; ++i)
+      for (int i = 0; i < TT; ++i)
 #pragma unroll
-      for (int j = 0; j < TT; ++j) {
-        const int y = 16 * i + c, x = 16 * j + 4 * g;
-        if (y < s && x + 4 <= s)
-          read4(m + y * s + x, q[i][j]);
-        else
+        for (int j = 0; j < TT; ++j)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) q[i][j][k] = y < s && x + k < s ? m[y * s + x + k] : 0.f;
-      }
+          for (int k = 0; k < 4; ++k) mine[i][j][k] = (A)m[((i * TT + j) * 4 + k) * 64 + lane];
+    }
   }
+  auto q = [&](int i, int j, int k) -> A {
+    if constexpr (LDS)
+      return qs[((i * TT + j) * 4 + k) * 64 + lane];
+    else
+      return mine[i][j][k];
+  };
+  auto scale = [&]() {
+#pragma unroll
+    for (int i = 0; i < (WIDE ? TT : U); ++i)
+#pragma unroll
+      for (int k = 0; k < (WIDE ? 4 : TT); ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][k][e] = ldexpf(x[i][k][e], ex);
+  };
+  auto store_wide = [&](int row, int64_t j, float v0, float v1, float v2, float v3) {  // entries j .. j + 3 of a row
+    if (row >= s) return;
+    O *z = o + row * a.o.row + j * a.o.col;
+    if (a.ovec && j + 4 <= l1) {
+      write4(z, v0, v1, v2, v3);
+    } else {
+      const float v[4] = {v0, v1, v2, v3};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e < l1) z[e * a.o.col] = from_f32<O>(v[e]);
+    }
+  };
+  auto store_tall = [&](int row, int64_t j, const vec &v) {  // entries row .. row + 3 of a column
+    O *z = o + row * a.o.row + j * a.o.col;
+    if (a.ovec && row + 4 <= s) {
+      write4(z, (float)v[0], (float)v[1], (float)v[2], (float)v[3]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (row + r < s) z[r * a.o.row] = from_f32<O>((float)v[r]);
+    }
+  };
   for (int64_t base = base0; base < l1; base += 4 * SPAN) {
     if (TT > 1) load(base);
-    if (WIDE) {
+    if (!Q64 && ex) scale();
+    if constexpr (LDS) asm volatile("" ::: "memory");  // Q is read in every round: it would not fit into the registers
+    if constexpr (WIDE && LDS) {
+      // a column of the lane's four at a time, all rows: four instructions' results more would not fit into the registers
+      float y[TT][4][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        vec d[TT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) d[i] = (vec){0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < TT; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const A v = (A)x[k][r][e];
+#pragma unroll
+            for (int i = 0; i < TT; ++i) d[i] = small_multiply(q(i, k, r), v, d[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < TT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[i][r][e] = (float)d[i][r];
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) store_wide(16 * i + 4 * g + r, base + 4 * c, y[i][r][0], y[i][r][1], y[i][r][2], y[i][r][3]);
+    } else if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
-        f32x4 d[4];
+        vec d[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < 4; ++e) d[e] = (vec){0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < TT; ++k)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[i][k][r], x[k][r][e], d[e], 0, 0, 0);
+            for (int e = 0; e < 4; ++e) d[e] = small_multiply(q(i, k, r), (A)x[k][r][e], d[e]);
         if (TT == 1) load(base + 4 * SPAN);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * i + 4 * g + r;
-          if (row >= s) continue;
-          const int64_t j = base + 4 * c;
-          T *z = o + row * a.o.row + j * a.o.col;
-          if (a.ovec && j + 4 <= l1) {
-            write4(z, d[0][r], d[1][r], d[2][r], d[3][r]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (j + e < l1) z[e * a.o.col] = from_f32<T>(d[e][r]);
-          }
-        }
+        for (int r = 0; r < 4; ++r) store_wide(16 * i + 4 * g + r, base + 4 * c, (float)d[0][r], (float)d[1][r], (float)d[2][r], (float)d[3][r]);
       }
     } else {
-      f32x4 d[U][TT];
+      vec d[U][TT];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int i = 0; i < TT; ++i) d[u][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < TT; ++i) d[u][i] = (vec){0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < TT; ++k)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < 4; ++r) {
+            const A v = (A)x[u][k][r];
 #pragma unroll
-            for (int i = 0; i < TT; ++i) d[u][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[i][k][r], x[u][k][r], d[u][i], 0, 0, 0);
+            for (int i = 0; i < TT; ++i) d[u][i] = small_multiply(q(i, k, r), v, d[u][i]);
+          }
       }
       if (TT == 1) load(base + 4 * SPAN);
 #pragma unroll
@@ -468,17 +566,7 @@ __global__ __launch_bounds__(256) void small_apply_kernel(SmallArgs a, Coefs cf)
         const int64_t j = base + 16 * u + c;
         if (j >= l1) continue;
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
-          const int row = 16 * i + 4 * g;
-          T *z = o + row * a.o.row + j * a.o.col;
-          if (a.ovec && row + 4 <= s) {
-            write4(z, d[u][i][0], d[u][i][1], d[u][i][2], d[u][i][3]);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (row + r < s) z[r * a.o.row] = from_f32<T>(d[u][i][r]);
-          }
-        }
+        for (int i = 0; i < TT; ++i) store_tall(16 * i + 4 * g, j, d[u][i]);
       }
     }
   }
@@ -978,6 +1066,8 @@ struct Layout {
   int64_t bytes;
 };
 
+int64_t small_q_bytes(int64_t s) { return s <= 16 ? 0 : (nmfk_div_up(s, 16) * nmfk_div_up(s, 16) * 256 + 32) * 8; }
+
 Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
   Layout y = {};
   y.s = std::min(rows, cols);
@@ -999,7 +1089,7 @@ Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     y.chunk = nmfk_round_up(nmfk_div_up(y.l, y.chunks), 64);
     y.chunks = nmfk_div_up(y.l, y.chunk);
     y.part = take(batch * y.chunks * y.s * y.s * 8);
-    y.q = take(batch * y.s * y.s * 4);
+    y.q = take(batch * small_q_bytes(y.s));
   } else {
     y.lp = nmfk_round_up(y.l, 32);
     y.ldt = nmfk_round_up(y.s, 32) * 4;
@@ -1039,6 +1129,13 @@ double peak(double a, double b, double c, double u, int odd) {
   return best;
 }
 
+// What a step can multiply a singular value of at most u by, and then u itself
+double step_growth(const double *c, double &u) {
+  const double g = std::max(1.0, peak(c[0], c[1], c[2], u, EVEN));
+  u = std::max(peak(c[0], c[1], c[2], u, ODD), TINY);
+  return g;
+}
+
 // the power of two that brings `bound` to at most 2^15: an entry is never larger than the norm, and 65504 stays out of reach
 int exponent(double bound) {
   int e;
@@ -1057,13 +1154,24 @@ void small_launch(const SmallArgs &a, const Coefs &cf, unsigned nb, hipStream_t 
     if (a.chunks > SUMS) small_join_kernel<<<dim3((unsigned)nmfk_div_up((int64_t)a.s * a.s, 256), nb), 256, 0, st>>>(a);
     small_iterate_kernel<TT><<<dim3(nb), 64 * small_waves(TT), BYTES, st>>>(a, cf, a.chunks > SUMS ? 1 : a.chunks);
   }
-  small_apply_kernel<T, TT, WIDE><<<grid, 256, 0, st>>>(a, cf);
+  if (!a.q64) {
+    small_apply_kernel<T, T, float, TT, WIDE><<<grid, 256, 0, st>>>(a, cf);
+    return;
+  }
+  constexpr int Q = TT > 1 ? TT * TT * 2048 : 0;
+  if (TT > 1) {
+    static std::atomic<uint64_t> done{0};
+    nmfk_allow_dynamic_lds((const void *)small_apply_kernel<T, T, double, TT, WIDE>, done, Q);
+  }
+  small_apply_kernel<T, T, double, TT, WIDE><<<grid, 256, Q, st>>>(a, cf);
 }
 
 template <typename T>
 int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, const double *coef, char *work, hipStream_t st) {
   Coefs cf = {};
+  double growth = 1, u = 1;
   for (int k = 0; k < 3 * steps; ++k) cf.v[k] = coef[k];
+  for (int k = 0; k < steps; ++k) growth *= step_growth(coef + 3 * k, u);
   const bool wide = g.col == 1 && g.row != 1;
   for (int64_t b0 = 0; b0 < y.batch; b0 += BATCH) {
     const unsigned nb = (unsigned)std::min<int64_t>(BATCH, y.batch - b0);
@@ -1071,11 +1179,12 @@ int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, 
     a.g = g;
     a.o = o;
     a.part = (double *)(work + y.part) + b0 * y.chunks * y.s * y.s;
-    a.q = (float *)(work + y.q) + b0 * y.s * y.s;
+    a.q = (double *)(work + y.q + b0 * small_q_bytes(y.s));
     a.b0 = b0;
     a.s = (int)y.s;
     a.chunks = (int)y.chunks;
     a.steps = steps;
+    a.q64 = growth > GROWTH32;
     a.l = y.l;
     a.chunk = y.chunk;
     a.gvec = wide || g.row == 1;

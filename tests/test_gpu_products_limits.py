@@ -1,0 +1,122 @@
+"""The matrix operators at the ends of what they accept: many steps and matrices of low rank, extreme norms, every size of tile, views and
+outputs of unusual shape.
+
+Tolerances of orthogonalize with a shorter side s <= 96.  u = 2^-24, e = 2^-53, f(t) = t (a + b t^2 + c t^4) a step on the singular values.
+  S is formed and its polynomials are multiplied in 64 bits: S is off by (l + 2) e, each product of the iteration adds 3 s e, and an error of S
+    reaches O through the derivative of the polynomial Q, at most A^2 for growth A = product of max |a + b t^2 + c t^4|.  4 A^2 e (l + 3 s steps) holds all of it.
+  A growth of up to 512: Q is rounded to fp32 and applied in fp32, |error| <= (s + 3) u (|Q| |X|)[i, j].  Beyond: in 64 bits, and in groups of steps
+    with a growth of up to 2048; between groups X is rounded to fp32, |error|_F <= u |X|_F, and a step takes an error of X to at most L = max |f'| of it
+    (an odd function of a matrix has, in the Frobenius norm, the Lipschitz constant of the function).
+  The result is rounded to fp32 and then to its type."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from test_gpu_products import CF, F8, HALF, P, TINY, TYPES, check_ortho, check_product, check_quantized, randn, ref_ortho, values64  # noqa: F401,E402
+
+pytestmark = pytest.mark.gpu
+
+CONVERGING = (1.875, -1.25, 0.375)
+U, E = 2.0 ** -24, 2.0 ** -53
+
+
+def step_bounds(cf, u):
+    """growth, Lipschitz constant and largest singular value after a step on singular values up to u"""
+    a, b, c = cf
+    t = np.linspace(0.0, u, 100001)
+    return (max(1.0, np.abs(a + b * t ** 2 + c * t ** 4).max()), np.abs(a + 3 * b * t ** 2 + 5 * c * t ** 4).max() * 1.0001,
+            np.abs(a * t + b * t ** 3 + c * t ** 5).max() * 1.0001)
+
+
+def short_reference(x, cf):
+    """O of one matrix with rows <= columns in 64 bits, a bound of its entries' errors before the result is rounded, and the largest singular value"""
+    s, l = x.shape
+    n = torch.linalg.matrix_norm(x.double())
+    x0 = y = torch.where(n > 0, x.double() / n, 0.0)
+    q = torch.eye(s, dtype=torch.float64, device=x.device)
+    u = growth = whole = 1.0
+    tol = steps = 0
+    for a, b, c in cf:
+        g, lip, u_next = step_bounds((a, b, c), u)
+        if steps and growth * g > 2048:
+            tol += 4 * growth ** 2 * E * (l + 3 * s * steps) + U * float(y.norm())
+            growth, steps = 1.0, 0
+        growth, whole, steps, u = growth * g, whole * g, steps + 1, u_next
+        sq = y @ y.t()
+        p = b * sq + c * (sq @ sq)
+        y, q = a * y + p @ y, a * q + p @ q
+        tol = tol * lip
+    tol += 4 * growth ** 2 * E * (l + 3 * s * steps)
+    if whole <= 512:
+        tol = tol + (s + 3) * U * (q.abs() @ x0.abs())
+    return y, tol, u
+
+
+def check_short(o, g, cf):
+    assert o.shape == g.shape and o.dtype == g.dtype
+    for x, y in zip(g.reshape(-1, *g.shape[-2:]), o.reshape(-1, *o.shape[-2:])):
+        if x.shape[0] > x.shape[1]:
+            x, y = x.t(), y.t()
+        want, tol, top = short_reference(x, cf)
+        assert bool(torch.isfinite(y).all())
+        h = HALF[g.dtype]
+        err = (y.double() - want).abs()
+        bound = tol + (want.abs() + tol) * (U + h) * (1 + h) + TINY[g.dtype]
+        assert bool((err <= bound).all()), f"largest error {float(err.max())}, largest error / tolerance {float((err / bound).max())}"
+        assert float(torch.linalg.eigvalsh((y.double() @ y.double().t()).cpu())[-1]) ** 0.5 <= top * (1 + 8 * (h + U) * min(x.shape) ** 0.5)
+
+
+def spectrum(name, s, l, seed=3):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *shape: torch.randn(*shape, generator=gen, dtype=torch.float64)
+    if name == "rows twice":
+        x = r(s, l)
+        x = torch.cat([x[: (s + 1) // 2], x[: s // 2]])
+    elif name == "low rank":
+        k = max(1, s // 4)
+        x = r(s, k) @ r(k, l)
+    elif name == "ones":
+        x = torch.ones(s, l, dtype=torch.float64)
+    elif name == "binary":
+        x = (torch.rand(s, 3, generator=gen) < 0.5).double() @ (torch.rand(3, l, generator=gen) < 0.5).double()
+    elif name == "sizes":  # rows of very different size
+        x = r(s, l) * torch.exp(2 * r(s, 1))
+    else:  # condition
+        q, w = torch.linalg.qr(r(s, s))[0], torch.linalg.qr(r(l, s))[0]
+        x = (q * torch.logspace(0, -np.log10(float(name)), s, dtype=torch.float64)) @ w.t()
+    return x.float().cuda()
+
+
+SPECTRA = ["rows twice", "low rank", "ones", "binary", "sizes", "1e3", "1e6"]
+
+
+# ---- orthogonalize, shorter side up to 96: its factor in 64 bits -------------------------------------------------------------------
+
+@pytest.mark.parametrize("name", SPECTRA)
+@pytest.mark.parametrize("s,l", [(2, 9), (16, 200), (17, 40), (40, 60), (48, 700), (64, 64), (65, 300), (80, 81), (96, 130)])
+def test_short_side(P, name, s, l):
+    for k in (1, 5, 6):
+        g = spectrum(name, s, l)
+        check_short(P.orthogonalize(g, steps=k), g, [CF] * k)
+        g = g.t().contiguous()
+        check_short(P.orthogonalize(g, steps=k), g, [CF] * k)
+    for t in (torch.bfloat16, torch.float16):
+        g = (spectrum(name, s, l) / 8).to(t)
+        check_short(P.orthogonalize(g, steps=6), g, [CF] * 6)
+
+
+@pytest.mark.parametrize("s", [1, 2, 16, 40, 90])
+@pytest.mark.parametrize("size", [1e-36, 1e-39, 3e-45, 1e36, 3e38])
+def test_short_side_of_any_norm(P, s, size):
+    """matrices of low rank: null directions grow to 485 / |G|, which fp32 does not hold"""
+    x = torch.zeros(s, 2 * s, device="cuda")
+    x[0, 0] = size
+    x[s // 2, 3 % (2 * s)] = size / 2
+    check_short(P.orthogonalize(x), x, [CF] * 5)
+    check_short(P.orthogonalize(x.t().contiguous()), x.t(), [CF] * 5)
+    b = x.bfloat16()
+    check_short(P.orthogonalize(b), b, [CF] * 5)
+    g = spectrum("low rank", s, 3 * s)
+    g = g / g.abs().max() * size
+    check_short(P.orthogonalize(g), g, [CF] * 5)
+    check_short(P.orthogonalize(g, steps=6), g, [CF] * 6)
