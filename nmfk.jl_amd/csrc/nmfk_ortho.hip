@@ -5,10 +5,14 @@
 // which drives every singular value of X towards one and leaves its singular vectors.  Small singular values grow by a in each step, so
 // does a rounding error made early: everything is carried to 32-bit accuracy or better.
 //
-//   s <= 96: the polynomials of all steps are polynomials of the first S.  One pass over G makes S in 64 bits, one workgroup per matrix
+//   s <= 96: the polynomials of several steps are polynomials of their first S.  One pass over X makes S in 64 bits, one workgroup per matrix
 //     iterates on s x s matrices in LDS in 64 bits (S <- P S P, Q <- Q P), a second pass applies Q.  Two reads and a write of G.  (Five steps on
 //     90 x 20000: 133 us, the other form 194; 60 of 96 x 3000: 245 and 488; one of 96 x 96, where the iteration is all there is: 118 and 105.
 //     Beyond, three matrices do not fit into LDS.)
+//     What is iterated is not X: a rounding error e = 2^-53 in an eigenvalue of S near zero, which may make it negative, grows by growth^2 (growth: the
+//     product of the steps' largest a + b S + c S S), and from some 1e-2 on it takes over -- where rows of G depend on each other, the default steps leave
+//     the right place after 12 steps and every bound after 16.  So the steps are taken in groups of growth up to 2048 (5e-10), X is formed after
+//     each (in fp32: in O, or for 16-bit types in the workspace, some matrices at a time), and the next group starts from the S of that X.
 //   s > 96: products on the 16-bit matrix pipes.  An entry x is kept as two fp16 numbers, hi + lo (22 significant bits), scaled by a power of
 //     two that the growth bound of the step allows; a product is hi hi + hi lo + lo hi, summed in 32 bits (what is dropped is 2^-22 of it).
 #include <type_traits>
@@ -21,6 +25,8 @@ namespace {
 
 constexpr int SMALL = 96;
 constexpr double GROWTH32 = 512;  // up to which s <= 96 applies its factor in 32 bits: five of the default steps, 3e-5 of |G| in the directions that grow so
+constexpr double GROWTH = 2048;   // ... and up to which one factor holds: six of the default steps
+constexpr int64_t PORTION = (int64_t)1 << 26;  // bytes of X between the factors of 16-bit matrices
 constexpr int64_t BATCH = 32768;  // matrices a launch
 constexpr double TINY = 1e-20;    // bounds below it are not followed any further
 
@@ -44,8 +50,8 @@ struct SmallArgs {
   Strided g, o;
   double *part;  // [batch][chunks][s][s]
   double *q;     // s > 16, [batch][small_q_size]: Q / |G| in the order in which small_apply_kernel takes it, then the exponent left out of it
-  int64_t b0;
   int s, chunks, steps;
+  int first;         // X is G / |G|; otherwise it is taken as it is
   int q64;           // Q is applied in 64 bits
   int64_t l, chunk;  // entries of l per workgroup
   int gvec, ovec;    // the side that is walked is contiguous: four entries at once
@@ -74,7 +80,7 @@ __device__ __forceinline__ void small_load4(const Strided &g, const T *p, int s,
 template <typename T, int TT, bool WIDE>
 __global__ __launch_bounds__(256) void small_gram_kernel(SmallArgs a) {
   __shared__ double sum[4][256];
-  const int64_t b = a.b0 + blockIdx.y;
+  const int64_t b = blockIdx.y;
   const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
   const int s = a.s, t = threadIdx.x, w = t >> 6, lane = t & 63, c = lane & 15, g = lane >> 4;
   const int packed = TT == 1 ? max(1, 16 / s) : 1, grp = TT == 1 ? c / s : 0, row = TT == 1 ? c - grp * s : c;
@@ -194,8 +200,12 @@ __global__ __launch_bounds__(256) void small_gram_kernel(SmallArgs a) {
     }
 }
 
-// 1 / |G|^2 and 1 / |G| as the iteration uses them: 0 for a matrix of zeros, NaN for one that is not finite
-__device__ __forceinline__ void small_norm(double norm2, double &inv2, double &inv) {
+// 1 / |G|^2 and 1 / |G| as the iteration uses them: 0 for a matrix of zeros, NaN for one that is not finite; 1 behind the first group of steps
+__device__ __forceinline__ void small_norm(double &norm2, int first, double &inv2, double &inv) {
+  if (!first) {
+    norm2 = inv2 = inv = 1.0;
+    return;
+  }
   const double nan = __longlong_as_double(0x7ff8000000000000ll);
   const bool finite = norm2 <= 1.7e308;
   inv2 = !finite ? nan : norm2 > 0 ? 1.0 / norm2 : 0.0;
@@ -304,7 +314,7 @@ __global__ __launch_bounds__(64 * small_waves(TT)) void small_iterate_kernel(Sma
 #pragma unroll
   for (int o = 32; o; o >>= 1) norm2 += __shfl_xor(norm2, o);
   double inv2, inv;
-  small_norm(norm2, inv2, inv);
+  small_norm(norm2, a.first, inv2, inv);
   __syncthreads();
 #pragma unroll
   for (int o = 0; o < OWN; ++o) sv[o] *= inv2;
@@ -375,11 +385,10 @@ __global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(Small
   __shared__ int exponent;
   extern __shared__ __attribute__((aligned(16))) double qs[];  // LDS: the operands of Q as in memory
   const int by = gridDim.y - 1 - blockIdx.y;  // the matrices read last are still in the last-level cache: take them first
-  const int64_t b = a.b0 + by;
   const int64_t l0 = blockIdx.x * a.chunk, l1 = min(a.l, l0 + a.chunk);
   const int s = a.s, t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 15, g = lane >> 4;
-  const T *p = (const T *)a.g.p + b * a.g.batch;
-  O *o = (O *)a.o.p + b * a.o.batch;
+  const T *p = (const T *)a.g.p + by * a.g.batch;
+  O *o = (O *)a.o.p + by * a.o.batch;
   constexpr int U = WIDE ? 4 : TT == 1 ? 4 : TT == 2 ? 2 : 1, SPAN = 16 * U;  // columns a wave takes at a time
   float x[WIDE ? TT : U][WIDE ? 4 : TT][4];
   auto load = [&](int64_t base) {
@@ -427,7 +436,7 @@ __global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(Small
       for (int r = 0; r < 4; ++r) S[r] = sum[(4 * r + g) * 16 + c];
 #pragma unroll
       for (int i = 0; i < 16; ++i) norm2 += sum[i * 17];
-      small_norm(norm2, inv2, inv);
+      small_norm(norm2, a.first, inv2, inv);
       S *= inv2;
       for (int k = 0; k < a.steps; ++k) {
         P = cf.v[3 * k + 1] * S + cf.v[3 * k + 2] * sym_product(S, S);
@@ -1060,7 +1069,7 @@ int full_side(int64_t m, int64_t n, int64_t batch, int64_t kb) {
 
 struct Layout {
   int64_t s, l, batch;
-  int64_t chunks, chunk;                // small
+  int64_t chunks, chunk, portion, x;    // small; portion: matrices of 16 bits that more than one group of steps works on at a time
   int64_t xt[2], sq[2], norm, part, q;  // byte offsets
   int64_t ldt, lp;
   int64_t bytes;
@@ -1090,6 +1099,8 @@ Layout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     y.chunks = nmfk_div_up(y.l, y.chunk);
     y.part = take(batch * y.chunks * y.s * y.s * 8);
     y.q = take(batch * small_q_bytes(y.s));
+    y.portion = std::max<int64_t>(1, std::min(BATCH, PORTION / (4 * y.s * y.l)));
+    y.x = take(4 * y.s * y.l * std::min(y.portion, batch));
   } else {
     y.lp = nmfk_round_up(y.l, 32);
     y.ldt = nmfk_round_up(y.s, 32) * 4;
@@ -1143,7 +1154,7 @@ int exponent(double bound) {
   return std::min(15 - e, 100);
 }
 
-template <typename T, int TT, bool WIDE>
+template <typename T, typename O, int TT, bool WIDE>
 void small_launch(const SmallArgs &a, const Coefs &cf, unsigned nb, hipStream_t st) {
   const dim3 grid((unsigned)a.chunks, nb);
   small_gram_kernel<T, TT, WIDE><<<grid, 256, 0, st>>>(a);
@@ -1154,55 +1165,86 @@ void small_launch(const SmallArgs &a, const Coefs &cf, unsigned nb, hipStream_t 
     if (a.chunks > SUMS) small_join_kernel<<<dim3((unsigned)nmfk_div_up((int64_t)a.s * a.s, 256), nb), 256, 0, st>>>(a);
     small_iterate_kernel<TT><<<dim3(nb), 64 * small_waves(TT), BYTES, st>>>(a, cf, a.chunks > SUMS ? 1 : a.chunks);
   }
-  if (!a.q64) {
-    small_apply_kernel<T, T, float, TT, WIDE><<<grid, 256, 0, st>>>(a, cf);
-    return;
-  }
+  if constexpr (std::is_same<T, O>::value)
+    if (!a.q64) {
+      small_apply_kernel<T, O, float, TT, WIDE><<<grid, 256, 0, st>>>(a, cf);
+      return;
+    }
   constexpr int Q = TT > 1 ? TT * TT * 2048 : 0;
   if (TT > 1) {
     static std::atomic<uint64_t> done{0};
-    nmfk_allow_dynamic_lds((const void *)small_apply_kernel<T, T, double, TT, WIDE>, done, Q);
+    nmfk_allow_dynamic_lds((const void *)small_apply_kernel<T, O, double, TT, WIDE>, done, Q);
   }
-  small_apply_kernel<T, T, double, TT, WIDE><<<grid, 256, Q, st>>>(a, cf);
+  small_apply_kernel<T, O, double, TT, WIDE><<<grid, 256, Q, st>>>(a, cf);
+}
+
+// one group of steps on nb matrices: O = Q G
+template <typename T, typename O>
+void small_group(SmallArgs a, const Strided &g, const Strided &o, int steps, const double *coef, unsigned nb, hipStream_t st) {
+  Coefs cf = {};
+  for (int k = 0; k < 3 * steps; ++k) cf.v[k] = coef[k];
+  const bool wide = g.col == 1 && g.row != 1;
+  a.g = g;
+  a.o = o;
+  a.steps = steps;
+  a.gvec = wide || g.row == 1;
+  a.ovec = (wide ? o.col : o.row) == 1;
+#define NMFK_SMALL(TT) (wide ? small_launch<T, O, TT, true>(a, cf, nb, st) : small_launch<T, O, TT, false>(a, cf, nb, st))
+  if (a.s <= 16)
+    NMFK_SMALL(1);
+  else if (a.s <= 32)
+    NMFK_SMALL(2);
+  else if (a.s <= 48)
+    NMFK_SMALL(3);
+  else if (a.s <= 64)
+    NMFK_SMALL(4);
+  else if (a.s <= 80)
+    NMFK_SMALL(5);
+  else
+    NMFK_SMALL(6);
+#undef NMFK_SMALL
 }
 
 template <typename T>
 int ortho_small(const Layout &y, const Strided &g, const Strided &o, int steps, const double *coef, char *work, hipStream_t st) {
-  Coefs cf = {};
+  constexpr bool F32 = std::is_same<T, float>::value;
+  int end[32], groups = 0;
   double growth = 1, u = 1;
-  for (int k = 0; k < 3 * steps; ++k) cf.v[k] = coef[k];
-  for (int k = 0; k < steps; ++k) growth *= step_growth(coef + 3 * k, u);
-  const bool wide = g.col == 1 && g.row != 1;
-  for (int64_t b0 = 0; b0 < y.batch; b0 += BATCH) {
-    const unsigned nb = (unsigned)std::min<int64_t>(BATCH, y.batch - b0);
+  for (int k = 0; k < steps; ++k) {
+    const double by = step_growth(coef + 3 * k, u);
+    if (k > (groups ? end[groups - 1] : 0) && growth * by > GROWTH) {
+      end[groups++] = k;
+      growth = 1;
+    }
+    growth *= by;
+  }
+  end[groups++] = steps;
+  const int64_t most = groups > 1 && !F32 ? y.portion : BATCH;
+  for (int64_t b0 = 0; b0 < y.batch; b0 += most) {
+    const unsigned nb = (unsigned)std::min<int64_t>(most, y.batch - b0);
     SmallArgs a = {};
-    a.g = g;
-    a.o = o;
     a.part = (double *)(work + y.part) + b0 * y.chunks * y.s * y.s;
     a.q = (double *)(work + y.q + b0 * small_q_bytes(y.s));
-    a.b0 = b0;
     a.s = (int)y.s;
     a.chunks = (int)y.chunks;
-    a.steps = steps;
-    a.q64 = growth > GROWTH32;
     a.l = y.l;
     a.chunk = y.chunk;
-    a.gvec = wide || g.row == 1;
-    a.ovec = (wide ? o.col : o.row) == 1;
-#define NMFK_SMALL(TT) (wide ? small_launch<T, TT, true>(a, cf, nb, st) : small_launch<T, TT, false>(a, cf, nb, st))
-    if (y.s <= 16)
-      NMFK_SMALL(1);
-    else if (y.s <= 32)
-      NMFK_SMALL(2);
-    else if (y.s <= 48)
-      NMFK_SMALL(3);
-    else if (y.s <= 64)
-      NMFK_SMALL(4);
-    else if (y.s <= 80)
-      NMFK_SMALL(5);
-    else
-      NMFK_SMALL(6);
-#undef NMFK_SMALL
+    a.first = 1;
+    a.q64 = groups > 1 || growth > GROWTH32;
+    Strided from = g, to = o;
+    from.p += b0 * g.batch * (int64_t)sizeof(T);
+    to.p += b0 * o.batch * (int64_t)sizeof(T);
+    if (groups == 1) {
+      small_group<T, T>(a, from, to, steps, coef, nb, st);
+      continue;
+    }
+    // between the groups X is O itself, or stands in the workspace along the side that is contiguous in G
+    Strided x = to;
+    if (!F32) x = g.col == 1 && g.row != 1 ? Strided{work + y.x, y.s * y.l, y.l, 1} : Strided{work + y.x, y.s * y.l, 1, y.s};
+    small_group<T, float>(a, from, x, end[0], coef, nb, st);
+    a.first = 0;
+    for (int k = 1; k + 1 < groups; ++k) small_group<float, float>(a, x, x, end[k] - end[k - 1], coef + 3 * end[k - 1], nb, st);
+    small_group<float, T>(a, x, to, steps - end[groups - 2], coef + 3 * end[groups - 2], nb, st);
   }
   return nmfk_launched("nmfk_orthogonalize");
 }

@@ -120,3 +120,116 @@ def test_short_side_of_any_norm(P, s, size):
     g = g / g.abs().max() * size
     check_short(P.orthogonalize(g), g, [CF] * 5)
     check_short(P.orthogonalize(g, steps=6), g, [CF] * 6)
+
+
+# ---- orthogonalize, shorter side up to 96: many steps ----------------------------------------------------------------------------------
+
+STEPS = {"7": [CF] * 7, "10": [CF] * 10, "14": [CF] * 14, "20": [CF] * 20, "32": [CF] * 32, "10 + 4": [CF] * 10 + [CONVERGING] * 4, "steep": [(100.0, -200.0, 101.0), (1 / 32, 0.0, 0.0)] + [CF] * 5,
+         "24": [CF] * 8 + [CONVERGING] * 16}
+
+
+@pytest.mark.parametrize("name", SPECTRA)
+@pytest.mark.parametrize("steps", list(STEPS))
+@pytest.mark.parametrize("s,l", [(1, 5), (16, 200), (40, 60), (64, 70), (90, 300), (96, 96)])
+def test_many_steps(P, name, steps, s, l):
+    cf = STEPS[steps]
+    g = spectrum(name, s, l)
+    check_short(P.orthogonalize(g, len(cf), cf), g, cf)
+    g = g.t().contiguous()
+    check_short(P.orthogonalize(g, len(cf), cf), g, cf)
+    for t in (torch.bfloat16, torch.float16):
+        h = (g / 8).to(t)
+        check_short(P.orthogonalize(h, len(cf), cf), h, cf)
+
+
+@pytest.mark.parametrize("s,l", [(12, 3000), (40, 60), (72, 900), (96, 130)])
+@pytest.mark.parametrize("name", ["sizes", "1e2", "1e3", "1e4"])
+def test_many_steps_to_orthonormal(P, name, s, l):
+    """ten default steps bring singular values from 2e-5 of the norm up, four that converge make the rows orthonormal: entries off by u of themselves
+    give 2 u, what is left of the iteration and the 64 bits less than that"""
+    g = spectrum(name, s, l)
+    cf = [CF] * 10 + [CONVERGING] * 4
+    o = P.orthogonalize(g, len(cf), cf).double()
+    assert float((o @ o.t() - torch.eye(s, device="cuda")).abs().max()) <= 4 * U
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("shape", [(3, 20, 70), (2, 300, 40), (5, 96, 100), (260, 30, 64)])
+def test_many_steps_in_place_and_strided(P, t, shape):
+    cf = [CF] * 10 + [CONVERGING] * 4
+    g = randn(31, *shape, t=TYPES[t])
+    want = P.orthogonalize(g, len(cf), cf)
+    check_short(want[-2:], g[-2:], cf)
+    assert torch.equal(want, P.orthogonalize(g, len(cf), cf))
+    out = torch.full((shape[0], shape[1] + 3, 2 * shape[2] + 5), 7.0, device="cuda", dtype=TYPES[t])
+    view = out[:, 2:-1, 1:-4:2]
+    P.orthogonalize(g, len(cf), cf, out=view)
+    check_short(view[-2:], g[-2:], cf)
+    view.fill_(7.0)
+    assert bool((out == 7.0).all())
+    inplace = g.clone()
+    P.orthogonalize(inplace, len(cf), cf, out=inplace)
+    assert torch.equal(inplace, want)
+    turned = g.mT.contiguous().mT
+    P.orthogonalize(turned, len(cf), cf, out=turned)
+    check_short(turned[-2:], g[-2:], cf)
+
+
+def test_many_steps_of_zeros_and_of_what_is_not_finite(P):
+    for s in (3, 30, 90):
+        for t in TYPES.values():
+            g = randn(32, 5, s, 2 * s, t=t)
+            g[1], g[2, 1, 2], g[3, 0, 0] = 0, float("nan"), float("-inf")
+            o = P.orthogonalize(g, steps=20)
+            assert bool((o[1] == 0).all()) and bool(torch.isnan(o[2]).all()) and bool(torch.isnan(o[3]).all())
+            check_short(o[[0, 4]], g[[0, 4]], [CF] * 20)
+
+
+def test_many_steps_of_large_stacks(P):
+    """more than one launch of matrices, and more than one portion of a 16-bit stack"""
+    for shape, t in (((40000, 3, 7), torch.float32), ((40000, 3, 7), torch.bfloat16), ((400, 90, 1000), torch.bfloat16), ((3, 60, 300000), torch.float16)):
+        g = torch.randn(*shape, device="cuda").to(t)
+        o = P.orthogonalize(g, steps=8)
+        pick = sorted({0, 1, shape[0] // 2, shape[0] - 2, shape[0] - 1, min(32768, shape[0] - 1)})
+        check_short(o[pick], g[pick], [CF] * 8)
+        assert bool(torch.isfinite(o).all())
+
+
+def test_many_steps_in_a_graph(P):
+    g, h = randn(33, 4, 50, 90), randn(34, 2, 700, 16, t=torch.bfloat16)
+    run = lambda: (P.orthogonalize(g, steps=12), P.orthogonalize(h, steps=12))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    cg = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(cg):
+        out = run()
+    for rep in range(4):
+        for v in (g, h):
+            v.copy_(torch.roll(v, 1, 0) * 1.25)
+        want = run()
+        for o in out:
+            o.zero_()
+        cg.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(out, want))
+
+
+@pytest.mark.parametrize("kind", ["ones", "binary"])
+def test_rangebasis_of_low_rank(P, kind):
+    """a sketch of low rank: the singular values that X has come out, and their directions are orthonormal"""
+    gen = torch.Generator().manual_seed(5)
+    n, m, k = 600, 300, 4
+    rank = 1 if kind == "ones" else 3
+    X = torch.ones(n, m) if kind == "ones" else (torch.rand(n, 3, generator=gen) < 0.5).float() @ (torch.rand(3, m, generator=gen) < 0.5).float()
+    want = torch.linalg.svdvals(X.double())
+    Q, B, sigma = P.rangebasis(X.cuda(), k)
+    # small whole numbers are exact in 8 bits up to the rounding of x / scale: 2^-4 of themselves at most, at random
+    noise = 2.0 ** -4 * float(X.norm()) / m ** 0.5
+    assert float((sigma.cpu().double() - want[:k]).abs().max()) <= noise
+    lead = Q[:, :rank].double()
+    assert float((lead.t() @ lead - torch.eye(rank, device="cuda")).abs().max()) <= 1e-5
+    assert float(torch.linalg.matrix_norm(Q.double(), 2)) <= 1 + 1e-5
+    assert float((Q.double() @ B.double() - X.cuda().double()).norm()) <= noise * k ** 0.5
