@@ -6,6 +6,7 @@ The operators take and return torch tensors on the GPU; they run on torch's curr
 captured into a graph (a Quantized matrix used on another stream than its own needs what a tensor needs there: the streams ordered, the object kept).  `rangebasis` takes a numpy array like `execute` does, or a tensor."""
 import ctypes as C
 import functools
+import math
 
 import numpy as np
 
@@ -250,6 +251,9 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
         key = tuple(cf.tolist()) if cf.ndim == 1 else tuple(map(tuple, cf.tolist())) if cf.ndim == 2 else ()
     cf, cf_at = _coefficients(key, steps)
     if out is None:
+        if G.dim() > 3:
+            g = G.reshape(math.prod(G.shape[:-2]), *G.shape[-2:])  # (a copy where the leading dimensions do not fold into one)
+            return orthogonalize(g, steps, coefficients).view(G.shape)
         out = torch.empty_like(G)
     else:
         _tensor(out, "out", ndim=0)
@@ -268,10 +272,10 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
     else:
         if G.dim() > 3:
             try:
-                o = out.view(-1, *out.shape[-2:])
+                o = out.view(math.prod(out.shape[:-2]), *out.shape[-2:])
             except RuntimeError:
                 raise _bad("the leading dimensions of out must fold into one") from None
-            g = o if out.data_ptr() == G.data_ptr() else G.reshape(-1, *G.shape[-2:])
+            g = o if out.data_ptr() == G.data_ptr() else G.reshape(o.shape)
         b, r, c = g.shape
         gs, os = g.stride(), o.stride()
     dev, nb = G.device, _orthogonalize_workspace(b, r, c)

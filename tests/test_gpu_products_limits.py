@@ -233,3 +233,22 @@ def test_rangebasis_of_low_rank(P, kind):
     assert float((lead.t() @ lead - torch.eye(rank, device="cuda")).abs().max()) <= 1e-5
     assert float(torch.linalg.matrix_norm(Q.double(), 2)) <= 1 + 1e-5
     assert float((Q.double() @ B.double() - X.cuda().double()).norm()) <= noise * k ** 0.5
+
+
+# ---- views and outputs of unusual shape -------------------------------------------------------------------------------------------------
+
+def test_orthogonalize_stacks_whose_leading_dimensions_do_not_fold(P):
+    for s, l in ((20, 40), (100, 130)):
+        g = randn(41, 2, 3, s, l).permute(1, 0, 2, 3)
+        o = P.orthogonalize(g)
+        assert o.shape == g.shape
+        check_ortho(o, g)
+        g = randn(42, 2, 3, 2, l, s).permute(2, 0, 1, 4, 3)
+        check_ortho(P.orthogonalize(g), g)
+        with pytest.raises(P.NMFkError, match="fold"):
+            P.orthogonalize(g, out=torch.empty_like(g))
+    g = randn(43, 2, 3, 5, 7)
+    assert P.orthogonalize(g).stride() == g.stride() and P.orthogonalize(g.mT).stride() == g.mT.stride()
+    for shape in ((2, 3, 0, 5), (0, 2, 3, 5), (2, 0, 4, 4)):
+        e = torch.empty(shape, device="cuda")
+        assert P.orthogonalize(e).shape == shape and P.orthogonalize(e, out=torch.empty_like(e)).shape == shape
