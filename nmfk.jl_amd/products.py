@@ -146,6 +146,8 @@ class Quantized:
 def _contiguous_side(X):
     """X and its strides: as it is if its rows or its columns are contiguous, else a copy"""
     (r, c), (sr, sc) = X.shape, X.stride()
+    if r == c == 1:  # (contiguous to torch whatever its strides)
+        return X, 1, 1
     if not (sc == 1 and (sr >= c or r == 1)) and not (sr == 1 and (sc >= r or c == 1)):
         X = X.contiguous()
         sr, sc = X.stride()

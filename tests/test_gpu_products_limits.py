@@ -252,3 +252,20 @@ def test_orthogonalize_stacks_whose_leading_dimensions_do_not_fold(P):
     for shape in ((2, 3, 0, 5), (0, 2, 3, 5), (2, 0, 4, 4)):
         e = torch.empty(shape, device="cuda")
         assert P.orthogonalize(e).shape == shape and P.orthogonalize(e, out=torch.empty_like(e)).shape == shape
+
+
+
+
+# ---- quantize, views of one entry ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_quantize_one_entry_of_a_larger_matrix(P, tiles):
+    x = randn(44, 5, 9)
+    for v in (x[2:3, 4:5], x[:1, ::3][:, :1], x.t()[3:4, ::5][:, :1], x[:1, 1:2].expand(1, 1), x[::5, ::9]):
+        q, w = P.quantize(v, tiles=tiles, both=True)
+        check_quantized(q, v, tiles)
+        check_quantized(w, v.t(), tiles)
+        check_quantized(P.quantize(v, tiles=tiles), v, tiles)
+    v = x[::5, ::9]
+    da, db = P.product_grads(v, P.quantize(randn(47, 30, 1)), P.quantize(randn(48, 30, 1)))
+    assert da.shape == db.shape == (1, 30)
