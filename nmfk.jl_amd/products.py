@@ -47,6 +47,13 @@ def _tensor(x, name, ndim=2):
         raise _bad(f"{name} must be a matrix")
     if x.requires_grad and torch.is_grad_enabled():
         raise _bad(f"{name} requires a gradient, which this operator does not record: pass {name}.detach()")
+    return x.resolve_neg()  # (itself, unless its entries are the negative of what its memory holds)
+
+
+def _output(x, ndim=2):
+    _tensor(x, "out", ndim)
+    if x.is_neg():
+        raise _bad("out must not be a view with a pending negation")
     return x
 
 
@@ -159,7 +166,7 @@ def quantize(X, tiles=False, both=False):
     128 x 128 tile.  scale = max(max |x| / 448, 2^-126) over the block's finite entries, value = x / scale rounded to e4m3, ties to even; an
     entry that is not finite becomes NaN and leaves its block alone.
     both=True: a pair, X and its transpose (blocks along ITS rows), from one pass over X."""
-    _tensor(X, "X")
+    X = _tensor(X, "X")
     r, c = X.shape
     X, sr, sc = _contiguous_side(X)
     dev, tiles = X.device, bool(tiles)
@@ -193,7 +200,7 @@ def product(A, B, dtype=None, out=None):
             raise _bad(f"dtype must be float32, bfloat16 or float16, not {dtype}")
         out = torch.empty((m, n), dtype=dtype, device=dev)
     else:
-        _tensor(out, "out")
+        _output(out)
         if tuple(out.shape) != (m, n) or out.device != dev or (dtype is not None and out.dtype != dtype) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
             raise _bad(f"out must be {m} x {n} on {dev} with contiguous rows")
     t = _TYPES[out.dtype]
@@ -209,7 +216,7 @@ def product_grads(dY, At, Bt, dtype=None):
     rows; At and Bt are the Quantized transposes of A and of B (quantize(..., both=True) leaves them beside the forward's).  The gradients are
     those with respect to the matrices that the 8 bits stand for."""
     torch = _torch()
-    _tensor(dY, "dY")
+    dY = _tensor(dY, "dY")
     _quantized(At, "At")
     _quantized(Bt, "Bt")
     m, n = dY.shape
@@ -240,7 +247,7 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
     for orthonormal rows or columns add steps with (1.875, -1.25, 0.375).  Sums in 32 bits or more, one rounding to G's type.
     Zeros give zeros, an entry that is not finite gives NaN in its matrix.  out: where to write, G itself or apart from it."""
     torch = _torch()
-    _tensor(G, "G", ndim=0)
+    G = _tensor(G, "G", ndim=0)
     if G.dim() < 2:
         raise _bad("G must be a matrix or a stack of matrices")
     steps = int(steps)
@@ -258,7 +265,7 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
             return orthogonalize(g, steps, coefficients).view(G.shape)
         out = torch.empty_like(G)
     else:
-        _tensor(out, "out", ndim=0)
+        _output(out, ndim=0)
         if out.shape != G.shape or out.dtype != G.dtype or out.device != G.device:
             raise _bad("out must have G's shape, type and GPU")
         if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
@@ -303,7 +310,7 @@ def rangebasis(X, k, oversample=8, iterations=2, seed=0, device=None):
         if _lib.device_count() == 0:
             raise NMFkError(_lib.ERR_NO_DEVICE, "no usable gfx950 device: the library has no CPU fallback")
         X = torch.from_numpy(np.ascontiguousarray(X, dtype=np.float32)).to(torch.device("cuda", int(device or 0)))
-    _tensor(X, "X")
+    X = _tensor(X, "X")
     n, m = X.shape
     k = int(k)
     if not 1 <= k <= min(n, m):

@@ -269,3 +269,23 @@ def test_quantize_one_entry_of_a_larger_matrix(P, tiles):
     v = x[::5, ::9]
     da, db = P.product_grads(v, P.quantize(randn(47, 30, 1)), P.quantize(randn(48, 30, 1)))
     assert da.shape == db.shape == (1, 30)
+
+
+# ---- tensors that stand for something else than their memory ------------------------------------------------------------------------------
+
+def test_views_with_a_pending_negation(P):
+    """the imaginary part of a conjugate: torch keeps the sign apart from the memory"""
+    z = torch.complex(randn(51, 40, 300), randn(52, 40, 300))
+    v = z.conj().imag
+    assert v.is_neg()
+    plain = v.clone()
+    assert not plain.is_neg()
+    for tiles in (False, True):
+        check_quantized(P.quantize(v, tiles=tiles), plain, tiles)
+    assert torch.equal(P.orthogonalize(v), P.orthogonalize(plain))
+    at, bt = P.quantize(randn(53, 20, 40)), P.quantize(randn(54, 20, 300))
+    for got, want in zip(P.product_grads(v, at, bt), P.product_grads(plain, at, bt)):
+        assert torch.equal(got, want)
+    for f in (lambda: P.orthogonalize(plain, out=v), lambda: P.orthogonalize(v, out=v), lambda: P.product(P.quantize(randn(55, 40, 64)), P.quantize(randn(56, 300, 64)), out=v)):
+        with pytest.raises(P.NMFkError, match="negat"):
+            f()
