@@ -289,3 +289,19 @@ def test_views_with_a_pending_negation(P):
     for f in (lambda: P.orthogonalize(plain, out=v), lambda: P.orthogonalize(v, out=v), lambda: P.product(P.quantize(randn(55, 40, 64)), P.quantize(randn(56, 300, 64)), out=v)):
         with pytest.raises(P.NMFkError, match="negat"):
             f()
+
+
+def test_forward_mode_tangents_are_refused(P):
+    """no operator records a tangent: it must not vanish without a word"""
+    import torch.autograd.forward_ad as fwAD
+
+    x, w = randn(57, 6, 8), P.quantize(randn(58, 5, 8))
+    at, bt = P.quantize(randn(59, 4, 6)), P.quantize(randn(60, 4, 8))
+    with fwAD.dual_level():
+        d = fwAD.make_dual(x, torch.ones_like(x))
+        for f in (lambda: P.quantize(d), lambda: P.orthogonalize(d), lambda: P.product_grads(d, at, bt), lambda: P.rangebasis(d, 2),
+                  lambda: P.orthogonalize(x, out=d), lambda: P.product(P.quantize(x), P.quantize(randn(61, 8, 8)), out=d)):
+            with pytest.raises(P.NMFkError, match="tangent"):
+                f()
+        P.quantize(x), P.orthogonalize(x)  # a tensor without one is taken inside a level, too
+        P.quantize(fwAD.unpack_dual(d).primal)
