@@ -117,6 +117,8 @@ class Quantized:
             raise _bad("values and scales must be torch tensors on one GPU")
         if values.dtype not in (torch.float8_e4m3fn, torch.uint8) or values.dim() != 2 or scales.dtype != torch.float32:
             raise _bad("values must be a float8_e4m3fn matrix and scales float32")
+        _no_derivative(values, "values")
+        _no_derivative(scales, "scales")
         r, c = values.shape
         kb = -(-c // 128)
         if tuple(scales.shape) != ((-(-r // 128) if tiles else r), kb):
@@ -126,7 +128,7 @@ class Quantized:
         v[:, :c].copy_(values.view(torch.uint8))
         if c < self._ldv:
             v[:, c:].zero_()
-        self.scales.copy_(scales)
+        self.scales.copy_(scales.detach())
 
     def _make(self, r, c, tiles, device):
         # one allocation: r rows of whole blocks, then the scales block by block (kb x r, or kb x tiles)

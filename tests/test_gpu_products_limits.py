@@ -305,3 +305,18 @@ def test_forward_mode_tangents_are_refused(P):
                 f()
         P.quantize(x), P.orthogonalize(x)  # a tensor without one is taken inside a level, too
         P.quantize(fwAD.unpack_dual(d).primal)
+
+
+def test_quantized_refuses_a_gradient_it_does_not_record(P):
+    import torch.autograd.forward_ad as fwAD
+
+    v, s = P.quantize(randn(62, 6, 200)).values, torch.ones(6, 2, device="cuda", requires_grad=True)
+    with pytest.raises(P.NMFkError, match="detach"):
+        P.Quantized(v, s)
+    P.Quantized(v, s.detach())
+    with torch.no_grad():
+        q = P.Quantized(v, s)
+    assert not q.scales.requires_grad
+    with fwAD.dual_level():
+        with pytest.raises(P.NMFkError, match="tangent"):
+            P.Quantized(v, fwAD.make_dual(s.detach(), torch.ones_like(s)))
