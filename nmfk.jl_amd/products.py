@@ -278,8 +278,11 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
         _output(out, ndim=0)
         if out.shape != G.shape or out.dtype != G.dtype or out.device != G.device:
             raise _bad("out must have G's shape, type and GPU")
-        if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
-            raise _bad("out must have a place for every entry")
+        reach = 0  # of the dimensions with shorter strides
+        for st, n in sorted((st, n) for st, n in zip(out.stride(), out.shape) if n > 1):
+            if st <= reach:
+                raise _bad("out must have a place for every entry, apart from the others")
+            reach += st * (n - 1)
         if out.numel() and not (out.data_ptr() == G.data_ptr() and out.stride() == G.stride()):
             (a0, a1), (b0, b1) = _extent(out), _extent(G)
             if a0 < b1 and b0 < a1:

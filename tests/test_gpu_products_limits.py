@@ -320,3 +320,20 @@ def test_quantized_refuses_a_gradient_it_does_not_record(P):
     with fwAD.dual_level():
         with pytest.raises(P.NMFkError, match="tangent"):
             P.Quantized(v, fwAD.make_dual(s.detach(), torch.ones_like(s)))
+
+
+def test_outputs_whose_entries_share_memory_are_refused(P):
+    base = torch.zeros(1000, device="cuda")
+    g = randn(63, 5, 8)
+    for shape, strides in (((5, 8), (1, 1)), ((5, 8), (4, 1)), ((5, 8), (1, 3)), ((3, 5, 8), (8, 8, 1)), ((3, 5, 8), (39, 8, 1)), ((2, 3, 5, 8), (40, 40, 8, 1)), ((5, 8), (0, 1)),
+                           ((3, 5, 8), (7, 35, 1))):
+        out = base.as_strided(shape, strides)
+        with pytest.raises(P.NMFkError, match="place for every entry"):
+            P.orthogonalize(g.expand(shape).contiguous(), out=out)
+        with pytest.raises(P.NMFkError, match="place for every entry"):
+            P.orthogonalize(out, out=out)
+    for shape, strides in (((5, 8), (8, 1)), ((5, 8), (1, 5)), ((5, 8), (20, 2)), ((3, 5, 8), (8, 24, 1)), ((3, 5, 8), (1, 24, 3)), ((1, 5, 8), (0, 8, 1)), ((5, 1), (1, 0)), ((3, 1, 8), (16, 16, 2))):
+        out = base.as_strided(shape, strides)
+        gg = randn(64, *shape)
+        assert P.orthogonalize(gg, out=out) is out
+        check_ortho(out, gg)
