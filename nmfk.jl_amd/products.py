@@ -65,6 +65,12 @@ def _output(x, ndim=2):
     return x
 
 
+def _written(out):
+    """tells autograd that a caller's tensor has changed, as torch's own in-place operations do"""
+    if not out.is_inference():
+        _TORCH.autograd.graph.increment_version(out)
+
+
 def _stream(device):
     raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)  # (a tenth of the time that a Stream object takes to make)
     return raw(device.index) if raw else _torch().cuda.current_stream(device).cuda_stream
@@ -203,7 +209,7 @@ def product(A, B, dtype=None, out=None):
     _quantized(B, "B")
     if A.shape[1] != B.shape[1] or A.device != B.device:
         raise _bad(f"A * B' needs rows of one length on one GPU, not {A.shape} on {A.device} and {B.shape} on {B.device}")
-    (m, k), n, dev = A.shape, B.shape[0], A.device
+    (m, k), n, dev, given = A.shape, B.shape[0], A.device, out is not None
     if out is None:
         dtype = dtype or torch.float32
         if dtype not in _TYPES:
@@ -218,6 +224,8 @@ def product(A, B, dtype=None, out=None):
     work = torch.empty(nb, dtype=_U8, device=dev) if nb else None
     _check(_lib.lib().nmfk_product(dev.index, _stream(dev), m, n, k, A._pv, A._ldv, A._ps, A._lds, A.tiles, B._pv, B._ldv, B._ps, B._lds, B.tiles, t,
                                    out.data_ptr(), out.stride(0) if m > 1 else n, work.data_ptr() if nb else None, nb))
+    if given:
+        _written(out)
     return out
 
 
@@ -269,6 +277,7 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
         cf = np.asarray(coefficients, dtype=np.float64)
         key = tuple(cf.tolist()) if cf.ndim == 1 else tuple(map(tuple, cf.tolist())) if cf.ndim == 2 else ()
     cf, cf_at = _coefficients(key, steps)
+    given = out is not None
     if out is None:
         if G.dim() > 3:
             g = G.reshape(math.prod(G.shape[:-2]), *G.shape[-2:])  # (a copy where the leading dimensions do not fold into one)
@@ -304,6 +313,8 @@ def orthogonalize(G, steps=5, coefficients=None, out=None):
     work = torch.empty(nb, dtype=_U8, device=dev) if nb else None
     _check(_lib.lib().nmfk_orthogonalize(dev.index, _stream(dev), _TYPES[G.dtype], b, r, c, g.data_ptr(), *gs, o.data_ptr(), *os,
                                          steps, cf_at, work.data_ptr() if nb else None, nb))
+    if given:
+        _written(out)
     return out
 
 

@@ -337,3 +337,24 @@ def test_outputs_whose_entries_share_memory_are_refused(P):
         gg = randn(64, *shape)
         assert P.orthogonalize(gg, out=out) is out
         check_ortho(out, gg)
+
+
+def test_writing_out_is_a_change_that_autograd_sees(P):
+    x = torch.ones(6, 8, device="cuda", requires_grad=True)
+    a, b = P.quantize(randn(65, 6, 40)), P.quantize(randn(66, 8, 40))
+    for write in (lambda w: P.orthogonalize(w, out=w), lambda w: P.orthogonalize(randn(67, 6, 8), out=w), lambda w: P.product(a, b, out=w)):
+        w = randn(68, 6, 8)
+        y = (x * w).sum()
+        write(w)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        w = randn(69, 6, 8)
+        P.orthogonalize(w, out=w)
+        P.product(a, b, out=w)
+    P.product(a, b, out=w)
+    leaf = torch.ones(6, 8, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        P.product(a, b, out=leaf)
+        P.orthogonalize(leaf, out=leaf)
+    (leaf * 2).sum().backward()
