@@ -1131,11 +1131,14 @@ double peak(double a, double b, double c, double u, int odd) {
   };
   if (!odd) {
     if (c != 0) at(-b / (2 * c));
-  } else if (c != 0) {
+  } else {
+    // a + 3 b x + 5 c x^2 = 0: one root from the sum without cancellation, the other one from the roots' product
     const double disc = 9 * b * b - 20 * a * c;
-    if (disc >= 0) at((-3 * b + sqrt(disc)) / (10 * c)), at((-3 * b - sqrt(disc)) / (10 * c));
-  } else if (b != 0) {
-    at(-a / (3 * b));
+    if (disc >= 0) {
+      const double q = -0.5 * (3 * b + copysign(sqrt(disc), b));
+      if (c != 0) at(q / (5 * c));
+      if (q != 0) at(a / q);
+    }
   }
   return best;
 }
