@@ -6,6 +6,8 @@
 // What bounds it: memory.  An fp32 matrix in both orientations is 4 bytes read and 2 written for each entry, so the entries are read ONCE:
 // a workgroup holds a 128 x 128 tile in registers, has the maxima of its rows, of its columns and of the whole, and writes the tile and
 // its transpose (the latter turned in LDS, so that whole 128-byte lines leave).  65536 x 2048 of fp32 in tiles, both orientations: 141 us, 5.7 TB/s.
+#include <algorithm>
+
 #include "nmfk_matrix.h"
 
 using namespace nmfk_mat;
@@ -213,11 +215,18 @@ __global__ __launch_bounds__(1024) void quant_tile_kernel(QuantArgs a) {
 }
 
 template <typename T>
-void quant_launch(const QuantArgs &a, bool tiles, hipStream_t st) {
+void quant_launch(QuantArgs a, bool tiles, hipStream_t st) {
   const int64_t kb = nmfk_div_up(a.cols, 128), rb = nmfk_div_up(a.rows, 128);
   if (!tiles && !a.tv) {
-    const int64_t blocks = a.rows * kb;
-    quant_rows_kernel<T><<<dim3((unsigned)nmfk_div_up(blocks, 8)), 256, 0, st>>>(a, blocks, kb);
+    // a launch holds fewer than 2^32 threads, 32 for each block
+    const int64_t rows = a.rows, most = ((int64_t)1 << 26) / kb;
+    for (int64_t r = 0; r < rows; r += most) {
+      a.rows = std::min(most, rows - r);
+      quant_rows_kernel<T><<<dim3((unsigned)nmfk_div_up(a.rows * kb, 8)), 256, 0, st>>>(a, a.rows * kb, kb);
+      a.x = (const T *)a.x + a.rows * a.ld;
+      a.v += a.rows * a.ldv;
+      a.s += a.rows;
+    }
   } else if (tiles) {
     quant_tile_kernel<T, true><<<dim3((unsigned)kb, (unsigned)rb), 1024, 0, st>>>(a);
   } else {

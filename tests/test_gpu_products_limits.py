@@ -358,3 +358,25 @@ def test_writing_out_is_a_change_that_autograd_sees(P):
         P.product(a, b, out=leaf)
         P.orthogonalize(leaf, out=leaf)
     (leaf * 2).sum().backward()
+
+
+# ---- sizes beyond what one launch holds -------------------------------------------------------------------------------------------------
+
+def test_quantize_rows_of_more_blocks_than_a_launch_holds(P):
+    """4194304 x 4100 of bf16 (34 GB): 138 million blocks of a row, 32 threads each"""
+    r, c = 1 << 22, 4100
+    x = torch.zeros(r, c, dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, 1000003, 2033600, 2033601, 2033602, r // 2, r - 2, r - 1]
+    rows = randn(71, len(at), c, t=torch.bfloat16)
+    x[at] = rows
+    q = P.quantize(x)
+    assert q.shape == (r, c)
+    got, want = q.values[at], P.quantize(rows)
+    assert torch.equal(got.view(torch.uint8), want.values.view(torch.uint8))
+    assert torch.equal(q.scales[at], want.scales)
+    s = q.scales
+    assert int((s != 2.0 ** -126).sum()) == int((want.scales != 2.0 ** -126).sum())  # every other block: zeros
+    del x
+    v = q._values()
+    for i in range(0, r, 1 << 20):  # (a part at a time: a reduction of bytes takes eight times their memory)
+        assert int((v[i:i + (1 << 20)] != 0).sum()) == int((want._values()[[k for k, a in enumerate(at) if i <= a < i + (1 << 20)]] != 0).sum())
