@@ -395,10 +395,10 @@ __global__ __launch_bounds__(256) void prod_join_kernel(const float *part, int s
 
 template <typename T>
 __global__ __launch_bounds__(256) void prod_zero_kernel(T *y, int64_t m, int64_t n, int64_t ldy) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= m * n) return;
-  const int64_t r = i / n;
-  y[r * ldy + (i - r * n)] = from_f32<T>(0.f);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < m * n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / n;
+    y[r * ldy + (i - r * n)] = from_f32<T>(0.f);
+  }
 }
 
 struct Plan {
@@ -485,7 +485,7 @@ int prod_run(ProdArgs p, const Plan &q, void *work, hipStream_t st) {
   const int64_t mn = (int64_t)p.m * p.n;
   T *y = (T *)p.y;
   if (p.kb == 0) {
-    prod_zero_kernel<T><<<dim3((unsigned)nmfk_div_up(mn, 256)), 256, 0, st>>>(y, p.m, p.n, p.ldy);
+    prod_zero_kernel<T><<<dim3((unsigned)std::min<int64_t>(nmfk_div_up(mn, 256), 1 << 16)), 256, 0, st>>>(y, p.m, p.n, p.ldy);
     return nmfk_launched("nmfk_product");
   }
   p.tiles_m = (int)nmfk_div_up(p.m, q.bm);

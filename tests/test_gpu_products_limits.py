@@ -380,3 +380,13 @@ def test_quantize_rows_of_more_blocks_than_a_launch_holds(P):
     v = q._values()
     for i in range(0, r, 1 << 20):  # (a part at a time: a reduction of bytes takes eight times their memory)
         assert int((v[i:i + (1 << 20)] != 0).sum()) == int((want._values()[[k for k, a in enumerate(at) if i <= a < i + (1 << 20)]] != 0).sum())
+
+
+def test_product_of_no_terms_with_many_outputs(P):
+    """k = 0 gives zeros, also where the outputs are more than the threads that a launch holds"""
+    m, n = 65537, 65600
+    a, b = P.quantize(torch.empty(m, 0, device="cuda")), P.quantize(torch.empty(n, 0, device="cuda"))
+    out = torch.full((m, n + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    y = P.product(a, b, out=out[:, :n])
+    assert int(torch.count_nonzero(y)) == 0
+    assert bool((out[:, n:] == 7.0).all())
