@@ -455,29 +455,37 @@ template <typename F, typename T, bool SPLIT>
 void prod_launch(const ProdArgs &p, const Plan &q, hipStream_t st) {
   if (q.bn <= 32) {
     const dim3 grid((unsigned)nmfk_div_up(p.n, q.bn), (unsigned)q.splits);
+    if constexpr (!SPLIT)  // (32 columns a workgroup: 8192 columns and more, whose workgroups are many)
+      if (q.bn == 32) {
+        if (q.bm == 32)
+          prod_rows_kernel<2, 2, F, T, false><<<grid, 512, 0, st>>>(p);
+        else
+          prod_rows_kernel<4, 2, F, T, false><<<grid, 512, 0, st>>>(p);
+        return;
+      }
     if (q.bm == 16)
       prod_rows_kernel<1, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
-    else if (q.bm == 32 && q.bn == 16)
-      prod_rows_kernel<2, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
     else if (q.bm == 32)
-      prod_rows_kernel<2, 2, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
-    else if (q.bn == 16)
-      prod_rows_kernel<4, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
+      prod_rows_kernel<2, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
     else
-      prod_rows_kernel<4, 2, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
+      prod_rows_kernel<4, 1, F, T, SPLIT><<<grid, 512, 0, st>>>(p);
     return;
   }
-  if constexpr (std::is_same<F, Bytes>::value && !SPLIT)
-    if (q.bn == 256) {
-      prod_tile_side<256, 256, 2, 4, F, T, false>(p, 1, st);
+  if constexpr (!SPLIT) {  // (tiles of 128 x 128 and larger are many: prod_plan splits no sum of theirs)
+    if constexpr (std::is_same<F, Bytes>::value)
+      if (q.bn == 256) {
+        prod_tile_side<256, 256, 2, 4, F, T, false>(p, 1, st);
+        return;
+      }
+    if (q.bn == 128) {
+      prod_tile_side<128, 128, 2, 2, F, T, false>(p, 1, st);
       return;
     }
+  }
   if (q.bm == 64)
     prod_tile_side<64, 64, 1, 2, F, T, SPLIT>(p, q.splits, st);
-  else if (q.bn == 64)
-    prod_tile_side<128, 64, 2, 2, F, T, SPLIT>(p, q.splits, st);
   else
-    prod_tile_side<128, 128, 2, 2, F, T, SPLIT>(p, q.splits, st);
+    prod_tile_side<128, 64, 2, 2, F, T, SPLIT>(p, q.splits, st);
 }
 
 template <typename F, typename T>

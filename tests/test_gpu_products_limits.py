@@ -390,3 +390,93 @@ def test_product_of_no_terms_with_many_outputs(P):
     y = P.product(a, b, out=out[:, :n])
     assert int(torch.count_nonzero(y)) == 0
     assert bool((out[:, n:] == 7.0).all())
+
+
+# ---- every kernel of the large forms ------------------------------------------------------------------------------------------------------
+# Which tiles a size takes is a matter of an estimate; with the one of today: (sides of the Gram matrix, its square, the product onto X; "split": some of
+# the sums are)
+
+@pytest.mark.parametrize("shape,t", [
+    ((2000, 2100), "f32"),     # 128 split, 128 split, 128
+    ((2050, 2150), "f16"),     # the same, one entry more than whole tiles
+    ((4, 1000, 4096), "bf16"),  # 128 split, 128, 128
+    ((2, 1501, 1500), "f32"),  # 128, 128, 128
+    ((4096, 4109), "f32"),     # 128: a whole round and a split rest; 256
+    ((4200, 4001), "bf16"),    # 64 or 128, 256
+    ((3000, 3001), "f32"),     # 64: a whole round and a split rest; 128
+    ((1500, 6000), "f16"),     # 128 split
+    ((16000, 700), "f32"),     # 64 split; 128
+    ((16, 513, 520), "bf16"),  # 64; 128
+    ((97, 16384), "f32"),      # 64 in 64 parts
+])
+def test_orthogonalize_tiles(P, shape, t):
+    g = randn(81, *shape, t=TYPES[t])
+    o = P.orthogonalize(g, steps=3)
+    check_ortho(o, g, 3)
+    assert torch.equal(o, P.orthogonalize(g, steps=3))
+
+
+def test_orthogonalize_large_layouts_of_large_tiles(P):
+    """128 and 256 tiles with the turned layout, an output apart from its surroundings, and in place"""
+    for s, l in ((1500, 1600), (4100, 4200)):
+        g = randn(82, l, s).t()
+        o = P.orthogonalize(g, steps=2)
+        check_ortho(o, g, 2)
+        out = torch.full((s + 3, l + 9), 5.0, device="cuda")
+        P.orthogonalize(g, steps=2, out=out[1:s + 1, 4:l + 4])
+        check_ortho(out[1:s + 1, 4:l + 4], g, 2)
+        out[1:s + 1, 4:l + 4] = 5.0
+        assert bool((out == 5.0).all())
+        inplace = g.clone()
+        P.orthogonalize(inplace, steps=2, out=inplace)
+        check_ortho(inplace, g, 2)
+
+
+@pytest.mark.parametrize("s", [97, 130])
+def test_orthogonalize_more_matrices_than_a_launch_of_the_large_form(P, s):
+    """32768 matrices a launch: the second launch's places in the workspace, and its matrices"""
+    g = torch.randn(32768 + 70, s, s + 1, device="cuda", dtype=torch.bfloat16)
+    g[32768 + 3] = 0
+    o = P.orthogonalize(g, steps=2)
+    pick = [0, 1, 32766, 32767, 32768, 32769, 32768 + 3, 32768 + 69]
+    check_ortho(o[[p for p in pick if p != 32768 + 3]], g[[p for p in pick if p != 32768 + 3]], 2)
+    assert bool((o[32768 + 3] == 0).all())
+    each = P.orthogonalize(g[32768:], steps=2)
+    assert float((each.float() - o[32768:].float()).abs().max()) <= 2.0 ** -7 * float(each.float().abs().max())
+
+
+def test_orthogonalize_far_offsets_of_the_large_form(P):
+    """100 rows of 4098 entries, 4095 apart: the last one more than 2^30 entries from the first, the last matrix more than 2^32 bytes"""
+    big = torch.empty(2, 100, 1 << 24, device="cuda")
+    big.uniform_(-1, 1)
+    v = big[:, :, ::4095]
+    o = P.orthogonalize(v, steps=2)
+    check_ortho(o, v, 2)
+    P.orthogonalize(v, steps=2, out=v)
+    assert torch.equal(v, o) or float((v - o).abs().max()) <= 2.0 ** -18
+    w = big[:, :, 1 << 20::5].mT[:, :2000]  # columns of 100, 2^24 entries apart, rows 5 apart
+    check_ortho(P.orthogonalize(w, steps=2), w, 2)
+
+
+@pytest.mark.parametrize("steps", [14, 20, 32])
+@pytest.mark.parametrize("s,l", [(100, 130), (160, 900), (1200, 1300)])
+def test_large_form_with_many_steps_stays_bounded(P, steps, s, l):
+    """directions that G does not have come back as rounding noise, never beyond the largest value of the steps"""
+    g = spectrum("low rank", s, l)
+    o = P.orthogonalize(g, steps=steps).double()
+    assert bool(torch.isfinite(o).all())
+    top = torch.linalg.eigvalsh((o @ o.t()).cpu())
+    assert float(top[-1]) ** 0.5 <= 1.21
+    u, sv, _ = torch.linalg.svd(g.double().cpu(), full_matrices=False)
+    u = u[:, sv > 1e-3 * sv[0]].cuda()
+    lead = torch.linalg.svdvals((u.t() @ o).cpu())
+    assert float(lead[-1]) >= 0.65  # what is there comes to between 0.68 and 1.21
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 2048, 256), (8192, 8192, 128), (4000, 4100, 300), (3500, 3400, 1000), (20, 9000, 700), (50, 8200, 500), (64, 30000, 130), (40, 8192, 129), (64, 65, 9000)])
+@pytest.mark.parametrize("ta,tb", [(False, True), (False, False), (True, True), (True, False)])
+def test_product_tiles(P, m, n, k, ta, tb):
+    """256 x 256, 128 x 128 and the forms of up to 64 rows with 16 and 32 columns a workgroup"""
+    a, b = P.quantize(randn(m + k, m, k), tiles=ta), P.quantize(randn(n * 3 + k, n, k), tiles=tb)
+    for t in TYPES.values():
+        check_product(P.product(a, b, dtype=t), values64(a), values64(b), t)
