@@ -401,8 +401,9 @@ def test_product_of_no_terms_with_many_outputs(P):
     ((2050, 2150), "f16"),     # the same, one entry more than whole tiles
     ((4, 1000, 4096), "bf16"),  # 128 split, 128, 128
     ((2, 1501, 1500), "f32"),  # 128, 128, 128
-    ((4096, 4109), "f32"),     # 128: a whole round and a split rest; 256
-    ((4200, 4001), "bf16"),    # 64 or 128, 256
+    ((4096, 4109), "f32"),     # 128: a whole round and a split rest; 128
+    ((4090, 4095), "f32"),     # 128: a whole round and a split rest; 256
+    ((6200, 2500), "bf16"),    # 128, 128, 256
     ((3000, 3001), "f32"),     # 64: a whole round and a split rest; 128
     ((1500, 6000), "f16"),     # 128 split
     ((16000, 700), "f32"),     # 64 split; 128
@@ -418,7 +419,7 @@ def test_orthogonalize_tiles(P, shape, t):
 
 def test_orthogonalize_large_layouts_of_large_tiles(P):
     """128 and 256 tiles with the turned layout, an output apart from its surroundings, and in place"""
-    for s, l in ((1500, 1600), (4100, 4200)):
+    for s, l in ((1500, 1600), (3900, 4090)):
         g = randn(82, l, s).t()
         o = P.orthogonalize(g, steps=2)
         check_ortho(o, g, 2)
