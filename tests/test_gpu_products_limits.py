@@ -481,3 +481,26 @@ def test_product_tiles(P, m, n, k, ta, tb):
     a, b = P.quantize(randn(m + k, m, k), tiles=ta), P.quantize(randn(n * 3 + k, n, k), tiles=tb)
     for t in TYPES.values():
         check_product(P.product(a, b, dtype=t), values64(a), values64(b), t)
+
+
+# ---- what the type of a product's result decides ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m", [3, 200])
+def test_product_where_large_terms_cancel(P, m):
+    """448^2 - 448^2 and fourteen terms of 8 in one group of sixteen: fp32 results hold the small ones, 16-bit ones are within 2^-9 of the sum of |terms|"""
+    a, b = torch.zeros(m, 128, device="cuda"), torch.zeros(70, 128, device="cuda")
+    a[:, 0], a[:, 1], a[:, 2:16] = 448.0, -448.0, 2.0
+    b[:, 0], b[:, 1], b[:, 2:16] = 448.0, 448.0, 4.0
+    qa, qb = P.quantize(a), P.quantize(b)
+    assert float(qa.scales.min()) == float(qa.scales.max()) == 1.0
+    mag = 2 * 448.0 ** 2 + 14 * 8
+    y = P.product(qa, qb).double()
+    assert bool(((y - 112).abs() <= (256 + 2 + 3) * U * mag).all())
+    for t in (torch.bfloat16, torch.float16):
+        y = P.product(qa, qb, dtype=t).double()
+        assert bool(((y - 112).abs() <= 2.0 ** -9 * mag).all())
+        exact = P.product(qa, qb).to(t).double()  # as documented: fp32, rounded by the caller
+        assert bool(((exact - 112).abs() <= (256 + 2 + 3) * U * mag + HALF[t] * 128).all())
+    # the same of the backward pass: dA = dY8 * (B'8)'
+    da, _ = P.product_grads(a[:, :70].contiguous(), P.quantize(torch.zeros(5, m, device="cuda")), P.quantize(b[:5, :70].contiguous()), dtype=torch.float32)
+    assert bool(((da.double() - 112).abs() <= (256 + 2 + 3) * U * mag).all())
