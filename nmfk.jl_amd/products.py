@@ -19,17 +19,16 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 # three more of the steps that converge (error^3 in each) make the columns orthonormal to 32 bits
 CONVERGING = (1.875, -1.25, 0.375)
 
-_TYPES = _U8 = _F8 = _F32 = _UNPACK = _TORCH = None
+_TYPES = _U8 = _F8 = _F32 = _FORWARD = _TORCH = None
 
 
 def _torch():
     """torch, imported when the first of these operators is called (the rest of the package does without)"""
-    global _TYPES, _U8, _F8, _F32, _UNPACK, _TORCH
+    global _TYPES, _U8, _F8, _F32, _FORWARD, _TORCH
     if _TORCH is None:
         import torch
-        from torch.autograd.forward_ad import unpack_dual
 
-        _UNPACK = unpack_dual
+        _FORWARD = torch.autograd.forward_ad
         _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
         _U8, _F8, _F32, _TORCH = torch.uint8, torch.float8_e4m3fn, torch.float32, torch
     return _TORCH
@@ -42,7 +41,7 @@ def _bad(msg):
 def _no_derivative(x, name):
     if x.requires_grad and _TORCH.is_grad_enabled():
         raise _bad(f"{name} requires a gradient, which this operator does not record: pass {name}.detach()")
-    if _UNPACK(x).tangent is not None:
+    if getattr(_FORWARD, "_current_level", 0) >= 0 and _FORWARD.unpack_dual(x).tangent is not None:
         raise _bad(f"{name} carries a forward-mode tangent, which this operator does not record: pass the primal of torch.autograd.forward_ad.unpack_dual({name})")
 
 
@@ -55,7 +54,7 @@ def _tensor(x, name, ndim=2):
     if ndim and x.dim() != ndim:
         raise _bad(f"{name} must be a matrix")
     _no_derivative(x, name)
-    return x.resolve_neg()  # (itself, unless its entries are the negative of what its memory holds)
+    return x.resolve_neg() if x.is_neg() else x  # (is_neg: its entries are the negative of what its memory holds)
 
 
 def _output(x, ndim=2):
