@@ -504,3 +504,19 @@ def test_product_where_large_terms_cancel(P, m):
     # the same of the backward pass: dA = dY8 * (B'8)'
     da, _ = P.product_grads(a[:, :70].contiguous(), P.quantize(torch.zeros(5, m, device="cuda")), P.quantize(b[:5, :70].contiguous()), dtype=torch.float32)
     assert bool(((da.double() - 112).abs() <= (256 + 2 + 3) * U * mag).all())
+
+
+# ---- rangebasis: matrices without, or of few, directions, and of any size -----------------------------------------------------------------
+
+@pytest.mark.parametrize("n,m,k", [(300, 120, 8), (3000, 1200, 88), (200, 120, 100), (1, 50, 1), (700, 1, 1), (1, 1, 1)])
+@pytest.mark.parametrize("kind", ["zeros", "one entry", "ones"])
+def test_rangebasis_of_few_directions(P, n, m, k, kind):
+    X = torch.ones(n, m, device="cuda") if kind == "ones" else torch.zeros(n, m, device="cuda")
+    if kind == "one entry":
+        X[n // 2, m // 3] = -3.0
+    Q, B, sigma = P.rangebasis(X, k)
+    top = {"zeros": 0.0, "one entry": 3.0, "ones": (n * m) ** 0.5}[kind]
+    assert Q.shape == (n, k) and B.shape == (k, m) and bool(torch.isfinite(Q).all()) and bool(torch.isfinite(B).all())
+    assert abs(float(sigma[0]) - top) <= 1e-5 * top
+    assert float(sigma[1:].sum()) <= 2.0 ** -4 * k * top
+    assert float((Q.double() @ B.double() - X.double()).norm()) <= 1e-4 * top
