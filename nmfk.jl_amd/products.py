@@ -338,8 +338,15 @@ def rangebasis(X, k, oversample=8, iterations=2, seed=0, device=None):
     k = int(k)
     if not 1 <= k <= min(n, m):
         raise _bad(f"k must be between 1 and {min(n, m)}")
-    if not bool(torch.isfinite(X).all()):
+    low, high = (float(x) for x in torch.aminmax(X))
+    top = max(-low, high)
+    if not math.isfinite(top):
         raise _bad("X must be finite (no missing data)")
+    e = math.frexp(top)[1]
+    if abs(e) <= 40:
+        e = 0
+    else:  # far from 1: a copy by a power of two, so that neither the products nor the scales leave the range of fp32
+        X = X.float() * 2.0 ** (-e // 2) * 2.0 ** (-e - -e // 2)
     r = min(k + max(0, int(oversample)), n, m)
     X8, Xt8 = quantize(X, tiles=True, both=True)
     g = torch.Generator(device=X.device)
@@ -357,6 +364,6 @@ def rangebasis(X, k, oversample=8, iterations=2, seed=0, device=None):
     # the singular vectors of B from its r x r Gram matrix, in 64 bits: what the squares lose is below 1e-8 of the largest one, far below the noise of 8 bits
     # (an SVD of B itself does not converge on matrices of zeros)
     U = torch.linalg.eigh(B @ B.t())[1].flip(1)[:, :k]
-    Q, B = (Q.double() @ U).float(), U.t() @ B
+    Q, B = (Q.double() @ U).float(), U.t() @ B * 2.0 ** e
     sigma, B = torch.linalg.vector_norm(B, dim=1).float(), B.float()
     return tuple(x.cpu().numpy() for x in (Q, B, sigma)) if host else (Q, B, sigma)

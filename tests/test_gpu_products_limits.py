@@ -520,3 +520,38 @@ def test_rangebasis_of_few_directions(P, n, m, k, kind):
     assert abs(float(sigma[0]) - top) <= 1e-5 * top
     assert float(sigma[1:].sum()) <= 2.0 ** -4 * k * top
     assert float((Q.double() @ B.double() - X.double()).norm()) <= 1e-4 * top
+
+
+@pytest.mark.parametrize("e", [-125, -100, -45, 45, 100, 119])
+def test_rangebasis_of_any_size(P, e):
+    """scaling X by a power of two scales B and sigma, and changes no bit of Q"""
+    gen = torch.Generator().manual_seed(9)
+    X = (torch.rand(400, 3, generator=gen) @ torch.rand(3, 250, generator=gen) + 0.01 * torch.rand(400, 250, generator=gen)).cuda()
+    X[X < 2.0 ** -8] = 2.0 ** -8  # (no entry becomes subnormal at 2^-125 but for its last bits)
+    X = (X * 2.0 ** 14).round() * 2.0 ** -14
+    if e == 119:
+        X = X[:20, :10].contiguous()  # its singular values fit into fp32
+    Q, B, sigma = P.rangebasis(X, 4)
+    scaled = X * 2.0 ** (e // 2) * 2.0 ** (e - e // 2)
+    for t in (torch.float32, torch.bfloat16) if e > -125 else (torch.float32,):  # (bf16 has no room for the last bits at 2^-125)
+        x, y = (X, scaled) if t == torch.float32 else (X.to(t), (X.to(t).float() * 2.0 ** (e // 2) * 2.0 ** (e - e // 2)).to(t))
+        (q0, b0, s0), (q1, b1, s1) = P.rangebasis(x, 4), P.rangebasis(y, 4)
+        back = lambda v: v.double() * 2.0 ** -e
+        assert torch.equal(q0, q1)
+        assert float((back(s1) - s0.double()).abs().max()) <= 2.0 ** -20 * float(s0[0])
+        assert float((back(b1) - b0.double()).abs().max()) <= 2.0 ** -20 * float(s0[0])
+    assert float((scaled.double() - Q.double() @ B.double() * 2.0 ** e).norm()) <= 2.0 ** e * 2.0 ** -4 * float(X.norm())
+
+
+@pytest.mark.parametrize("size", [3e38, 1e38, 2.0 ** -126, 2.0 ** -149])
+@pytest.mark.parametrize("r,c", [(1, 1), (2, 2), (40, 30)])
+def test_rangebasis_of_the_largest_and_smallest_entries(P, size, r, c):
+    X = torch.zeros(r, c, device="cuda")
+    X[0, 0] = -size
+    X[-1, -1] = size
+    rank = 1 if r == c == 1 else 2
+    Q, B, sigma = P.rangebasis(X, rank)
+    want = float(X[-1, -1])
+    assert float((sigma.double() - want).abs().max()) <= 1e-5 * want
+    # (an entry of B is rounded to a multiple of 2^-149: off by 2^-150 at most, `rank` of them in an entry of Q B)
+    assert float((Q.double() @ B.double() - X.double()).abs().max()) <= 1e-4 * want + rank * 2.0 ** -150
