@@ -89,9 +89,8 @@ __device__ __forceinline__ void read4(const T *p, float (&out)[4]) {
 }
 template <typename T>
 __device__ __forceinline__ void write4(T *p, float a, float b, float c, float d) {
-  struct __attribute__((packed, aligned(sizeof(T)))) raw {
-    uint32_t w[sizeof(T)];
-  };
+  // (a vector, not a struct: the compiler would share a struct's last entry with the branch that stores entry by entry, and store in two pieces)
+  typedef uint32_t raw __attribute__((ext_vector_type(sizeof(T)), aligned(sizeof(T))));
   *(raw *)p = __builtin_bit_cast(raw, (vec4<T>{from_f32<T>(a), from_f32<T>(b), from_f32<T>(c), from_f32<T>(d)}));
 }
 
