@@ -377,7 +377,7 @@ __device__ __forceinline__ f32x4 small_multiply(float a, float b, f32x4 c) { ret
 __device__ __forceinline__ f64x4 small_multiply(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 
 template <typename T, typename O, typename A, int TT, bool WIDE>
-__global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(SmallArgs a, Coefs cf) {
+__global__ __launch_bounds__(256, TT == 1 ? 4 : (std::is_same<A, double>::value && (TT < 4 || !WIDE) ? 2 : 1)) void small_apply_kernel(SmallArgs a, Coefs cf) {
   constexpr bool Q64 = std::is_same<A, double>::value, LDS = Q64 && TT > 1;
   using vec = typename std::conditional<Q64, f64x4, f32x4>::type;
   __shared__ double sum[TT == 1 ? 256 : 1];
@@ -391,17 +391,23 @@ __global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(Small
   O *o = (O *)a.o.p + by * a.o.batch;
   constexpr int U = WIDE ? 4 : TT == 1 ? 4 : TT == 2 ? 2 : 1, SPAN = 16 * U;  // columns a wave takes at a time
   float x[WIDE ? TT : U][WIDE ? 4 : TT][4];
+  // the strides as the compiler cannot know them from the round before: it would keep the addresses of all entries in registers otherwise
+  auto afresh = [](Strided v) {
+    asm volatile("" : "+s"(v.row), "+s"(v.col));
+    return v;
+  };
   auto load = [&](int64_t base) {
+    const Strided from = afresh(a.g);
     if (WIDE) {
 #pragma unroll
       for (int k = 0; k < TT; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) small_load4<T, true>(a.g, p, s, l1, a.gvec, 16 * k + 4 * g + r, base + 4 * c, x[k][r]);
+        for (int r = 0; r < 4; ++r) small_load4<T, true>(from, p, s, l1, a.gvec, 16 * k + 4 * g + r, base + 4 * c, x[k][r]);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int k = 0; k < TT; ++k) small_load4<T, false>(a.g, p, s, l1, a.gvec, 16 * k + 4 * g, base + 16 * u + c, x[u][k]);
+        for (int k = 0; k < TT; ++k) small_load4<T, false>(from, p, s, l1, a.gvec, 16 * k + 4 * g, base + 16 * u + c, x[u][k]);
     }
   };
   const int64_t base0 = l0 + (int64_t)w * SPAN;
@@ -485,35 +491,36 @@ __global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(Small
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[i][k][e] = ldexpf(x[i][k][e], ex);
   };
+  Strided to = a.o;
   auto store_wide = [&](int row, int64_t j, float v0, float v1, float v2, float v3) {  // entries j .. j + 3 of a row
     if (row >= s) return;
-    O *z = o + row * a.o.row + j * a.o.col;
+    O *z = o + row * to.row + j * to.col;
     if (a.ovec && j + 4 <= l1) {
       write4(z, v0, v1, v2, v3);
     } else {
       const float v[4] = {v0, v1, v2, v3};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (j + e < l1) z[e * a.o.col] = from_f32<O>(v[e]);
+        if (j + e < l1) z[e * to.col] = from_f32<O>(v[e]);
     }
   };
   auto store_tall = [&](int row, int64_t j, const vec &v) {  // entries row .. row + 3 of a column
-    O *z = o + row * a.o.row + j * a.o.col;
+    O *z = o + row * to.row + j * to.col;
     if (a.ovec && row + 4 <= s) {
       write4(z, (float)v[0], (float)v[1], (float)v[2], (float)v[3]);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (row + r < s) z[r * a.o.row] = from_f32<O>((float)v[r]);
+        if (row + r < s) z[r * to.row] = from_f32<O>((float)v[r]);
     }
   };
   for (int64_t base = base0; base < l1; base += 4 * SPAN) {
     if (TT > 1) load(base);
+    to = afresh(a.o);
     if (!Q64 && ex) scale();
     if constexpr (LDS) asm volatile("" ::: "memory");  // Q is read in every round: it would not fit into the registers
     if constexpr (WIDE && LDS) {
-      // a column of the lane's four at a time, all rows: four instructions' results more would not fit into the registers
-      float y[TT][4][4];
+      // a column of the lane's four at a time, all rows: O's entries take the places of G's, whose column is no longer needed
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         vec d[TT];
@@ -530,14 +537,14 @@ __global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(Small
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[i][r][e] = (float)d[i][r];
+          for (int r = 0; r < 4; ++r) x[i][r][e] = (float)d[i][r];
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int i = 0; i < TT; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) store_wide(16 * i + 4 * g + r, base + 4 * c, y[i][r][0], y[i][r][1], y[i][r][2], y[i][r][3]);
+        for (int r = 0; r < 4; ++r) store_wide(16 * i + 4 * g + r, base + 4 * c, x[i][r][0], x[i][r][1], x[i][r][2], x[i][r][3]);
     } else if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
@@ -553,6 +560,7 @@ __global__ __launch_bounds__(256, TT == 1 ? 4 : 1) void small_apply_kernel(Small
         if (TT == 1) load(base + 4 * SPAN);
 #pragma unroll
         for (int r = 0; r < 4; ++r) store_wide(16 * i + 4 * g + r, base + 4 * c, (float)d[0][r], (float)d[1][r], (float)d[2][r], (float)d[3][r]);
+        if (TT > 1) __builtin_amdgcn_sched_barrier(0);  // (rows of tiles one after the other: all at once take twice the registers)
       }
     } else {
       vec d[U][TT];
