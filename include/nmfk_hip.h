@@ -279,7 +279,12 @@ int nmfk_quantize(int device, void *stream, int dtype, const void *X, int64_t ro
                   int64_t ldtv, float *tscales, int64_t ldts);
 
 /* Y = A * B' (m x n, entry (i, j) at Y[i * ldy + j]) of two matrices in 8 bits, A m x k and B n x k, as nmfk_quantize lays them out:
- * Y[i, j] = sum over blocks b of sA[i, b] * sB[j, b] * sum of the block's a[i, t] * b[j, t], summed in fp32, rounded once to `dtype`.
+ * Y[i, j] = sum over blocks b of sA[i, b] * sB[j, b] * sum of the block's a[i, t] * b[j, t], rounded once to `dtype`.  `dtype` decides the arithmetic,
+ * too: NMFK_F32 sums in fp32 throughout (an entry is off by at most (2 * 128 + 2 blocks + 3) * 2^-24 of the sum of its |terms|).  NMFK_BF16 and
+ * NMFK_F16 take the 8-bit matrix instruction at twice the rate, which adds 16 products at a time and drops what lies more than 13 bits below the
+ * largest of them: at most 2^-9 of the sum of the |terms| more for an entry, 1.4e-5 of the norm on normal entries (below a tenth of such a result's own
+ * rounding).  Where large terms cancel and what they leave counts, ask for NMFK_F32.  sA * sB is formed in fp32: blocks whose product of scales is below
+ * 2^-126 (entries of A times entries of B below about 2^-108) lose bits, and one above 2^128 gives infinities or NaN.
  * m, n, k: at most 2^22; lda, ldb: at most 2^23.  k = 0 gives zeros.  The result does not depend on the run (no atomics).  nmfk_product_workspace: bytes of `work` for these sizes and this type of Y. */
 int nmfk_product_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes);
 int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, const uint8_t *A, int64_t lda, const float *sA,
@@ -287,7 +292,7 @@ int nmfk_product(int device, void *stream, int64_t m, int64_t n, int64_t k, cons
                  void *Y, int64_t ldy, void *work, int64_t work_bytes);
 
 /* The backward pass of Y = A * B' in one call: dY (m x n, entry (i, j) at dY[i * row_stride + j * col_stride], one of the strides 1) and its
- * transpose are quantized by rows, then dA (m x k) = dY8 * (B'8)' and dB (n x k) = dY'8 * (A'8)'.  At (k x m) and Bt (k x n) are the
+ * transpose are quantized by rows, then dA (m x k) = dY8 * (B'8)' and dB (n x k) = dY'8 * (A'8)', each as nmfk_product computes it for `dtype`.  At (k x m) and Bt (k x n) are the
  * transposes of A and B as nmfk_quantize leaves them (tvalues, tscales).  dA, dB and the other operands must not overlap. */
 int nmfk_product_grads_workspace(int64_t m, int64_t n, int64_t k, int dtype, int64_t *bytes);
 int nmfk_product_grads(int device, void *stream, int64_t m, int64_t n, int64_t k, int dy_dtype, const void *dY, int64_t row_stride,
@@ -297,11 +302,13 @@ int nmfk_product_grads(int device, void *stream, int64_t m, int64_t n, int64_t k
 
 /* The orthogonal factor of each of `batch` matrices G (rows x cols) by Newton-Schulz products: X = G / |G|_F, then for every step, with
  * its three coefficients (a, b, c), X <- a X + (b S + c S S) X where S = X X' (rows <= cols; otherwise of the transpose).  Singular values
- * go towards one (which ones and how close is the coefficients' doing), singular vectors stay.  Accuracy of fp32 or better inside.
+ * go towards one (which ones and how close is the coefficients' doing), singular vectors stay.  Accuracy of fp32 inside: an error of 2^-24 of X in a
+ * step, which the steps behind it raise like any part of X (directions that G does not have come back as such noise, by a factor of at most a for
+ * each step).  Shorter sides up to 96 have better: S in 64 bits and X rounded once in about six of the usual steps.
  * A matrix of zeros gives zeros; one with an entry that is not finite gives NaN everywhere.
  *  G, O       entry (i, j) of matrix r at G[r * g_batch + i * g_row + j * g_col]; O likewise: G itself with the same strides, or not overlapping it
  *  coefficients   3 * steps doubles on the HOST (1 to 32 steps), read before the call returns; refused when they let a singular value grow beyond 64
- * The shorter side is at most 32768, the entries of all matrices together 2^38. */
+ * The shorter side is at most 32768, the entries of all matrices together 2^38.  The workspace does for every type and number of steps. */
 int nmfk_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int64_t *bytes);
 int nmfk_orthogonalize(int device, void *stream, int dtype, int64_t batch, int64_t rows, int64_t cols, const void *G,
                        int64_t g_batch, int64_t g_row, int64_t g_col, void *O, int64_t o_batch, int64_t o_row, int64_t o_col,

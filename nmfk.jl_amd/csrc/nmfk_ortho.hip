@@ -7,8 +7,8 @@
 //
 //   s <= 96: the polynomials of several steps are polynomials of their first S.  One pass over X makes S in 64 bits, one workgroup per matrix
 //     iterates on s x s matrices in LDS in 64 bits (S <- P S P, Q <- Q P), a second pass applies Q.  Two reads and a write of G.  (Five steps on
-//     90 x 20000: 133 us, the other form 194; 60 of 96 x 3000: 245 and 488; one of 96 x 96, where the iteration is all there is: 118 and 105.
-//     Beyond, three matrices do not fit into LDS.)
+//     90 x 20000: 131 us, the other form 192; 60 of 96 x 3000: 234 and 465; one of 96 x 96, where the iteration is all there is: 114 and 105.  Fourteen:
+//     359 and 493, 647 and 1220, 315 and 279.  Beyond, three matrices do not fit into LDS.)
 //     What is iterated is not X: a rounding error e = 2^-53 in an eigenvalue of S near zero, which may make it negative, grows by growth^2 (growth: the
 //     product of the steps' largest a + b S + c S S), and from some 1e-2 on it takes over -- where rows of G depend on each other, the default steps leave
 //     the right place after 12 steps and every bound after 16.  So the steps are taken in groups of growth up to 2048 (5e-10), X is formed after
@@ -368,11 +368,11 @@ __global__ __launch_bounds__(64 * small_waves(TT)) void small_iterate_kernel(Sma
 // O = Q G over a chunk of l, on the fp32 matrix pipe (16 x 16 x 4: entry [c][.] of the first, [.][c] of the second operand in lane 16 g + c, result
 // [4 g + r][c] in register r) or on the fp64 one.  Which four of the sum's entries a step takes is free: a lane's four consecutive entries of G or of Q
 // serve four steps, or four columns, and its four results stand next to each other in O.  s <= 16: every workgroup iterates for itself, a wave in registers
-// (about 2 microseconds, less than a launch), while the first entries of G are on their way.  480 of 8192 x 16 in fp32: 90 us, 5.6 TB/s.
+// (about 2 microseconds, less than a launch), while the first entries of G are on their way.  480 of 8192 x 16 in fp32: 86 us, 5.9 TB/s.
 //
 // A = float: Q in registers, rounded to 32 bits, which puts an error of growth * 2^-24 |G| into O like the same steps in fp32 would.  A = double where that is
 // too much: O is off by its own rounding (to fp32, then to its type).  Q stands in LDS, which is quick enough for an instruction of 64 cycles.  60 of 96 x 3000:
-// 75 us in 32 bits, 112 in 64.
+// 67 us in 32 bits, 123 in 64.
 __device__ __forceinline__ f32x4 small_multiply(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f64x4 small_multiply(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 

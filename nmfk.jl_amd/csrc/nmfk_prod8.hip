@@ -84,8 +84,8 @@ enum { ROWS_ROWS = 0, B_TILES = 1, A_TILES = 2 };
 // registers, so B's half of a buffer is free after the first row of tiles and A's before the last two: at these two places the waves meet, and
 // the copies of the block after the next start, spread over the rows (all at once: 6 % slower).  The operands of the next block are read while the matrix
 // pipe is still busy with the last row of this one.
-// What bounds it at 8192^3 (256 x 256, 490 .. 540 microseconds, 2.0 .. 2.2 PFLOP/s on different cards): the matrix and vector instructions of a block alone, without
-// any memory, take 413, the additions about 35 of these; the copies add 100.  The same in 32 x 32 x 64 instructions: 7 % slower.
+// What bounds it at 8192^3 (256 x 256, 447 .. 465 microseconds, 2.4 PFLOP/s): the matrix and vector instructions of a block alone, without any memory,
+// take 413, the additions about 35 of these; copies and stores add 40.  The same in 32 x 32 x 64 instructions: 7 % slower.
 // The first operand of the matrix instruction is B, so that a lane's four outputs are neighbours in a row of Y.
 template <int BM, int BN, int WM, int WN, int MODE, typename F, typename T, bool SPLIT>
 __device__ __forceinline__ void prod_tile(const ProdArgs &p, int id, int split) {
