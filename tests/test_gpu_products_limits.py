@@ -130,7 +130,7 @@ STEPS = {"7": [CF] * 7, "10": [CF] * 10, "14": [CF] * 14, "20": [CF] * 20, "32":
 
 @pytest.mark.parametrize("name", SPECTRA)
 @pytest.mark.parametrize("steps", list(STEPS))
-@pytest.mark.parametrize("s,l", [(1, 5), (16, 200), (40, 60), (64, 70), (90, 300), (96, 96)])
+@pytest.mark.parametrize("s,l", [(1, 5), (16, 200), (24, 1100), (40, 60), (64, 70), (72, 130), (90, 300), (96, 96)])
 def test_many_steps(P, name, steps, s, l):
     cf = STEPS[steps]
     g = spectrum(name, s, l)
