@@ -6,11 +6,13 @@
 
 #include "nmfk_ctx.h"
 
-// An entry point works on the device it is told and leaves the calling thread's current device as it was.
+// An entry point works on the device it is told and leaves the calling thread's current device as it was.  An error that another call of the runtime has
+// left behind is not this call's: nmfk_launched would take it for its own.
 struct NmfkDeviceGuard {
   int before = -1, status = 0;
   explicit NmfkDeviceGuard(int device) {
     int count = 0;
+    (void)hipGetLastError();
     hipError_t e = hipGetDevice(&before);
     if (e == hipSuccess && before != device) {
       e = hipGetDeviceCount(&count);

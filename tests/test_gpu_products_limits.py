@@ -555,3 +555,24 @@ def test_rangebasis_of_the_largest_and_smallest_entries(P, size, r, c):
     assert float((sigma.double() - want).abs().max()) <= 1e-5 * want
     # (an entry of B is rounded to a multiple of 2^-149: off by 2^-150 at most, `rank` of them in an entry of Q B)
     assert float((Q.double() @ B.double() - X.double()).abs().max()) <= 1e-4 * want + rank * 2.0 ** -150
+
+
+# ---- errors that are not the call's own ---------------------------------------------------------------------------------------------------
+
+def test_an_error_left_by_another_call_is_not_reported(P):
+    """a refused call of the HIP runtime (here: a device that does not exist) leaves its error behind for whoever asks next"""
+    import ctypes as C
+
+    path = {line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line}
+    hip = C.CDLL(path.pop())
+    x, g, h = randn(91, 40, 300), randn(92, 20, 40), randn(93, 120, 130)
+    want = (P.quantize(x), P.orthogonalize(g), P.orthogonalize(h))
+    q = want[0]
+    y = P.product(q, q)
+    torch.cuda.synchronize()
+    for f, w in ((lambda: P.quantize(x).values.view(torch.uint8), want[0].values.view(torch.uint8)), (lambda: P.orthogonalize(g), want[1]), (lambda: P.orthogonalize(h), want[2]),
+                 (lambda: P.product(q, q), y)):
+        assert hip.hipSetDevice(12345) != 0
+        got = f()
+        hip.hipGetLastError()
+        assert torch.equal(got, w)
